@@ -1,0 +1,562 @@
+// One-token attention over a paged key/value cache, with a prefix that the sequences of a group share.
+//
+//   s_n = scale * q . k_n over the tokens n of the row's group prefix and of its own pages;  m = max s, l = sum exp(s_n - m),
+//   o = sum exp(s_n - m) v_n / l,  lse = m + log l;   a row that sees no token: o = 0, lse = -inf.
+//
+// Work items: (sequence, kv head, 16 of its query heads) over the sequence's own pages, and (group, kv head, 16 of the group's
+// rows x query heads) over the group's prefix, which is therefore read once per 16 rows and not once per sequence.  Items are
+// cut into tiles of 64 keys; the tiles of all items in one row are dealt to the CTAs of one resident wave in equal, contiguous
+// ranges, so that ragged lengths and single long sequences fill the machine alike.  A range that does not hold an item alone
+// leaves (m, l, unnormalised o) in fp32, and a second kernel joins the parts of every row in a fixed order (no atomics: the
+// result does not depend on timing).
+//
+// Inside a CTA each of the four warps walks over its own 16 keys of every tile, with its own ring of asynchronous copies and
+// its own running maximum and sum: no barrier is crossed until the item ends.  Scores and the weighted sum are m16n8k16 tensor
+// core products with the query heads as (padded) rows; the bound is the bytes of the cache, not the products.  Keys behind the
+// length are filled with zeros by the copy and masked by index: what lies in those slots is never read.
+#include "common.cuh"
+#include "paged.h"
+
+namespace seg {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kKeys = 16;               // keys per warp and step
+constexpr int kTile = kWarps * kKeys;   // keys per tile
+constexpr int kRows = 16;               // query rows per item
+constexpr int kThreads = kWarps * 32;
+constexpr int kMaxLists = 8192;         // sequences + groups (their cumulative tile counts live in shared memory)
+
+template <int HD> struct Cfg {
+  static constexpr int kStages = HD == 128 ? 3 : 4;
+  static constexpr int kChunks = HD / 8;                   // 16-byte chunks of a row
+  static constexpr int kStageBytes = 2 * kKeys * HD * 2;   // K and V of one step
+  static constexpr int kRing = kStages * kStageBytes;      // per warp
+};
+
+struct Plan {        // sizes that host and device derive alike
+  int gqa, RT;       // query heads per kv head; 16-row tiles of a sequence's item row
+  int rows_s;        // rows of a part of an own-pages item
+  int items_s, items_p;
+  int ctas;
+};
+
+struct Work {
+  float* acc_s;    // [items_s + ctas, rows_s, HD]
+  float2* ml_s;    // [items_s + ctas, rows_s]
+  float* acc_p;    // [items_p + ctas, 16, HD]
+  float2* ml_p;
+  int2* meta;      // [items_s + items_p] first part and number of parts of every item that has tiles
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float exp2_(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Weight of a part (m, l) under the common maximum mm.  A part without a finite score has m = -inf and l = 0, unless NaN scores
+// made l NaN: then the row becomes NaN, as the formula says.
+__device__ __forceinline__ float part_weight(float m, float l, float mm) { return m == -INFINITY ? l : exp2_(m - mm); }
+__device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f; }
+// Byte offset of 16-byte chunk c of row r in a [rows][HD] bf16 tile; the chunks of neighbouring rows are permuted so that the
+// eight rows that one ldmatrix phase reads fall on eight different bank groups.
+template <int HD> __device__ __forceinline__ uint32_t swz(int r, int c) {
+  if (HD == 32) return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+  return r * (HD * 2) + ((c ^ (r & 7)) << 4);
+}
+
+__device__ __forceinline__ int clamp_len(int n, int width, int P, int* status) {
+  const int64_t cap = (int64_t)width * P;
+  if (n >= 0 && n <= cap) return n;
+  atomicCAS(status, 0, kStatusAttnLength);
+  return n < 0 ? 0 : (int)cap;
+}
+struct Group {
+  int r0, r1, len;
+};
+__device__ __forceinline__ Group load_group(const PagedAttnParams& p, int g) {
+  Group w;
+  w.r0 = p.groups != nullptr ? p.groups[g] : 0;
+  w.r1 = p.groups != nullptr ? p.groups[g + 1] : p.B;
+  if (w.r0 < 0 || w.r1 < w.r0 || w.r1 > p.B) {
+    atomicCAS(p.status, 0, kStatusAttnGroups);
+    w.r0 = w.r1 = 0;
+  }
+  w.len = w.r1 > w.r0 ? clamp_len(p.plens[g], p.ptable_width, p.pool.P, p.status) : 0;
+  return w;
+}
+__device__ __forceinline__ int row_tiles(const Group& g, int gqa) { return ((g.r1 - g.r0) * gqa + kRows - 1) / kRows; }
+// First item of a group's prefix: leaves room for the row tiles of the groups before it, whatever their sizes.
+__device__ __forceinline__ int first_item(const Plan& n, const PagedAttnParams& p, int g, int r0) {
+  return n.items_s + p.Hkv * (r0 * n.gqa / kRows + g);
+}
+
+// sum[i + 1] = tiles of the first i + 1 lists; all threads take part
+template <typename F>
+__device__ void scan_tiles(int* sum, int n, F tiles, int* warp_tot) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int carry = 0;
+  if (threadIdx.x == 0) sum[0] = 0;
+  for (int base = 0; base < n; base += kThreads) {
+    const int i = base + threadIdx.x;
+    int v = i < n ? tiles(i) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) warp_tot[warp] = v;
+    __syncthreads();
+    int add = carry;
+    for (int w = 0; w < warp; ++w) add += warp_tot[w];
+    if (i < n) sum[i + 1] = v + add;
+    for (int w = 0; w < kWarps; ++w) carry += warp_tot[w];
+    __syncthreads();
+  }
+}
+// last i with sum[i] <= t (t < sum[n]); empty lists are passed over
+__device__ __forceinline__ int find_list(const int* sum, int n, int t) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (sum[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// Addresses of one walk's keys: a list of pages and the kv head inside them.
+struct KeyWalk {
+  const int* pages;
+  const __nv_bfloat16 *k, *v;  // pools at the item's kv head
+  int len;
+};
+
+template <int HD>
+__device__ __forceinline__ void load_step(const PagedAttnParams& p, const KeyWalk& w, int key0, uint32_t stage) {
+  using C = Cfg<HD>;
+  const int lane = threadIdx.x & 31;
+  constexpr int kRowsPer = 32 / C::kChunks;  // rows that the warp covers at once
+#pragma unroll
+  for (int i = 0; i < kKeys / kRowsPer; ++i) {
+    const int r = i * kRowsPer + lane / C::kChunks, c = lane % C::kChunks;
+    const int key = key0 + r;
+    bool live = key < w.len;
+    int64_t page = 0;
+    int slot = 0;
+    if (live) {
+      const int j = p.pool.shift >= 0 ? key >> p.pool.shift : key / p.pool.P;
+      slot = key - j * p.pool.P;
+      page = __ldg(w.pages + j);
+      if ((uint64_t)page >= (uint64_t)p.pool.n_pages) {
+        atomicCAS(p.status, 0, kStatusAttnPage);
+        live = false;
+        page = 0;
+        slot = 0;
+      }
+    }
+    copy16(stage + swz<HD>(r, c), w.k + page * p.pool.k_page + slot * p.pool.k_slot + c * 8, live);
+    copy16(stage + kKeys * HD * 2 + swz<HD>(r, c), w.v + page * p.pool.v_page + slot * p.pool.v_slot + c * 8, live);
+  }
+}
+
+// kHalf: at most eight of the item's sixteen rows exist; the products' upper rows are zero and their softmax is left out.
+template <int HD, bool kHalf>
+__device__ __forceinline__ void walk(const PagedAttnParams& p, const KeyWalk& w, const uint32_t (*qf)[4], int key0, int steps, uint32_t ring, float (*o)[4],
+                                     float* m, float* l) {
+  using C = Cfg<HD>;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int s = 0; s < C::kStages - 1; ++s) {
+    if (s < steps) load_step<HD>(p, w, key0 + s * kTile, ring + s * C::kStageBytes);
+    copy_commit();
+  }
+  for (int s = 0; s < steps; ++s) {
+    copy_wait<C::kStages - 2>();
+    __syncwarp();
+    const int ahead = s + C::kStages - 1;
+    if (ahead < steps) load_step<HD>(p, w, key0 + ahead * kTile, ring + (ahead % C::kStages) * C::kStageBytes);
+    copy_commit();
+    const uint32_t sk = ring + (s % C::kStages) * C::kStageBytes, sv = sk + kKeys * HD * 2;
+    float sc[2][4] = {};
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk) {
+      uint32_t b[4];
+      ldsm4(b, sk + swz<HD>((lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
+      mma(sc[0], qf[kk], b[0], b[1]);
+      mma(sc[1], qf[kk], b[2], b[3]);
+    }
+    // scaled before the mask and the maximum: the scale may be zero or negative
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < (kHalf ? 2 : 4); ++e) sc[n][e] *= p.scale_log2;
+    const int left = w.len - (key0 + s * kTile);  // keys of this step that exist
+    if (left < kKeys) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n * 8 + (lane & 3) * 2 + (e & 1) >= left) sc[n][e] = -INFINITY;
+    }
+    uint32_t pf[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (kHalf && h == 1) {
+        pf[1] = pf[3] = 0u;
+        continue;
+      }
+      float mx = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float m_new = fmaxf(m[h], mx);
+      if (__any_sync(0xffffffffu, m_new > m[h])) {
+        const float a = m_new == -INFINITY ? 1.f : exp2_(m[h] - m_new);
+        l[h] *= a;
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d) {
+          o[d][2 * h] *= a;
+          o[d][2 * h + 1] *= a;
+        }
+        m[h] = m_new;
+      }
+      const float base = m_new == -INFINITY ? 0.f : m_new;  // nothing seen yet: every score is -inf and its weight exp2(-inf) = 0
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = exp2_(sc[i >> 1][2 * h + (i & 1)] - base);
+      l[h] += (e[0] + e[1]) + (e[2] + e[3]);
+      pf[h] = pack_bf16(e[0], e[1]);      // weights <= 1 rounded to bf16 (2^-9 relative), as operands of the tensor core
+      pf[2 + h] = pack_bf16(e[2], e[3]);
+    }
+#pragma unroll
+    for (int dd = 0; dd < HD / 16; ++dd) {
+      uint32_t b[4];
+      ldsm4t(b, sv + swz<HD>((lane & 7) + ((lane >> 3) & 1) * 8, dd * 2 + (lane >> 4)));
+      mma(o[2 * dd], pf, b[0], b[1]);
+      mma(o[2 * dd + 1], pf, b[2], b[3]);
+    }
+    __syncwarp();
+  }
+  copy_wait<0>();
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnParams p, const Plan n, const Work ws) {
+  using C = Cfg<HD>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int warp_tot[kWarps];
+  int* sum_s = reinterpret_cast<int*>(smem + kWarps * C::kRing);
+  int* sum_p = sum_s + p.B + 1;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  scan_tiles(sum_s, p.B, [&](int b) { return (clamp_len(p.lens[b], p.table_width, p.pool.P, p.status) + kTile - 1) / kTile; }, warp_tot);
+  scan_tiles(sum_p, p.G, [&](int g) {
+    const Group w = load_group(p, g);
+    return (w.len + kTile - 1) / kTile * row_tiles(w, n.gqa);
+  }, warp_tot);
+  __syncthreads();
+  const int per_seq = p.Hkv * n.RT;
+  const int64_t tiles_s = (int64_t)sum_s[p.B] * per_seq;
+  const int64_t total = tiles_s + (int64_t)sum_p[p.G] * p.Hkv;
+  const int64_t ctas = min((int64_t)gridDim.x, total);  // every one of them has a tile: the parts of an item have consecutive numbers
+  if (blockIdx.x >= ctas) return;
+  const int64_t t_end = total * (blockIdx.x + 1) / ctas;
+  for (int64_t t = total * blockIdx.x / ctas; t < t_end;) {
+    // ---- the item that tile t belongs to
+    KeyWalk w;
+    int item, kvh, rows, row0, h0, n_tiles, tile0;  // rows r = 0 .. rows-1 are query row row0 + (h0 + r) / gqa, head kvh * gqa + (h0 + r) % gqa
+    const bool own = t < tiles_s;
+    if (own) {
+      const int b = find_list(sum_s, p.B, (int)(t / per_seq));
+      n_tiles = sum_s[b + 1] - sum_s[b];
+      const int local = (int)(t - (int64_t)sum_s[b] * per_seq), i = local / n_tiles;
+      tile0 = local - i * n_tiles;
+      kvh = i / n.RT;
+      h0 = (i - kvh * n.RT) * kRows;
+      item = b * per_seq + i;
+      row0 = b;
+      rows = min(kRows, n.gqa - h0);
+      w.len = clamp_len(p.lens[b], p.table_width, p.pool.P, p.status);
+      w.pages = p.table + b * p.table_stride;
+    } else {
+      const int64_t tp = t - tiles_s;
+      const int g = find_list(sum_p, p.G, (int)(tp / p.Hkv));
+      const Group gr = load_group(p, g);
+      n_tiles = (gr.len + kTile - 1) / kTile;
+      const int local = (int)(tp - (int64_t)sum_p[g] * p.Hkv), i = local / n_tiles;
+      tile0 = local - i * n_tiles;
+      const int rt = row_tiles(gr, n.gqa);
+      kvh = i / rt;
+      h0 = (i - kvh * rt) * kRows;
+      item = first_item(n, p, g, gr.r0) + i;
+      row0 = gr.r0;
+      rows = min(kRows, (gr.r1 - gr.r0) * n.gqa - h0);
+      w.len = gr.len;
+      w.pages = p.ptable + g * p.ptable_stride;
+    }
+    w.k = static_cast<const __nv_bfloat16*>(p.pool.k) + kvh * p.pool.k_head;
+    w.v = static_cast<const __nv_bfloat16*>(p.pool.v) + kvh * p.pool.v_head;
+    const int steps = (int)min(t_end - t, (int64_t)(n_tiles - tile0));
+    const int64_t first_tile = t - tile0;
+    const int cta_first = (int)(((first_tile + 1) * ctas - 1) / total), cta_last = (int)(((first_tile + n_tiles) * ctas - 1) / total);
+    if (tile0 == 0 && threadIdx.x == 0) ws.meta[item] = make_int2((own ? item : item - n.items_s) + cta_first, cta_last - cta_first + 1);
+
+    // ---- queries: the A operand, straight from memory
+    uint32_t qf[HD / 16][4];
+    const __nv_bfloat16* qrow[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = (lane >> 2) + 8 * h, x = h0 + r;
+      qrow[h] = r < rows ? static_cast<const __nv_bfloat16*>(p.q) + (row0 + x / n.gqa) * p.q_row + (kvh * n.gqa + x % n.gqa) * p.q_head : nullptr;
+    }
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat16* src = qrow[e & 1];
+        qf[kk][e] = src != nullptr ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + (lane & 3) * 2 + (e >> 1) * 8) : 0u;
+      }
+
+    // ---- this warp's keys
+    float o[HD / 8][4] = {};
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    uint8_t* ring = smem + warp * C::kRing;
+    const int key0 = tile0 * kTile + warp * kKeys;
+    if (rows <= 8) walk<HD, true>(p, w, qf, key0, steps, smem_addr(ring), o, m, l);
+    else walk<HD, false>(p, w, qf, key0, steps, smem_addr(ring), o, m, l);
+
+    // ---- join the four warps: every warp's (m, l, o) into its own ring, then each thread sums its columns
+    float* part = reinterpret_cast<float*>(ring);                      // [16][HD]
+    float2* part_ml = reinterpret_cast<float2*>(ring + kRows * HD * 4);  // [16]
+    static_assert(kRows * HD * 4 + kRows * 8 <= C::kRing, "a warp's part must fit into its ring");
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = (lane >> 2) + 8 * h;
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if ((lane & 3) == 0) part_ml[r] = make_float2(m[h], l[h]);
+      if (r < rows) {
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(part + r * HD + d * 8 + (lane & 3) * 2) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
+      }
+    }
+    __syncthreads();
+    const bool whole = own && p.G == 0 && steps == n_tiles;
+    const int64_t slot = (own ? item : item - n.items_s) + (int64_t)blockIdx.x;
+    const int slot_rows = own ? n.rows_s : kRows;
+    for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
+      const int r = i / (HD / 4), c = i % (HD / 4) * 4;
+      float mw[kWarps], lw[kWarps], mm = -INFINITY, ll = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) {
+        const float2 ml = reinterpret_cast<const float2*>(smem + v * C::kRing + kRows * HD * 4)[r];
+        mw[v] = ml.x;
+        lw[v] = ml.y;
+        mm = fmaxf(mm, ml.x);
+      }
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) {
+        const float a = part_weight(mw[v], lw[v], mm);
+        ll += a * lw[v];
+        const float4 x = *reinterpret_cast<const float4*>(smem + v * C::kRing + (r * HD + c) * 4);
+        acc.x += a * x.x;
+        acc.y += a * x.y;
+        acc.z += a * x.z;
+        acc.w += a * x.w;
+      }
+      const int x = h0 + r;
+      if (whole) {
+        const int64_t out = (int64_t)(row0 + x / n.gqa) * p.H + kvh * n.gqa + x % n.gqa;
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        store4<__nv_bfloat16>(static_cast<__nv_bfloat16*>(p.o) + out * HD + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        if (c == 0) p.lse[out] = row_lse(mm, ll);
+      } else {
+        float* dst = (own ? ws.acc_s : ws.acc_p) + (slot * slot_rows + r) * HD + c;
+        *reinterpret_cast<float4*>(dst) = acc;
+        if (c == 0) (own ? ws.ml_s : ws.ml_p)[slot * slot_rows + r] = make_float2(mm, ll);
+      }
+    }
+    __syncthreads();
+    t += steps;
+  }
+}
+
+// Joins the parts of one (row, head): the prefix's, then the sequence's own, in order.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const PagedAttnParams p, const Plan n, const Work ws) {
+  __shared__ float4 acc_w[kWarps][HD / 4];
+  __shared__ float2 ml_w[kWarps];
+  const int b = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = h / n.gqa, hl = h - kvh * n.gqa;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int len = clamp_len(p.lens[b], p.table_width, p.pool.P, p.status);
+  int2 parts[2] = {make_int2(0, 0), make_int2(0, 0)};
+  int row_p = 0;
+  if (p.G > 0) {
+    int g = 0;
+    if (p.groups != nullptr) {
+      int hi = p.G;
+      while (hi - g > 1) {
+        const int mid = (g + hi) >> 1;
+        if (p.groups[mid] <= b) g = mid; else hi = mid;
+      }
+    }
+    const Group gr = load_group(p, g);
+    if (gr.len > 0 && b >= gr.r0 && b < gr.r1) {
+      const int x = (b - gr.r0) * n.gqa + hl;
+      parts[0] = ws.meta[first_item(n, p, g, gr.r0) + kvh * row_tiles(gr, n.gqa) + x / kRows];
+      row_p = x % kRows;
+      // out of order group rows could leave an item without its entry
+      if (parts[0].x < 0 || parts[0].y < 0 || (int64_t)parts[0].x + parts[0].y > n.items_p + n.ctas) parts[0] = make_int2(0, 0);
+    }
+  }
+  if (len > 0) {
+    parts[1] = ws.meta[(b * p.Hkv + kvh) * n.RT + hl / kRows];
+    if (p.G == 0 && parts[1].y == 1) return;  // written by the CTA that held the whole item
+  }
+  const int total = parts[0].y + parts[1].y;
+  float m = -INFINITY, l = 0.f;
+  constexpr int kPer = HD / 32;  // columns of a lane
+  float acc[kPer] = {};
+  for (int i = warp; i < total; i += kWarps) {
+    const bool pre = i < parts[0].y;
+    const int64_t at = pre ? (int64_t)(parts[0].x + i) * kRows + row_p : (int64_t)(parts[1].x + i - parts[0].y) * n.rows_s + hl % kRows;
+    const float2 ml = (pre ? ws.ml_p : ws.ml_s)[at];
+    const float* src = (pre ? ws.acc_p : ws.acc_s) + at * HD + lane * kPer;
+    float x[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) x[j] = src[j];
+    if (ml.x == -INFINITY) {
+      l += ml.y;  // 0, or NaN
+      continue;
+    }
+    const float m_new = fmaxf(m, ml.x);
+    const float a = exp2_(m - m_new), c = exp2_(ml.x - m_new);
+    l = l * a + ml.y * c;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) acc[j] = acc[j] * a + x[j] * c;
+    m = m_new;
+  }
+  float* mine = reinterpret_cast<float*>(acc_w[warp]);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) mine[lane * kPer + j] = acc[j];
+  if (lane == 0) ml_w[warp] = make_float2(m, l);
+  __syncthreads();
+  const int c = threadIdx.x;
+  if (c >= HD) return;
+  float mm = -INFINITY, ll = 0.f, out = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml_w[w].x);
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const float a = part_weight(ml_w[w].x, ml_w[w].y, mm);
+    ll += a * ml_w[w].y;
+    out += a * reinterpret_cast<const float*>(acc_w[w])[c];
+  }
+  const int64_t at = (int64_t)b * p.H + h;
+  static_cast<__nv_bfloat16*>(p.o)[at * HD + c] = __float2bfloat16_rn(ll == 0.f ? 0.f : out / ll);
+  if (c == 0) p.lse[at] = row_lse(mm, ll);
+}
+
+template <int HD> int smem_bytes(const PagedAttnParams& p) { return kWarps * Cfg<HD>::kRing + (p.B + p.G + 2) * (int)sizeof(int); }
+
+Plan make_plan(const PagedAttnParams& p) {
+  Plan n;
+  n.gqa = p.H / p.Hkv;
+  n.RT = (n.gqa + kRows - 1) / kRows;
+  n.rows_s = n.gqa < kRows ? n.gqa : kRows;
+  n.items_s = p.B * p.Hkv * n.RT;
+  n.items_p = p.G > 0 ? p.Hkv * (int)((int64_t)p.B * n.gqa / kRows + p.G + 1) : 0;
+  // one resident wave, but no more CTAs than there can be tiles
+  const int per_sm = p.hd == 128 || p.B + p.G > 2048 ? 2 : 3;
+  const int64_t P = p.pool.P;
+  int64_t tiles = (int64_t)n.items_s * ((p.table_width * P + kTile - 1) / kTile);
+  if (p.G > 0) tiles += (int64_t)n.items_p * ((p.ptable_width * P + kTile - 1) / kTile);
+  n.ctas = (int)(tiles < 148 * per_sm ? (tiles < 1 ? 1 : tiles) : 148 * per_sm);
+  return n;
+}
+
+int64_t round_up(int64_t n) { return (n + 255) / 256 * 256; }
+
+template <int HD>
+int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t st) {
+  static bool configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(paged_attn_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * Cfg<HD>::kRing + (kMaxLists + 2) * 4) != cudaSuccess) return -2;
+    configured[dev] = true;
+  }
+  paged_attn_kernel<HD><<<n.ctas, kThreads, smem_bytes<HD>(p), st>>>(p, n, ws);
+  if (cudaGetLastError() != cudaSuccess) return -3;
+  // The join may be brought in while the walk still runs (it waits for its end in griddepcontrol.wait).
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.B, p.H);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<HD>, p, n, ws) == cudaSuccess ? 0 : -3;
+}
+
+}  // namespace
+
+int64_t paged_attn_workspace(const PagedAttnParams& p) {
+  if (p.hd != 32 && p.hd != 64 && p.hd != 128) return -1;
+  if (p.B + p.G > kMaxLists) return -1;
+  const Plan n = make_plan(p);
+  const int64_t ss = ((int64_t)n.items_s + n.ctas) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas) * kRows : 0;
+  return round_up(ss * p.hd * 4) + round_up(ss * 8) + round_up(sp * p.hd * 4) + round_up(sp * 8) + round_up(((int64_t)n.items_s + n.items_p) * 8);
+}
+
+int paged_attn(const PagedAttnParams& p, void* workspace, cudaStream_t st) {
+  if (p.B == 0) return 0;
+  if (p.H < 1 || p.Hkv < 1 || p.H % p.Hkv != 0 || p.H > 65535 || p.B + p.G > kMaxLists) return -10;
+  const Plan n = make_plan(p);
+  const int64_t ss = ((int64_t)n.items_s + n.ctas) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas) * kRows : 0;
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  Work ws;
+  ws.acc_s = reinterpret_cast<float*>(at);
+  at += round_up(ss * p.hd * 4);
+  ws.ml_s = reinterpret_cast<float2*>(at);
+  at += round_up(ss * 8);
+  ws.acc_p = reinterpret_cast<float*>(at);
+  at += round_up(sp * p.hd * 4);
+  ws.ml_p = reinterpret_cast<float2*>(at);
+  at += round_up(sp * 8);
+  ws.meta = reinterpret_cast<int2*>(at);
+  switch (p.hd) {
+    case 32: return launch<32>(p, n, ws, st);
+    case 64: return launch<64>(p, n, ws, st);
+    case 128: return launch<128>(p, n, ws, st);
+  }
+  return -10;
+}
+
+}  // namespace seg

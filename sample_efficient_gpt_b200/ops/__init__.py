@@ -130,6 +130,72 @@ def attention_bwd(do, q, k, v, o, lse, causal: bool = True, q_start: int = 0):
     return ref.attention_bwd(do, q, k, v, o, lse, causal, q_start)
 
 
+# ----------------------------------------------------------------------------- paged cache (serving)
+def qkv_post_paged(qkv, v1, cos, sin, qgain, a1, a2, vscale, H, Hkv, hd, qknorm, k_pages, v_pages, page_table, seq_lens, cu_seqlens=None, pos_base=None,
+                   want_k=False, want_v=False):
+    """``qkv_post_fwd`` for tokens that join a paged cache: rotation, QK-norm and value residual, with the finished keys and
+    values written straight into their pages.  Returns (q [T, H, hd], k [T, Hkv, hd] if ``want_k`` else None, v likewise).
+
+    ``qkv`` [T, (H + 2 Hkv) hd] may be a column slice of a wider projection.  ``k_pages`` / ``v_pages`` [pages, P, Hkv, hd]: any
+    strides that are multiples of 8 elements with contiguous dims (token-major or head-major pools).  ``page_table`` [B, W]
+    int32: pages of every sequence in order.  ``seq_lens`` [B] int32: tokens that its pages hold already; new token i of
+    sequence b is stored at position p = seq_lens[b] + i and rotated for position p + pos_base[b] (``pos_base`` [B] int32:
+    length of a shared prefix that lies in other pages).  ``cu_seqlens`` [B + 1] int32: the sequences' first rows in ``qkv``;
+    None: one token per sequence.  Lengths of zero are fine; rows outside [cu_seqlens[0], cu_seqlens[B]) come back as zeros and
+    leave the cache as it was.  The caller raises ``seq_lens`` afterwards.  Two sequences that name the same page for
+    positions written in one call leave either's values there.
+
+    Lengths and page numbers are read on the device only: a position beyond the page table or the rotation table and a page
+    outside the pool leave that token out (zeros in q, no write) and set the package's status word (``ops.gemm.status()``:
+    51, 52).  CUDA: bf16, head_dim 32, 64 or 128; capturable into a graph."""
+    if _use_cuda(qkv, "paged_append"):
+        _count()
+        return ext().paged_append(qkv, v1, cos, sin, qgain, a1, a2, vscale, H, Hkv, hd, qknorm, k_pages, v_pages, page_table, seq_lens, cu_seqlens, pos_base,
+                                  want_k, want_v)
+    return ref.qkv_post_paged(qkv, v1, cos, sin, qgain, a1, a2, vscale, H, Hkv, hd, qknorm, k_pages, v_pages, page_table, seq_lens, cu_seqlens, pos_base,
+                              want_k, want_v)
+
+
+def paged_attention(q, k_pages, v_pages, page_table, seq_lens, prefix_table=None, prefix_lens=None, group_rows=None, scale=None):
+    """Attention of one query token per sequence over a paged cache: (o [B, H, hd], lse [B, H] fp32).
+
+    Row b sees the first ``seq_lens[b]`` tokens of its own pages (``page_table`` [B, W] int32) and, before them, the tokens of
+    the prefix of its group: rows [group_rows[g], group_rows[g + 1]) share the first ``prefix_lens[g]`` tokens of
+    ``prefix_table[g]`` ([G, Wp] int32), whose keys and values are read once for the group and not once per row.  ``group_rows``
+    [G + 1] int32 ascends within [0, B] (groups may be empty, rows outside every group have no prefix); None: one group of
+    all rows.  ``scale`` defaults to 1 / sqrt(hd).  A row that sees no token gives o = 0, lse = -inf.  Slots behind a length and
+    table entries behind the last page needed are never read.
+
+    Lengths, pages and borders are read on the device only: a length beyond its table is cut to the table, a page outside the
+    pool reads as zeros, and groups out of order count as empty; each sets the status word (``ops.gemm.status()``: 53, 54, 55).
+    CUDA: bf16, head_dim 32, 64 or 128, at most 8192 sequences and groups; capturable into a graph."""
+    if _use_cuda(q, "paged_attention"):
+        _count(2)
+        return ext().paged_attention(q, k_pages, v_pages, page_table, seq_lens, prefix_table, prefix_lens, group_rows, scale)
+    return ref.paged_attention(q, k_pages, v_pages, page_table, seq_lens, prefix_table, prefix_lens, group_rows, scale)
+
+
+# ----------------------------------------------------------------------------- logits before sampling
+def process_logits(logits, tokens=None, prompt_lens=None, token_lens=None, repetition=None, presence=None, frequency=None, bias_ids=None,
+                   bias_values=None, mask=None, mask_rows=None, out=None):
+    """Logits [B, V] (fp32 or bf16; any row stride) on their way to the sampler; every step is optional, all in fp32:
+
+    1. of the first ``token_lens[b]`` entries of ``tokens`` [B, L] (int32 or int64; ids outside [0, V) are ignored), those from
+       ``prompt_lens[b]`` on are the answer.  Seen tokens: x = x / repetition[b] if x > 0 else x * repetition[b]; tokens of the
+       answer: x -= frequency[b] * count + presence[b] (``repetition``, ``presence``, ``frequency``: fp32 [B]);
+    2. x[bias_ids[b, i]] += bias_values[b, i] ([B, K] int32 / fp32; ids outside [0, V) are unused, values of an id given more
+       than once add up in order);
+    3. x = -inf where bit v % 32 of word mask[mask_rows[b], v // 32] is 0 (``mask`` int32 [M, ceil(V / 32)], ``mask_rows``
+       int32 [B], negative: all tokens allowed).  A mask without a bit leaves a row of -inf.
+
+    Returns a new tensor, or ``out`` (which may be ``logits``).  A history length outside [0, L] is cut to it, a mask row beyond M
+    counts as none; each sets the status word (``ops.gemm.status()``: 56, 57)."""
+    if _use_cuda(logits, "process_logits"):
+        _count()
+        return ext().process_logits(logits, tokens, prompt_lens, token_lens, repetition, presence, frequency, bias_ids, bias_values, mask, mask_rows, out)
+    return ref.process_logits(logits, tokens, prompt_lens, token_lens, repetition, presence, frequency, bias_ids, bias_values, mask, mask_rows, out)
+
+
 # ----------------------------------------------------------------------------- gate / swiglu
 def gate_fwd(o, z):
     if _use_cuda(o, "gate_fwd"):

@@ -184,6 +184,117 @@ def attention_bwd(do: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: T
     )
 
 
+# ----------------------------------------------------------------------------- paged cache (serving)
+def _paged_rows(pages: Tensor, table_row: Tensor, n: int) -> Tensor:
+    """The first n tokens that a row of a page table lists, [n, Hkv, hd]."""
+    P = pages.size(1)
+    if not 0 <= n <= table_row.numel() * P:
+        raise ValueError(f"length {n} does not fit into a page table of {table_row.numel()} pages of {P}")
+    i = torch.arange(n, device=pages.device)
+    page = table_row.long()[i // P]
+    if bool(((page < 0) | (page >= pages.size(0))).any()):
+        raise ValueError(f"page numbers must lie in [0, {pages.size(0)})")
+    return pages[page, i % P]
+
+
+def qkv_post_paged(qkv, v1, cos, sin, qgain, a1, a2, vscale, H, Hkv, hd, qknorm, k_pages, v_pages, page_table, seq_lens, cu_seqlens=None, pos_base=None,
+                   want_k=False, want_v=False):
+    """``qkv_post_fwd`` of tokens that join a paged cache (see ``ops.qkv_post_paged``); writes k_pages / v_pages in place."""
+    T, lp = qkv.size(0), qkv.dtype
+    q = qkv.new_zeros(T, H, hd)
+    k, v = qkv.new_zeros(T, Hkv, hd), qkv.new_zeros(T, Hkv, hd)
+    P, B = k_pages.size(1), seq_lens.numel()
+    starts = list(range(B + 1)) if cu_seqlens is None else cu_seqlens.tolist()
+    if cu_seqlens is None and B != T:
+        raise ValueError(f"without cu_seqlens every sequence brings one token: {T} tokens for {B} sequences")
+    for b in range(B):
+        t0, t1 = starts[b], starts[b + 1]
+        if t1 <= t0:
+            continue
+        at = int(seq_lens[b]) + torch.arange(t1 - t0, device=qkv.device)
+        pos = at + (0 if pos_base is None else int(pos_base[b]))
+        if int(seq_lens[b]) < 0 or int(at[-1]) >= page_table.size(1) * P or int(pos[0]) < 0 or int(pos[-1]) >= cos.size(0):
+            raise ValueError(f"sequence {b}: positions {int(at[0])}..{int(at[-1])} do not fit the page table or the rotation table")
+        page = page_table[b].long()[at // P]
+        if bool(((page < 0) | (page >= k_pages.size(0))).any()):
+            raise ValueError(f"sequence {b}: page numbers must lie in [0, {k_pages.size(0)})")
+        n = t1 - t0
+        qb, kb, vb = qkv_post_fwd(qkv[t0:t1], None if v1 is None else v1[t0:t1], cos[pos], sin[pos], qgain, a1, a2, vscale, 1, n, H, Hkv, hd, qknorm)
+        q[t0:t1], k[t0:t1], v[t0:t1] = qb[0], kb[0], vb[0]
+        k_pages[page, at % P] = kb[0].to(k_pages.dtype)
+        v_pages[page, at % P] = vb[0].to(v_pages.dtype)
+    return q.to(lp), k if want_k else None, v if want_v else None
+
+
+def paged_attention(q, k_pages, v_pages, page_table, seq_lens, prefix_table=None, prefix_lens=None, group_rows=None, scale=None):
+    """One query token per sequence over its group's prefix and its own pages (see ``ops.paged_attention``)."""
+    B, H, hd = q.shape
+    Hkv = k_pages.size(2)
+    scale = 1.0 / math.sqrt(hd) if scale is None else scale
+    o = q.new_zeros(B, H, hd)
+    lse = torch.full((B, H), float("-inf"), dtype=torch.float32, device=q.device)
+    group = [-1] * B
+    if prefix_table is not None:
+        rows = [0, B] if group_rows is None else group_rows.tolist()
+        if rows != sorted(rows) or rows[0] < 0 or rows[-1] > B:
+            raise ValueError(f"group_rows must ascend within [0, {B}], got {rows}")
+        for g in range(len(rows) - 1):
+            for b in range(rows[g], rows[g + 1]):
+                group[b] = g
+    for b in range(B):
+        k, v = _paged_rows(k_pages, page_table[b], int(seq_lens[b])), _paged_rows(v_pages, page_table[b], int(seq_lens[b]))
+        if group[b] >= 0:
+            n = int(prefix_lens[group[b]])
+            k = torch.cat((_paged_rows(k_pages, prefix_table[group[b]], n), k))
+            v = torch.cat((_paged_rows(v_pages, prefix_table[group[b]], n), v))
+        if k.size(0) == 0:
+            continue
+        s = torch.einsum("kgd,nkd->kgn", q[b].float().view(Hkv, H // Hkv, hd), k.float()) * scale
+        l = torch.logsumexp(s, dim=-1, keepdim=True)
+        p = torch.where(l == float("-inf"), 0.0, torch.exp(s - l))
+        o[b] = torch.einsum("kgn,nkd->kgd", p, v.float()).reshape(H, hd).to(q.dtype)
+        lse[b] = l.reshape(H)
+    return o, lse
+
+
+# ----------------------------------------------------------------------------- logits before sampling
+def process_logits(logits, tokens=None, prompt_lens=None, token_lens=None, repetition=None, presence=None, frequency=None, bias_ids=None,
+                   bias_values=None, mask=None, mask_rows=None, out=None):
+    """Penalties, biases and the mask of allowed tokens (see ``ops.process_logits``)."""
+    B, V = logits.shape
+    x = logits.float().clone()
+    if tokens is not None:
+        for b in range(B):
+            n = int(token_lens[b])
+            if not 0 <= n <= tokens.size(1):
+                raise ValueError(f"row {b}: history length {n} outside [0, {tokens.size(1)}]")
+            prompt = min(n, max(0, int(prompt_lens[b]))) if prompt_lens is not None else 0
+            row = tokens[b, :n].long()
+            real = (row >= 0) & (row < V)
+            seen = torch.bincount(row[real], minlength=V) > 0
+            count = torch.bincount(row[prompt:][real[prompt:]], minlength=V).float()
+            if repetition is not None:
+                x[b] = torch.where(seen, torch.where(x[b] > 0, x[b] / repetition[b], x[b] * repetition[b]), x[b])
+            if frequency is not None:
+                x[b] -= frequency[b] * count
+            if presence is not None:
+                x[b] -= presence[b] * (count > 0)
+    if bias_ids is not None:
+        for b in range(B):
+            for i, v in zip(bias_ids[b].tolist(), bias_values[b]):
+                if 0 <= i < V:
+                    x[b, i] += v
+    if mask is not None:
+        if bool((mask_rows >= mask.size(0)).any()):
+            raise ValueError(f"mask rows must be below {mask.size(0)}")
+        v = torch.arange(V, device=logits.device)
+        for b, m in enumerate(mask_rows.tolist()):
+            if m >= 0:
+                x[b, ((mask[m].long()[v // 32] >> (v % 32)) & 1) == 0] = float("-inf")
+    x = x.to(logits.dtype)
+    return x if out is None else out.copy_(x)
+
+
 # ----------------------------------------------------------------------------- per-head output gate
 def gate_fwd(o: Tensor, z: Tensor) -> Tensor:
     """o [T,H,hd], z [T,H] gate logits -> [T,H*hd] = 2*sigmoid(z) * o."""
