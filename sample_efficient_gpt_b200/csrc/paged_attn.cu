@@ -14,8 +14,7 @@
 // its own running maximum and sum: no barrier is crossed until the item ends.  Scores and the weighted sum are m16n8k16 tensor
 // core products with the query heads as (padded) rows; the bound is the bytes of the cache, not the products.  Keys behind the
 // length are filled with zeros by the copy and masked by index: what lies in those slots is never read.
-#include "common.cuh"
-#include "paged.h"
+#include "paged_common.cuh"
 
 namespace seg {
 
@@ -26,28 +25,12 @@ constexpr int kKeys = 16;               // keys per warp and step
 constexpr int kTile = kWarps * kKeys;   // keys per tile
 constexpr int kRows = 16;               // query rows per item
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxLists = 8192;         // sequences + groups (their cumulative tile counts live in shared memory)
 
 template <int HD> struct Cfg {
   static constexpr int kStages = HD == 128 ? 3 : 4;
   static constexpr int kChunks = HD / 8;                   // 16-byte chunks of a row
   static constexpr int kStageBytes = 2 * kKeys * HD * 2;   // K and V of one step
   static constexpr int kRing = kStages * kStageBytes;      // per warp
-};
-
-struct Plan {        // sizes that host and device derive alike
-  int gqa, RT;       // query heads per kv head; 16-row tiles of a sequence's item row
-  int rows_s;        // rows of a part of an own-pages item
-  int items_s, items_p;
-  int ctas;
-};
-
-struct Work {
-  float* acc_s;    // [items_s + ctas, rows_s, HD]
-  float2* ml_s;    // [items_s + ctas, rows_s]
-  float* acc_p;    // [items_p + ctas, 16, HD]
-  float2* ml_p;
-  int2* meta;      // [items_s + items_p] first part and number of parts of every item that has tiles
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -71,11 +54,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ float exp2_(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // Weight of a part (m, l) under the common maximum mm.  A part without a finite score has m = -inf and l = 0, unless NaN scores
 // made l NaN: then the row becomes NaN, as the formula says.
 __device__ __forceinline__ float part_weight(float m, float l, float mm) { return m == -INFINITY ? l : exp2_(m - mm); }
@@ -85,65 +63,6 @@ __device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -
 template <int HD> __device__ __forceinline__ uint32_t swz(int r, int c) {
   if (HD == 32) return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
   return r * (HD * 2) + ((c ^ (r & 7)) << 4);
-}
-
-__device__ __forceinline__ int clamp_len(int n, int width, int P, int* status) {
-  const int64_t cap = (int64_t)width * P;
-  if (n >= 0 && n <= cap) return n;
-  atomicCAS(status, 0, kStatusAttnLength);
-  return n < 0 ? 0 : (int)cap;
-}
-struct Group {
-  int r0, r1, len;
-};
-__device__ __forceinline__ Group load_group(const PagedAttnParams& p, int g) {
-  Group w;
-  w.r0 = p.groups != nullptr ? p.groups[g] : 0;
-  w.r1 = p.groups != nullptr ? p.groups[g + 1] : p.B;
-  if (w.r0 < 0 || w.r1 < w.r0 || w.r1 > p.B) {
-    atomicCAS(p.status, 0, kStatusAttnGroups);
-    w.r0 = w.r1 = 0;
-  }
-  w.len = w.r1 > w.r0 ? clamp_len(p.plens[g], p.ptable_width, p.pool.P, p.status) : 0;
-  return w;
-}
-__device__ __forceinline__ int row_tiles(const Group& g, int gqa) { return ((g.r1 - g.r0) * gqa + kRows - 1) / kRows; }
-// First item of a group's prefix: leaves room for the row tiles of the groups before it, whatever their sizes.
-__device__ __forceinline__ int first_item(const Plan& n, const PagedAttnParams& p, int g, int r0) {
-  return n.items_s + p.Hkv * (r0 * n.gqa / kRows + g);
-}
-
-// sum[i + 1] = tiles of the first i + 1 lists; all threads take part
-template <typename F>
-__device__ void scan_tiles(int* sum, int n, F tiles, int* warp_tot) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int carry = 0;
-  if (threadIdx.x == 0) sum[0] = 0;
-  for (int base = 0; base < n; base += kThreads) {
-    const int i = base + threadIdx.x;
-    int v = i < n ? tiles(i) : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
-    }
-    if (lane == 31) warp_tot[warp] = v;
-    __syncthreads();
-    int add = carry;
-    for (int w = 0; w < warp; ++w) add += warp_tot[w];
-    if (i < n) sum[i + 1] = v + add;
-    for (int w = 0; w < kWarps; ++w) carry += warp_tot[w];
-    __syncthreads();
-  }
-}
-// last i with sum[i] <= t (t < sum[n]); empty lists are passed over
-__device__ __forceinline__ int find_list(const int* sum, int n, int t) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (sum[mid] <= t) lo = mid; else hi = mid;
-  }
-  return lo;
 }
 
 // Addresses of one walk's keys: a list of pages and the kv head inside them.
@@ -270,19 +189,19 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnPar
   int* sum_p = sum_s + p.B + 1;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  scan_tiles(sum_s, p.B, [&](int b) { return (clamp_len(p.lens[b], p.table_width, p.pool.P, p.status) + kTile - 1) / kTile; }, warp_tot);
-  scan_tiles(sum_p, p.G, [&](int g) {
+  scan_tiles<kThreads>(sum_s, p.B, [&](int b) { return (clamp_len(p.lens[b], p.table_width, p.pool.P, p.status) + kTile - 1) / kTile; }, warp_tot);
+  const int n_groups = n.form == kPrefixSmall ? p.G : 0;
+  scan_tiles<kThreads>(sum_p, n_groups, [&](int g) {
     const Group w = load_group(p, g);
-    return (w.len + kTile - 1) / kTile * row_tiles(w, n.gqa);
+    return (w.len + kTile - 1) / kTile * row_tiles(w, n);
   }, warp_tot);
   __syncthreads();
   const int per_seq = p.Hkv * n.RT;
   const int64_t tiles_s = (int64_t)sum_s[p.B] * per_seq;
-  const int64_t total = tiles_s + (int64_t)sum_p[p.G] * p.Hkv;
+  const int64_t total = tiles_s + (int64_t)sum_p[n_groups] * p.Hkv;
   const int64_t ctas = min((int64_t)gridDim.x, total);  // every one of them has a tile: the parts of an item have consecutive numbers
-  if (blockIdx.x >= ctas) return;
-  const int64_t t_end = total * (blockIdx.x + 1) / ctas;
-  for (int64_t t = total * blockIdx.x / ctas; t < t_end;) {
+  const int64_t t_end = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
+  for (int64_t t = t_end > 0 ? total * blockIdx.x / ctas : 0; t < t_end;) {
     // ---- the item that tile t belongs to
     KeyWalk w;
     int item, kvh, rows, row0, h0, n_tiles, tile0;  // rows r = 0 .. rows-1 are query row row0 + (h0 + r) / gqa, head kvh * gqa + (h0 + r) % gqa
@@ -301,12 +220,12 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnPar
       w.pages = p.table + b * p.table_stride;
     } else {
       const int64_t tp = t - tiles_s;
-      const int g = find_list(sum_p, p.G, (int)(tp / p.Hkv));
+      const int g = find_list(sum_p, n_groups, (int)(tp / p.Hkv));
       const Group gr = load_group(p, g);
       n_tiles = (gr.len + kTile - 1) / kTile;
       const int local = (int)(tp - (int64_t)sum_p[g] * p.Hkv), i = local / n_tiles;
       tile0 = local - i * n_tiles;
-      const int rt = row_tiles(gr, n.gqa);
+      const int rt = row_tiles(gr, n);
       kvh = i / rt;
       h0 = (i - kvh * rt) * kRows;
       item = first_item(n, p, g, gr.r0) + i;
@@ -318,9 +237,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnPar
     w.k = static_cast<const __nv_bfloat16*>(p.pool.k) + kvh * p.pool.k_head;
     w.v = static_cast<const __nv_bfloat16*>(p.pool.v) + kvh * p.pool.v_head;
     const int steps = (int)min(t_end - t, (int64_t)(n_tiles - tile0));
-    const int64_t first_tile = t - tile0;
-    const int cta_first = (int)(((first_tile + 1) * ctas - 1) / total), cta_last = (int)(((first_tile + n_tiles) * ctas - 1) / total);
-    if (tile0 == 0 && threadIdx.x == 0) ws.meta[item] = make_int2((own ? item : item - n.items_s) + cta_first, cta_last - cta_first + 1);
+    if (tile0 == 0 && threadIdx.x == 0) ws.meta[item] = item_parts(own ? item : item - n.items_s, t, n_tiles, ctas, total);
 
     // ---- queries: the A operand, straight from memory
     uint32_t qf[HD / 16][4];
@@ -402,6 +319,9 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnPar
     __syncthreads();
     t += steps;
   }
+  // The prefix kernel before this one let it start early.  It must have ended when this one ends, for the join waits for this
+  // one alone.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Joins the parts of one (row, head): the prefix's, then the sequence's own, in order.
@@ -427,10 +347,12 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const PagedAt
     const Group gr = load_group(p, g);
     if (gr.len > 0 && b >= gr.r0 && b < gr.r1) {
       const int x = (b - gr.r0) * n.gqa + hl;
-      parts[0] = ws.meta[first_item(n, p, g, gr.r0) + kvh * row_tiles(gr, n.gqa) + x / kRows];
-      row_p = x % kRows;
+      parts[0] = ws.meta[first_item(n, p, g, gr.r0) + kvh * row_tiles(gr, n) + x / n.rows_p];
+      row_p = x % n.rows_p;
       // out of order group rows could leave an item without its entry
-      if (parts[0].x < 0 || parts[0].y < 0 || (int64_t)parts[0].x + parts[0].y > n.items_p + n.ctas) parts[0] = make_int2(0, 0);
+      if (parts[0].x < 0 || parts[0].y < 0 || (int64_t)parts[0].x + parts[0].y > n.items_p + n.ctas_p) parts[0] = make_int2(0, 0);
+      parts[0].x *= n.parts_p;
+      parts[0].y *= n.parts_p;
     }
   }
   if (len > 0) {
@@ -443,7 +365,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const PagedAt
   float acc[kPer] = {};
   for (int i = warp; i < total; i += kWarps) {
     const bool pre = i < parts[0].y;
-    const int64_t at = pre ? (int64_t)(parts[0].x + i) * kRows + row_p : (int64_t)(parts[1].x + i - parts[0].y) * n.rows_s + hl % kRows;
+    const int64_t at = pre ? (int64_t)(parts[0].x + i) * n.part_rows_p + row_p : (int64_t)(parts[1].x + i - parts[0].y) * n.rows_s + hl % kRows;
     const float2 ml = (pre ? ws.ml_p : ws.ml_s)[at];
     const float* src = (pre ? ws.acc_p : ws.acc_s) + at * HD + lane * kPer;
     float x[kPer];
@@ -483,19 +405,29 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const PagedAt
 
 template <int HD> int smem_bytes(const PagedAttnParams& p) { return kWarps * Cfg<HD>::kRing + (p.B + p.G + 2) * (int)sizeof(int); }
 
+// Rows of a kv head per group on average from which the tcgen05 forms are used for the prefixes.
+constexpr int kDenseRows = 32;
+
 Plan make_plan(const PagedAttnParams& p) {
   Plan n;
   n.gqa = p.H / p.Hkv;
   n.RT = (n.gqa + kRows - 1) / kRows;
   n.rows_s = n.gqa < kRows ? n.gqa : kRows;
   n.items_s = p.B * p.Hkv * n.RT;
-  n.items_p = p.G > 0 ? p.Hkv * (int)((int64_t)p.B * n.gqa / kRows + p.G + 1) : 0;
+  const int64_t rows = p.G > 0 ? (int64_t)p.B * n.gqa / p.G : 0;
+  n.form = rows >= kDenseRows && paged_prefix_usable(p) ? (p.hd == 64 && rows > 128 ? kPrefixRows : kPrefixKeys) : kPrefixSmall;
+  n.rows_p = n.form == kPrefixSmall ? kRows : n.form == kPrefixRows ? 256 : 128;
+  n.parts_p = n.form == kPrefixKeys ? 2 : 1;
+  n.part_rows_p = n.rows_p;
+  n.items_p = p.G > 0 ? p.Hkv * (int)((int64_t)p.B * n.gqa / n.rows_p + p.G + 1) : 0;
   // one resident wave, but no more CTAs than there can be tiles
   const int per_sm = p.hd == 128 || p.B + p.G > 2048 ? 2 : 3;
   const int64_t P = p.pool.P;
-  int64_t tiles = (int64_t)n.items_s * ((p.table_width * P + kTile - 1) / kTile);
-  if (p.G > 0) tiles += (int64_t)n.items_p * ((p.ptable_width * P + kTile - 1) / kTile);
+  int64_t tiles = (int64_t)n.items_s * ((p.table_width * P + kTile - 1) / kTile), tiles_p = 0;
+  if (n.form == kPrefixSmall) tiles += (int64_t)n.items_p * ((p.ptable_width * P + kTile - 1) / kTile);
+  else tiles_p = (int64_t)n.items_p * ((p.ptable_width * P + 127) / 128);
   n.ctas = (int)(tiles < 148 * per_sm ? (tiles < 1 ? 1 : tiles) : 148 * per_sm);
+  n.ctas_p = n.form == kPrefixSmall ? n.ctas : (int)(tiles_p < 148 ? tiles_p : 148);
   return n;
 }
 
@@ -510,18 +442,27 @@ int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t
     if (cudaFuncSetAttribute(paged_attn_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * Cfg<HD>::kRing + (kMaxLists + 2) * 4) != cudaSuccess) return -2;
     configured[dev] = true;
   }
-  paged_attn_kernel<HD><<<n.ctas, kThreads, smem_bytes<HD>(p), st>>>(p, n, ws);
-  if (cudaGetLastError() != cudaSuccess) return -3;
-  // The join may be brought in while the walk still runs (it waits for its end in griddepcontrol.wait).
+  // The kernels after the first may be brought in while the one before still runs: the walk over own pages needs nothing of the
+  // prefix kernel and shares the SMs with it (one is bound by bytes, the other by arithmetic); the join waits in
+  // griddepcontrol.wait.
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.B, p.H);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
+  cfg.stream = st;
+  cfg.blockDim = dim3(kThreads);
+  if (n.form != kPrefixSmall) {
+    const int rc = paged_prefix(p, n, ws, st);
+    if (rc != 0) return rc;
+    cfg.numAttrs = 1;
+  }
+  cfg.gridDim = dim3(n.ctas);
+  cfg.dynamicSmemBytes = smem_bytes<HD>(p);
+  if (cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD>, p, n, ws) != cudaSuccess) return -3;
   cfg.numAttrs = 1;
+  cfg.gridDim = dim3(p.B, p.H);
+  cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<HD>, p, n, ws) == cudaSuccess ? 0 : -3;
 }
 
@@ -531,7 +472,7 @@ int64_t paged_attn_workspace(const PagedAttnParams& p) {
   if (p.hd != 32 && p.hd != 64 && p.hd != 128) return -1;
   if (p.B + p.G > kMaxLists) return -1;
   const Plan n = make_plan(p);
-  const int64_t ss = ((int64_t)n.items_s + n.ctas) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas) * kRows : 0;
+  const int64_t ss = ((int64_t)n.items_s + n.ctas) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas_p) * n.parts_p * n.part_rows_p : 0;
   return round_up(ss * p.hd * 4) + round_up(ss * 8) + round_up(sp * p.hd * 4) + round_up(sp * 8) + round_up(((int64_t)n.items_s + n.items_p) * 8);
 }
 
@@ -539,7 +480,7 @@ int paged_attn(const PagedAttnParams& p, void* workspace, cudaStream_t st) {
   if (p.B == 0) return 0;
   if (p.H < 1 || p.Hkv < 1 || p.H % p.Hkv != 0 || p.H > 65535 || p.B + p.G > kMaxLists) return -10;
   const Plan n = make_plan(p);
-  const int64_t ss = ((int64_t)n.items_s + n.ctas) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas) * kRows : 0;
+  const int64_t ss = ((int64_t)n.items_s + n.ctas) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas_p) * n.parts_p * n.part_rows_p : 0;
   uint8_t* at = static_cast<uint8_t*>(workspace);
   Work ws;
   ws.acc_s = reinterpret_cast<float*>(at);

@@ -1,0 +1,466 @@
+// The prefix part of the paged attention for groups with many rows, on tcgen05 tensor cores (head_dim 64 and 128, bf16).
+//
+// For every (group, kv head) the rows are the group's sequences x query heads of the kv head; all of them see the same keys, so
+// this is a plain (unmasked) attention with few "queries" and a long walk: S = Q K^T, P = exp2(scale S - m), O += P V, with the
+// keys and values gathered page by page.  Its results are parts (m, l, unnormalised O) that the join kernel of paged_attn.cu
+// merges with the sequences' own tokens.
+//
+// Work: items of 256 rows (two tiles of 128 that share every key tile; kRows form) or of 128 rows whose key tiles are dealt to
+// the CTA's two halves alternately (kKeys form: fewer rows, or head_dim 128, where two query tiles would not fit into shared
+// memory).  The key tiles (128 keys) of all items in one row are dealt to one CTA per SM in equal, contiguous ranges.
+//
+// Roles of a CTA (384 threads): warp 0 loads, every lane one box of a page (2 to 16 boxes of 8 to 64 or 128 keys a tile, K and V
+// each in a ring of two; the last tile's missing keys are set to zero before the products see them); warps 1 and 2 issue the
+// products of half 0 / 1; warps 4-7 and 8-11 are the softmax of half 0 / 1, a row per thread.
+//
+// Bound: one exp2 per score on the special-function unit, 16 a cycle and SM: 2048 cycles for 256 x 128 scores against 1024 of
+// the tensor core at head_dim 64.  The softmax therefore takes the maximum off its critical path: the exponentials use the
+// maximum of the tiles before, and only when a new score exceeds it by more than 2^8 (rare after the first tile) is the row's
+// sum rescaled and the tile repeated from tensor memory.  Scores pass through the registers 32 columns at a time, the next
+// load in flight, which leaves room on the SM for a CTA of the kernel over own pages.
+#include <cuda.h>
+
+#include "paged_common.cuh"
+#include "sm100.cuh"
+
+namespace seg {
+
+using namespace sm100;
+
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kTileKeys = 128;
+constexpr int kBlock = kTileKeys * 128;  // bytes of 128 rows of 64 bf16: the unit of all operand tiles
+constexpr int kPBytes = 2 * kBlock;      // P of one half: 128 x 128
+
+template <int HD, bool kSplit> struct Lay {
+  static constexpr int kTile = HD / 64 * kBlock;        // a K or V tile
+  static constexpr int kQ = (kSplit ? 1 : 2) * kTile;   // query tiles
+  static constexpr int kK = kQ, kV = kK + 2 * kTile, kP = kV + 2 * kTile, kBars = kP + 2 * kPBytes, kSum = kBars + 256;
+};
+
+struct Seg {
+  int item, kvh, rows, row0, x0;  // rows r = x0 .. x0 + rows - 1 of the group: sequence row0 + r / gqa, head kvh * gqa + r % gqa
+  int len, tile0, n_tiles, steps;
+  const int* pages;
+};
+
+__device__ __forceinline__ Seg find_seg(const PagedAttnParams& p, const Plan& n, const int* sum, int64_t t, int64_t t_end) {
+  Seg s;
+  const int g = find_list(sum, p.G, (int)(t / p.Hkv));
+  const Group gr = load_group(p, g);
+  s.n_tiles = (gr.len + kTileKeys - 1) / kTileKeys;
+  const int local = (int)(t - (int64_t)sum[g] * p.Hkv), i = local / s.n_tiles, rt = row_tiles(gr, n);
+  s.tile0 = local - i * s.n_tiles;
+  s.kvh = i / rt;
+  s.x0 = (i - s.kvh * rt) * n.rows_p;
+  s.item = first_item(n, p, g, gr.r0) + i;
+  s.row0 = gr.r0;
+  s.rows = min(n.rows_p, (gr.r1 - gr.r0) * n.gqa - s.x0);
+  s.len = gr.len;
+  s.steps = (int)min(t_end - t, (int64_t)(s.n_tiles - s.tile0));
+  s.pages = p.ptable + g * p.ptable_stride;
+  return s;
+}
+
+template <int HD, bool kSplit>
+__global__ void __maxnreg__(128)  // of 384 threads: leaves 16384 registers for a CTA of the kernel over own pages
+paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedAttnParams p, const Plan n, const Work ws,
+                    const int box) {
+  using L = Lay<HD, kSplit>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need a 1024-byte aligned base
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, 60);
+    return;
+  }
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t *q_full = bars, *k_full = bars + 2, *k_empty = bars + 4, *v_full = bars + 6, *v_empty = bars + 8, *s_full = bars + 10, *s_empty = bars + 12,
+           *p_full = bars + 14, *pv_full = bars + 16, *tail = bars + 18, *q_free = bars + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* warp_tot = reinterpret_cast<int*>(bars + 21);
+  int* sum = reinterpret_cast<int*>(smem + L::kSum);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const AbortState ab{cta_abort, p.status};
+
+  if (threadIdx.x == 0) {
+    *cta_abort = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&q_full[i]), 4);
+      mbar_init(smem_u32(&k_full[i]), 1);
+      mbar_init(smem_u32(&v_full[i]), 1);
+      mbar_init(smem_u32(&k_empty[i]), kSplit ? 1 : 2);  // released by the products of every half that reads the tile
+      mbar_init(smem_u32(&v_empty[i]), kSplit ? 1 : 2);
+      mbar_init(smem_u32(&s_full[i]), 1);
+      mbar_init(smem_u32(&s_empty[i]), 4);
+      mbar_init(smem_u32(&p_full[i]), 4);
+      mbar_init(smem_u32(&pv_full[i]), 1);
+    }
+    mbar_init(smem_u32(tail), 1);
+    mbar_init(smem_u32(q_free), 5);  // the second half's softmax warps and its issuer
+    fence_barrier_init();
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+  }
+  if (warp == 0) {
+    __syncwarp();
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  scan_tiles<kThreads>(sum, p.G, [&](int g) {
+    const Group w = load_group(p, g);
+    return (w.len + kTileKeys - 1) / kTileKeys * row_tiles(w, n);
+  }, warp_tot);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // columns [0, 256): scores of half 0 / 1; from 256 on: outputs of half 0 / 1
+  const int64_t total = (int64_t)sum[p.G] * p.Hkv;
+  const int64_t ctas = min((int64_t)gridDim.x, total);
+  const int64_t t_begin = blockIdx.x < ctas ? total * blockIdx.x / ctas : 0, t_end = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------------------------------------ loads
+    const int boxes = kTileKeys / box;
+    int c = 0, tails = 0, used[2] = {0, 0};  // rows form: tiles so far; keys form: tiles so far of each half, whose ring slot is its own
+    bool ok = true;
+    for (int64_t t = t_begin; t < t_end && ok;) {
+      const Seg s = find_seg(p, n, sum, t, t_end);
+      for (int j = 0; j < s.steps && ok; ++j, ++c) {
+        const int st = kSplit ? j & 1 : c & 1, ph = (kSplit ? (j & 1 ? used[1]++ : used[0]++) : c >> 1) & 1;
+        const int first = (s.tile0 + j) * kTileKeys, key = first + lane * box;
+        int page = 0, slot = 0;
+        bool live = lane < boxes && key < s.len;
+        if (live) {
+          const int i = p.pool.shift >= 0 ? key >> p.pool.shift : key / p.pool.P;
+          page = s.pages[i];
+          slot = key - i * p.pool.P;
+          if ((unsigned)page >= (unsigned)p.pool.n_pages) {
+            atomicCAS(p.status, 0, kStatusAttnPage);
+            live = false;
+          }
+        }
+        const unsigned live_boxes = __ballot_sync(0xffffffffu, live);
+        const bool full = first + kTileKeys <= s.len && __popc(live_boxes) == boxes;
+        // K before V: the issuer wants the next scores before it issues the products that free the place of the V tile.
+#pragma unroll
+        for (int kv = 0; kv < 2 && ok; ++kv) {
+          uint64_t* tile_full = kv == 0 ? &k_full[st] : &v_full[st];
+          const uint32_t dst = (kv == 0 ? L::kK : L::kV) + st * L::kTile, bar = smem_u32(full ? tile_full : tail);
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(kv == 0 ? &k_empty[st] : &v_empty[st]), ph ^ 1, ab, 61 + kv));
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(bar, __popc(live_boxes) * box * HD * 2);
+          __syncwarp();
+          if (live) {
+#pragma unroll
+            for (int b = 0; b < HD / 64; ++b)
+              tma_load_4d(smem_u32(smem) + dst + b * kBlock + lane * box * 128, kv == 0 ? &map_k : &map_v, bar, b * 64, s.kvh, slot, page);
+          }
+          if (full) continue;
+          // Keys behind the length, and pages that do not exist: zeros, so that no weight of zero meets what lies there.
+          ok = __all_sync(0xffffffffu, mbar_wait(bar, tails & 1, ab, 63));
+          if (!ok) break;
+          ++tails;
+          for (int i = lane; i < kTileKeys * 8; i += 32) {
+            const int r = i >> 3;
+            if (first + r < s.len && ((live_boxes >> (r / box)) & 1)) continue;
+#pragma unroll
+            for (int b = 0; b < HD / 64; ++b) *reinterpret_cast<uint4*>(smem + dst + b * kBlock + i * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(tile_full));
+        }
+      }
+      t += s.steps;
+    }
+  } else if (warp <= 2) {
+    // ------------------------------------------------------------------------------------------------ products of half x
+    const int x = warp - 1;
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = make_idesc_bf16(128, kTileKeys, false, false);  // Q (K-major) x K (K-major)
+      constexpr uint32_t idesc_o = make_idesc_bf16(128, HD, false, true);          // P (K-major) x V (MN-major)
+      const uint64_t d_q = make_smem_desc(smem_u32(smem) + (kSplit ? 0 : x * L::kTile), 16, 1024);
+      const uint64_t d_p = make_smem_desc(smem_u32(smem + L::kP) + x * kPBytes, 16, 1024);
+      const uint32_t t_s = tmem + x * kTileKeys, t_o = tmem + 256 + x * HD;
+      int cx = 0, seg = 0;  // tiles of this half, segments
+      bool ok = true;
+      for (int64_t t = t_begin; t < t_end && ok; ++seg) {
+        const Seg s = find_seg(p, n, sum, t, t_end);
+        const int mine = kSplit ? (s.steps + 1 - x) / 2 : s.steps;
+        ok = mbar_wait(smem_u32(&q_full[kSplit ? 0 : x]), seg & 1, ab, 64);  // in every segment, so that no phase is missed
+        if (kSplit && x == 1 && ok) mbar_arrive(smem_u32(q_free));
+        auto scores = [&](int i) {
+          const int at = cx + i, st = kSplit ? x : at & 1, ph = (kSplit ? at : at >> 1) & 1;
+          if (!mbar_wait(smem_u32(&k_full[st]), ph, ab, 65)) return false;
+          if (at > 0 && !mbar_wait(smem_u32(&s_empty[x]), (at - 1) & 1, ab, 66)) return false;
+          const uint64_t d_k = make_smem_desc(smem_u32(smem + L::kK + st * L::kTile), 16, 1024);
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint64_t off = (uint64_t)(((k >> 2) * kBlock + (k & 3) * 32) >> 4);
+            umma_bf16(t_s, d_q + off, d_k + off, idesc_s, k > 0);
+          }
+          umma_commit(smem_u32(&s_full[x]));
+          umma_commit(smem_u32(&k_empty[st]));
+          return true;
+        };
+        if (ok && mine > 0) ok = scores(0);
+        for (int i = 0; i < mine && ok; ++i) {
+          if (i + 1 < mine && !scores(i + 1)) { ok = false; break; }
+          const int at = cx + i, st = kSplit ? x : at & 1, ph = (kSplit ? at : at >> 1) & 1;
+          if (!mbar_wait(smem_u32(&v_full[st]), ph, ab, 67) || !mbar_wait(smem_u32(&p_full[x]), at & 1, ab, 68)) { ok = false; break; }
+          const uint64_t d_v = make_smem_desc(smem_u32(smem + L::kV + st * L::kTile), kBlock, 1024);
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < kTileKeys / 16; ++k)
+            umma_bf16(t_o, d_p + (uint64_t)(((k >> 2) * kBlock + (k & 3) * 32) >> 4), d_v + (uint64_t)(k * 128), idesc_o, i > 0 || k > 0);
+          umma_commit(smem_u32(&pv_full[x]));
+          umma_commit(smem_u32(&v_empty[st]));
+        }
+        cx += mine;
+        t += s.steps;
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------------------------------------ softmax of half x
+    const int x = (warp >> 2) - 1, sub = warp & 3, r = sub * 32 + lane;  // r: row of the half's tile == TMEM lane
+    const uint32_t lane_addr = (uint32_t)(sub * 32) << 16;
+    const uint32_t t_s = tmem + x * kTileKeys + lane_addr, t_o = tmem + 256 + x * HD + lane_addr;
+    uint8_t* sP = smem + L::kP + x * kPBytes + r * 128;
+    const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
+    int cx = 0, seg = 0;
+    bool ok = true;
+    // tensor memory is read by whole warps: when a wait gives up, all lanes leave together
+    auto wait = [&](uint64_t* bar, int parity, int code) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, ab, code)) != 0; };
+    for (int64_t t = t_begin; t < t_end && ok; ++seg) {
+      const Seg s = find_seg(p, n, sum, t, t_end);
+      const int mine = kSplit ? (s.steps + 1 - x) / 2 : s.steps;
+      if (s.tile0 == 0 && threadIdx.x == 128) ws.meta[s.item] = item_parts(s.item - n.items_s, t, s.n_tiles, ctas, total);
+      const int row = (kSplit ? 0 : x * 128) + r;
+      // Queries of the segment.  The products of the segment before with the old ones are complete: this warp has seen its last
+      // scores, and where both halves read one query tile the other half says so (its issuer too: it may have had no tile).
+      if (kSplit && x == 0 && seg > 0) {
+        ok = wait(q_free, (seg - 1) & 1, 73);
+        if (!ok) break;
+      }
+      if (!kSplit || x == 0) {
+        uint8_t* sQ = smem + (kSplit ? 0 : x * L::kTile) + r * 128;
+        const int q = s.x0 + row;
+        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.q) + (s.row0 + q / n.gqa) * p.q_row + (s.kvh * n.gqa + q % n.gqa) * p.q_head;
+        const bool live = row < s.rows;
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          const uint4 v = live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(sQ + (c >> 3) * kBlock + (((c & 7) ^ (r & 7)) << 4)) = v;
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&q_full[kSplit ? 0 : x]));
+      } else {  // without a tile of its own in a segment this half would run ahead and count twice on q_free
+        ok = wait(&q_full[0], seg & 1, 74);
+        if (!ok) break;
+      }
+      float m = -INFINITY, l = 0.f;  // m: reference of the exponentials, the row's maximum up to 2^8
+      for (int i = 0; i < mine && ok; ++i) {
+        const int at = cx + i, tile = s.tile0 + (kSplit ? 2 * i + x : i);
+        const int left = s.len - tile * kTileKeys;  // keys of this tile that exist
+        ok = wait(&s_full[x], at & 1, 69);
+        if (!ok) break;
+        tc_fence_after();
+        // The first pass uses the reference that there is (on a segment's first tile it only finds the maximum); a pass with a
+        // new reference follows where it was too low.  A third one is for scores so large that their own rounding exceeds 8.
+        for (int pass = 0;; ++pass) {
+          const bool only_max = i == 0 && pass == 0;
+          const float base = m == -INFINITY ? 0.f : m;
+          const uint64_t neg2 = pack2(-base, -base);
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          uint64_t l2[2] = {0ull, 0ull};
+          uint32_t v[2][32];
+          bool redo = false;
+          tmem_ld_32x32(t_s, v[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t* w = v[c & 1];
+            tmem_ld_wait_regs(w);
+            if (c < 3) tmem_ld_32x32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
+            uint64_t y[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              y[e] = fma2(pack2(w[2 * e], w[2 * e + 1]), scale2, neg2);
+              float a, b;
+              unpack2(y[e], a, b);
+              if (left < kTileKeys) {
+                if (c * 32 + 2 * e >= left) a = -INFINITY;
+                if (c * 32 + 2 * e + 1 >= left) b = -INFINITY;
+                y[e] = pack2(a, b);
+              }
+              mx4[e & 3] = max3(mx4[e & 3], a, b);
+            }
+            if (c == 3) {
+              const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+              const bool low = mx > 8.f || (m == -INFINITY && mx > -INFINITY);
+              redo = only_max || (pass < 2 && __any_sync(0xffffffffu, low));
+              if (redo) {
+                const float m_new = low ? mx + base : m;
+                if (i > 0) {  // what was summed so far is rescaled (P V of the tile before is complete: waited for at c == 0)
+                  const float a = low && m != -INFINITY ? exp2_(m - m_new) : 1.f;
+                  l *= a;
+#pragma unroll
+                  for (int o = 0; o < HD / 32; ++o) {
+                    uint32_t f[32];
+                    tmem_ld_32x32(t_o + o * 32, f);
+                    tmem_ld_wait_regs(f);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) f[e] = __float_as_uint(__uint_as_float(f[e]) * a);
+                    tmem_st_32x32(t_o + o * 32, f);
+                  }
+                  tmem_st_wait();
+                }
+                m = m_new;
+                break;
+              }
+              // the scores are in registers: the next product may overwrite them
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(&s_empty[x]));
+            }
+            if (only_max) continue;
+            if (c == 0 && i > 0 && pass == 0) {  // P V of the tile before has read the P tile
+              ok = wait(&pv_full[x], (at - 1) & 1, 71);
+              if (!ok) break;
+              tc_fence_after();
+            }
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+              float e[8];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                float a, b;
+                unpack2(y[q4 * 4 + k], a, b);
+                e[2 * k] = exp2_(a);
+                e[2 * k + 1] = exp2_(b);
+                l2[k & 1] = add2(l2[k & 1], pack2(e[2 * k], e[2 * k + 1]));
+              }
+              const int c16 = c * 4 + q4;  // bf16 operand tile: 16-byte chunk c16 of row r at c16 ^ (r & 7) inside its 64-column block
+              *reinterpret_cast<bf16x8*>(sP + (c16 >> 3) * kBlock + (((c16 & 7) ^ (r & 7)) << 4)) = pack8(e);
+            }
+          }
+          if (!ok) break;
+          if (redo) continue;
+          float a0, a1, a2, a3;
+          unpack2(l2[0], a0, a1);
+          unpack2(l2[1], a2, a3);
+          l += (a0 + a1) + (a2 + a3);
+          break;
+        }
+        if (!ok) break;
+        tc_fence_before();
+        fence_proxy_async();  // the P tile is visible to the tensor core
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&p_full[x]));
+      }
+      if (kSplit && x == 1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(q_free));
+      }
+      // ---- the part of this segment
+      const int64_t part = kSplit ? ((int64_t)(s.item - n.items_s) + blockIdx.x) * 2 + x : (int64_t)(s.item - n.items_s) + blockIdx.x;
+      const int64_t out = part * n.part_rows_p + row;
+      if (ok && row < s.rows) ws.ml_p[out] = make_float2(m, l);
+      if (ok && mine > 0) {
+        ok = wait(&pv_full[x], (cx + mine - 1) & 1, 72);
+        tc_fence_after();
+        if (ok) {
+#pragma unroll
+          for (int o = 0; o < HD / 32; ++o) {
+            uint32_t f[32];
+            tmem_ld_32x32(t_o + o * 32, f);
+            tmem_ld_wait_regs(f);
+            if (row < s.rows) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                reinterpret_cast<uint4*>(ws.acc_p + out * HD + o * 32)[e] = make_uint4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+            }
+          }
+        }
+      }
+      cx += mine;
+      t += s.steps;
+    }
+  }
+
+  if (*cta_abort != 0) {
+    tmem_ld_wait();
+    for (int i = 0; i < 2000; ++i) __nanosleep(100);  // copies in flight land before the CTA's memory is given away
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// 4-D bf16 map over a pool [pages, P, Hkv, hd] with any strides, a box of 64 dims x `box` tokens, 128-byte swizzle.
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int make_pool_map(CUtensorMap* map, void* base, const PagedAttnParams& p, int64_t page, int64_t slot, int64_t head, int box) {
+  static EncodeFn fn = nullptr;
+  if (fn == nullptr) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess) return -1;
+    fn = reinterpret_cast<EncodeFn>(ptr);
+  }
+  // a dimension of one element may have any stride in the framework; the map wants a multiple of 16 bytes
+  const cuuint64_t dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)p.Hkv, (cuuint64_t)p.pool.P, (cuuint64_t)p.pool.n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)(p.Hkv == 1 ? p.hd : head) * 2, (cuuint64_t)(p.pool.P == 1 ? p.hd : slot) * 2,
+                                 (cuuint64_t)(p.pool.n_pages == 1 ? p.hd : page) * 2};
+  const cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1}, ones[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -1;
+}
+
+// Tokens of a box: the largest power of two that divides the page, so that a box never leaves its page; whole 8-row groups of
+// the swizzle pattern.
+int box_of(int P) {
+  int box = P & -P;
+  return box > kTileKeys ? kTileKeys : box;
+}
+
+template <int HD, bool kSplit>
+int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t st) {
+  using L = Lay<HD, kSplit>;
+  const int box = box_of(p.pool.P);
+  CUtensorMap mk, mv;
+  if (make_pool_map(&mk, p.pool.k, p, p.pool.k_page, p.pool.k_slot, p.pool.k_head, box) != 0 ||
+      make_pool_map(&mv, p.pool.v, p, p.pool.v_page, p.pool.v_slot, p.pool.v_head, box) != 0)
+    return -5;
+  static bool configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(paged_prefix_kernel<HD, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return -2;
+    configured[dev] = true;
+  }
+  paged_prefix_kernel<HD, kSplit><<<n.ctas_p, kThreads, L::kSum + (p.G + 1) * 4, st>>>(mk, mv, p, n, ws, box);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+}  // namespace
+
+bool paged_prefix_usable(const PagedAttnParams& p) {
+  if (p.hd != 64 && p.hd != 128) return false;
+  if (box_of(p.pool.P) < 8) return false;
+  const int smem = (p.hd == 128 ? Lay<128, true>::kSum : Lay<64, false>::kSum) + (p.G + 1) * 4;
+  return smem <= 227 * 1024;
+}
+
+int paged_prefix(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t st) {
+  if (n.form == kPrefixRows) return p.hd == 64 ? launch<64, false>(p, n, ws, st) : -10;
+  return p.hd == 64 ? launch<64, true>(p, n, ws, st) : p.hd == 128 ? launch<128, true>(p, n, ws, st) : -10;
+}
+
+}  // namespace seg

@@ -177,7 +177,8 @@ def test_attention_shared_prefix(H, Hkv, hd, P, layout):
 
 
 @pytest.mark.parametrize("B,plen,H,Hkv,hd,P", [(1, 5000, 18, 6, 64, 16), (7, 129, 12, 12, 64, 16), (64, 1000, 18, 6, 64, 64), (100, 2100, 24, 2, 64, 32), (70, 513, 32, 8, 128, 128),
-                                               (33, 700, 16, 4, 64, 40)])
+                                               (33, 700, 16, 4, 64, 40), (20, 900, 18, 6, 64, 16), (11, 127, 18, 6, 64, 8), (45, 128, 18, 6, 64, 128),
+                                               (40, 300, 18, 6, 64, 12)])
 def test_attention_one_prefix_for_all(B, plen, H, Hkv, hd, P):
     lens = [(13 * b) % 70 for b in range(B)]
     c = cache_case(lens, H, Hkv, hd, P, "token", [plen], seed=B)
@@ -185,12 +186,65 @@ def test_attention_one_prefix_for_all(B, plen, H, Hkv, hd, P):
     check_attention(o, lse, attention_oracle(c["q"], c["ks"], c["vs"], [0] * B), hd)
 
 
+# rows of a kv head per group: few (16 at a time), tens (128, the keys in two halves), hundreds (256)
+@pytest.mark.parametrize("H,Hkv,hd,P,layout", [(18, 6, 64, 16, "token"), (24, 2, 64, 24, "head"), (32, 8, 128, 32, "head"), (64, 2, 128, 8, "token"), (40, 1, 64, 256, "token")])
+def test_attention_large_groups(H, Hkv, hd, P, layout):
+    sizes, plens = [40, 0, 1, 44], [1500, 64, 129, 700]
+    rows = [0, 40, 40, 41, 85]
+    lens = [(17 * b) % 90 for b in range(88)]  # three rows without a prefix, some rows without tokens of their own
+    c = cache_case(lens, H, Hkv, hd, P, layout, plens, seed=hd + P)
+    o, lse = run_attention(c, rows)
+    group = [g for g, n in enumerate(sizes) for _ in range(n)] + [-1] * 3
+    check_attention(o, lse, attention_oracle(c["q"], c["ks"], c["vs"], group), hd)
+
+
+@pytest.mark.parametrize("B,H,Hkv,hd", [(4, 6, 2, 64), (30, 6, 2, 64), (90, 6, 2, 64), (30, 8, 2, 128)])
+@pytest.mark.parametrize("scale", [0.125, -0.4, 0.0])
+def test_attention_maximum_that_grows(B, H, Hkv, hd, scale):
+    """Scores whose maximum climbs from tile to tile, by little and by a lot, and falls again."""
+    n = 1000
+    c = cache_case([3] * B, H, Hkv, hd, 16, prefix_lens=[n], seed=B)
+    climb = torch.cat((torch.linspace(0.1, 2, 400), torch.linspace(2, 40, 300), torch.full((299,), 0.5), torch.tensor([100.0])))
+    c["ks"][B] = (c["ks"][B].float() * climb[:, None, None]).bfloat16()
+    from tests.paged_cases import fill
+
+    fill(c["k_pages"], c["prefix_table"], [n], [c["ks"][B]])
+    o, lse = run_attention(c, scale=scale)
+    check_attention(o, lse, attention_oracle(c["q"], c["ks"], c["vs"], [0] * B, scale=scale), hd)
+
+
+@pytest.mark.parametrize("B", [4, 30, 90])
+def test_attention_prefix_special_values(B):
+    """A key that no query can prefer (-inf scores), a query of NaN, a page that does not exist - in every form."""
+    c = cache_case([0] * B, 6, 2, 64, 16, prefix_lens=[300], seed=B)
+    c["q"][:, :, 0] = c["q"][:, :, 0].abs() + 0.1
+    from tests.paged_cases import fill
+
+    c["ks"][B][5:200, :, 0] = float("-inf")
+    fill(c["k_pages"], c["prefix_table"], [300], [c["ks"][B]])
+    want = attention_oracle(c["q"], [k[:0] for k in c["ks"][:B]] + [torch.cat((c["ks"][B][:5], c["ks"][B][200:]))],
+                            [v[:0] for v in c["vs"][:B]] + [torch.cat((c["vs"][B][:5], c["vs"][B][200:]))], [0] * B)
+    o, lse = run_attention(c)
+    check_attention(o, lse, want, 64)
+    c["q"][B - 1, 3] = float("nan")
+    bad = torch.isnan(run_attention(c)[0]).any(-1).cpu()
+    assert int(bad.sum()) == 1 and bool(bad[B - 1, 3])
+    c["ks"][B][:, :, 0] = float("-inf")  # nothing can be preferred at all
+    fill(c["k_pages"], c["prefix_table"], [300], [c["ks"][B]])
+    o, lse = run_attention(c)
+    assert (o[: B - 1] == 0).all() and (lse[: B - 1] == -math.inf).all()
+    c["prefix_table"][0, 3] = 10**7
+    run_attention(c)
+    assert take_status() == 54
+
+
 def test_attention_is_the_same_every_time():
-    c = cache_case([5, 900, 0, 2000, 1], 18, 6, 64, 16, "token", [3000], seed=3)
-    first = run_attention(c)
-    for _ in range(3):
-        again = run_attention(c)
-        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    for lens in ([5, 900, 0, 2000, 1], list(range(40)), list(range(120))):
+        c = cache_case(lens, 18, 6, 64, 16, "token", [2900], seed=3)
+        first = run_attention(c)
+        for _ in range(3):
+            again = run_attention(c)
+            assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
