@@ -3,10 +3,12 @@
 //   tokens of the answer:             x -= frequency * count + presence
 //   x += bias[i] for every i with ids[i] = v (added in the order of the list);  x = -inf where the mask's bit v is 0.
 //
-// Bound by bytes: one read and one write of the logits.  A CTA takes kPer * threads neighbouring entries of a row, with their
-// loads in flight while it counts the row's history that falls into its range in shared memory (integer atomics: the order
-// does not matter).  Bit 31 of a count says that the prompt has the token, bit 30 that a bias waits for it: such entries are
-// left to the threads that hold the biases, so that no second array is needed and the call may work in place.
+// Bound by bytes: one read and one write of the logits.  A CTA takes a range of neighbouring entries of a row, 16 bytes a
+// thread and access, with their loads in flight while it counts the part of the row's history that falls into its range in
+// shared memory (integer atomics: the order does not matter).  Every CTA of a row reads the whole history, out of L2; eight
+// loads a thread are in flight, otherwise their latency bounds the kernel.  Bit 31 of a count says that the prompt has the
+// token, bit 30 that a bias waits for it, bit 29 that more than one does: entries with a bias are left to the threads that hold
+// the biases, so that no second array is needed and the call may work in place.
 #include "common.cuh"
 #include "paged.h"
 
@@ -14,7 +16,11 @@ namespace seg {
 
 namespace {
 
-constexpr uint32_t kPrompt = 1u << 31, kBiased = 1u << 30, kCount = kBiased - 1;
+constexpr uint32_t kPrompt = 1u << 31, kBiased = 1u << 30, kTwice = 1u << 29, kCount = kTwice - 1;
+constexpr int kThreads = 512;
+constexpr int kEntries = 16;                  // entries per thread
+constexpr int kRange = kThreads * kEntries;   // entries per CTA
+constexpr int kBatch = 8;                     // history loads of a thread in flight
 
 struct RowScale {
   float rep, pres, freq;
@@ -27,17 +33,60 @@ __device__ __forceinline__ float penalise(float x, uint32_t seen, const RowScale
   return x;
 }
 
-template <typename T, int kThreads, int kPer, bool kCounts>
-__global__ void __launch_bounds__(kThreads) process_logits_kernel(const LogitsParams p) {
-  constexpr int kRange = kThreads * kPer;
-  extern __shared__ uint32_t seen[];
-  __shared__ int dup;
-  const int b = blockIdx.y, v0 = blockIdx.x * kRange, n = min(kRange, p.V - v0), tid = threadIdx.x;
-  const T* x = static_cast<const T*>(p.x) + b * p.x_row + v0;
-  T* y = static_cast<T*>(p.y) + b * p.y_row + v0;
-  float f[kPer];
+// VEC neighbouring entries in one access: 16 bytes, or one entry where the rows of input and output are aligned differently.
+template <typename T, int VEC> struct Pack;
+template <> struct Pack<float, 4> {
+  float4 v;
+  __device__ void get(float* f) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+  __device__ void set(const float* f) { v = make_float4(f[0], f[1], f[2], f[3]); }
+};
+template <> struct Pack<__nv_bfloat16, 8> {
+  bf16x8 v;
+  __device__ void get(float* f) const { unpack8(v, f); }
+  __device__ void set(const float* f) { v = pack8(f); }
+};
+template <typename T> struct Pack<T, 1> {
+  T v;
+  __device__ void get(float* f) const { f[0] = to_f<T>(v); }
+  __device__ void set(const float* f) { v = from_f<T>(f[0]); }
+};
+
+template <typename Tok>
+__device__ __forceinline__ void count_history(const Tok* tokens, int len, int prompt, int lo, int n, int base, uint32_t* seen) {
+  for (int i0 = threadIdx.x; i0 < len; i0 += kBatch * kThreads) {
+    Tok tok[kBatch];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) f[i] = i * kThreads + tid < n ? to_f<T>(x[i * kThreads + tid]) : 0.f;
+    for (int j = 0; j < kBatch; ++j) tok[j] = i0 + j * kThreads < len ? tokens[i0 + j * kThreads] : (Tok)-1;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (tok[j] < (Tok)lo || tok[j] - (Tok)lo >= (Tok)n) continue;
+      uint32_t* at = &seen[(int)tok[j] - base];
+      if (i0 + j * kThreads < prompt) atomicOr(at, kPrompt);
+      else atomicAdd(at, 1u);
+    }
+  }
+}
+
+template <typename T, int VEC, bool kCounts>
+__global__ void __launch_bounds__(kThreads) process_logits_kernel(const LogitsParams p) {
+  constexpr int kVecs = kEntries / VEC;
+  extern __shared__ uint4 seen4[];  // [kRange + VEC] counts
+  uint32_t* seen = reinterpret_cast<uint32_t*>(seen4);
+  const int b = blockIdx.y, tid = threadIdx.x;
+  const T* x = static_cast<const T*>(p.x) + b * p.x_row;
+  T* y = static_cast<T*>(p.y) + b * p.y_row;
+  // The vectors of a row start at its first aligned entry; the entries before it belong to the first CTA.  base: the entry
+  // that the first count stands for.
+  const int head = VEC == 1 ? 0 : (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T);
+  const int first = head + blockIdx.x * kRange, base = first - VEC;
+  const int lo = blockIdx.x == 0 ? 0 : first, hi = min(p.V, first + kRange);
+  if (lo >= hi) return;
+  Pack<T, VEC> in[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int v = first + (i * kThreads + tid) * VEC;
+    if (v + VEC <= hi) in[i] = *reinterpret_cast<const Pack<T, VEC>*>(x + v);
+  }
   const int* words = nullptr;
   if (p.mask != nullptr) {
     const int r = p.mask_rows[b];
@@ -45,70 +94,110 @@ __global__ void __launch_bounds__(kThreads) process_logits_kernel(const LogitsPa
     if (r >= 0 && r < p.n_masks) words = p.mask + r * p.mask_row;
   }
   RowScale s{1.f, 0.f, 0.f};
+  const int* ids = p.bias_ids + (int64_t)b * p.K;
   if (kCounts) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) seen[i * kThreads + tid] = 0u;
-    if (tid == 0) dup = 0;
-    if (p.repetition != nullptr) s.rep = p.repetition[b];
-    if (p.presence != nullptr) s.pres = p.presence[b];
-    if (p.frequency != nullptr) s.freq = p.frequency[b];
-    __syncthreads();
+    for (int i = tid; i < (kRange + VEC + 3) / 4; i += kThreads) seen4[i] = make_uint4(0, 0, 0, 0);
+    int len = 0, prompt = 0;
     if (p.tokens != nullptr) {
-      int len = p.token_lens[b];
+      len = p.token_lens[b];
+      if (p.prompt_lens != nullptr) prompt = p.prompt_lens[b];
       if (len < 0 || len > p.tokens_width) {
         if (tid == 0) atomicCAS(p.status, 0, kStatusLogitsLength);
         len = len < 0 ? 0 : p.tokens_width;
       }
-      const int prompt = p.prompt_lens != nullptr ? p.prompt_lens[b] : 0;
-      for (int i = tid; i < len; i += kThreads) {
-        const int64_t tok = p.tokens64 ? static_cast<const int64_t*>(p.tokens)[b * p.tokens_row + i] : static_cast<const int*>(p.tokens)[b * p.tokens_row + i];
-        const int64_t v = tok - v0;
-        if (v < 0 || v >= n) continue;
-        if (i < prompt) atomicOr(&seen[v], kPrompt);
-        else atomicAdd(&seen[v], 1u);
-      }
     }
+    if (p.repetition != nullptr) s.rep = p.repetition[b];
+    if (p.presence != nullptr) s.pres = p.presence[b];
+    if (p.frequency != nullptr) s.freq = p.frequency[b];
+    __syncthreads();
+    if (p.tokens64) count_history(static_cast<const int64_t*>(p.tokens) + b * p.tokens_row, len, prompt, lo, hi - lo, base, seen);
+    else count_history(static_cast<const int*>(p.tokens) + b * p.tokens_row, len, prompt, lo, hi - lo, base, seen);
     for (int i = tid; i < p.K; i += kThreads) {
-      const int64_t v = (int64_t)p.bias_ids[(int64_t)b * p.K + i] - v0;
-      if (v >= 0 && v < n && (atomicOr(&seen[v], kBiased) & kBiased) != 0) dup = 1;
+      const int v = ids[i];
+      if (v >= lo && v < hi && (atomicOr(&seen[v - base], kBiased) & kBiased) != 0) atomicOr(&seen[v - base], kTwice);
     }
     __syncthreads();
   }
-  const auto allowed = [&](int v) { return words == nullptr || ((words[(v0 + v) >> 5] >> ((v0 + v) & 31)) & 1) != 0; };
+  // bit j: entry v + j is allowed
+  const auto allowed = [&](int v) -> uint32_t {
+    if (words == nullptr) return ~0u;
+    const int w = v >> 5;
+    const uint32_t a = words[w];
+    if (VEC == 1 || (v & 31) + VEC <= 32) return a >> (v & 31);
+    return __funnelshift_r(a, (w + 1) * 32 < p.V ? (uint32_t)words[w + 1] : 0u, v & 31);
+  };
+  const auto entry = [&](int v) {  // one entry by itself
+    const uint32_t c = kCounts ? seen[v - base] : 0u;
+    if (c & kBiased) return;
+    const float f = to_f<T>(x[v]);
+    y[v] = from_f<T>(allowed(v) & 1 ? (c != 0 ? penalise(f, c, s) : f) : -INFINITY);
+  };
+  if (VEC > 1 && blockIdx.x == 0 && tid < min(head, p.V)) entry(tid);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int v = i * kThreads + tid;
-    if (v >= n) continue;
-    const uint32_t c = kCounts ? seen[v] : 0u;
-    if (c & kBiased) continue;
-    const float r = c != 0 ? penalise(f[i], c, s) : f[i];
-    y[v] = from_f<T>(allowed(v) ? r : -INFINITY);
+  for (int i = 0; i < kVecs; ++i) {
+    const int v = first + (i * kThreads + tid) * VEC;
+    if (v + VEC > hi) {  // the row's end
+      for (int j = v; j < hi; ++j) entry(j);
+      continue;
+    }
+    float f[VEC];
+    in[i].get(f);
+    uint32_t c[VEC], any = 0;
+    if (kCounts) {
+      if constexpr (VEC > 1) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) *reinterpret_cast<uint4*>(c + j) = seen4[(v - base + j) / 4];
+      } else {
+        c[0] = seen[v - base];
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) any |= c[j];
+    }
+    if (any != 0) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (c[j] != 0) f[j] = penalise(f[j], c[j], s);
+    }
+    const uint32_t ok = allowed(v);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (((ok >> j) & 1) == 0) f[j] = -INFINITY;
+    if (any & kBiased) {  // those with a bias are not written here
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if ((c[j] & kBiased) == 0) y[v + j] = from_f<T>(f[j]);
+    } else {
+      Pack<T, VEC> out;
+      out.set(f);
+      *reinterpret_cast<Pack<T, VEC>*>(y + v) = out;
+    }
   }
   if (kCounts && p.K > 0) {
-    const int* ids = p.bias_ids + (int64_t)b * p.K;
     const float* bias = p.bias + (int64_t)b * p.K;
     for (int i = tid; i < p.K; i += kThreads) {
-      const int64_t v = (int64_t)ids[i] - v0;
-      if (v < 0 || v >= n) continue;
-      float r = penalise(to_f<T>(x[v]), seen[v], s) + bias[i];
-      if (dup) {  // an id given more than once: the first entry's thread adds them all
-        bool first = true;
-        for (int j = 0; j < i && first; ++j) first = ids[j] != ids[i];
-        if (!first) continue;
+      const int v = ids[i];
+      if (v < lo || v >= hi) continue;
+      const uint32_t c = seen[v - base];
+      float r = penalise(to_f<T>(x[v]), c, s) + bias[i];
+      if (c & kTwice) {  // the first entry's thread adds them all
+        bool mine = true;
+#pragma unroll 8
+        for (int j = 0; j < i; ++j) mine &= ids[j] != v;
+        if (!mine) continue;
+#pragma unroll 8
         for (int j = i + 1; j < p.K; ++j)
-          if (ids[j] == ids[i]) r += bias[j];
+          if (ids[j] == v) r += bias[j];
       }
-      y[v] = from_f<T>(allowed((int)v) ? r : -INFINITY);
+      y[v] = from_f<T>(allowed(v) & 1 ? r : -INFINITY);
     }
   }
 }
 
-template <typename T, int kThreads, int kPer>
+template <typename T, int VEC>
 int launch(const LogitsParams& p, cudaStream_t st) {
-  constexpr int kRange = kThreads * kPer;
   const dim3 grid((p.V + kRange - 1) / kRange, p.B);
-  if (p.tokens != nullptr || p.K > 0) process_logits_kernel<T, kThreads, kPer, true><<<grid, kThreads, kRange * 4, st>>>(p);
-  else process_logits_kernel<T, kThreads, kPer, false><<<grid, kThreads, 0, st>>>(p);
+  if (p.tokens != nullptr || p.K > 0) process_logits_kernel<T, VEC, true><<<grid, kThreads, (kRange + VEC + 3) / 4 * 16, st>>>(p);
+  else process_logits_kernel<T, VEC, false><<<grid, kThreads, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
@@ -117,7 +206,11 @@ int launch(const LogitsParams& p, cudaStream_t st) {
 int process_logits(const LogitsParams& p, cudaStream_t st) {
   if (p.B == 0 || p.V == 0) return 0;
   if (p.B > 65535) return -10;
-  return p.bf16 ? launch<__nv_bfloat16, 512, 16>(p, st) : launch<float, 512, 16>(p, st);
+  const int size = p.bf16 ? 2 : 4;
+  // 16-byte accesses need every row of the output at the input's distance from a 16-byte boundary
+  const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.y)) & 15) == 0 && (p.B == 1 || ((p.x_row - p.y_row) * size & 15) == 0);
+  if (p.bf16) return aligned ? launch<__nv_bfloat16, 8>(p, st) : launch<__nv_bfloat16, 1>(p, st);
+  return aligned ? launch<float, 4>(p, st) : launch<float, 1>(p, st);
 }
 
 }  // namespace seg

@@ -5,19 +5,23 @@
 // Same formulas as qkv_post.cu; the results of token t of sequence b go to slot p % P of page table[b][p / P], where
 // p = lens[b] + (t - cu[b]), and the rotation is that of position p + pos_base[b].
 //
-// Bound by bytes: every element of the projection is read once and written once, about six operations each.  A CTA takes a
-// few whole tokens (kItems * 256 work items, an item being 16 elements of one head: 8 rotary pairs, two 16-byte loads), one
-// thread per token finds its sequence and page while the loads of all its items are already in flight; hd / 16 neighbouring
-// lanes share a head and sum its squares with shuffles.
+// Bound by bytes: every element of the projection is read once and written once, about six operations each.  A work item is 16
+// elements of one head (8 rotary pairs: two 16-byte accesses); hd / 16 neighbouring lanes share a head and sum its squares with
+// shuffles.  Few tokens: a CTA per token and an item per thread, so that the call lasts as long as one chain of dependent
+// loads (length -> page -> rotation).  Many: that chain, longer by the search for the token's sequence, would stand in front
+// of every CTA's work, so a producer warp runs it ahead and brings each group of tokens - projection rows, first values,
+// rotation rows - into a ring in shared memory with bulk copies, from which eight warps compute and store.
 #include "common.cuh"
 #include "paged.h"
+#include "sm100.cuh"
 
 namespace seg {
+
+using namespace sm100;
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 16;  // tokens of a CTA
 constexpr float kQkEps = 1e-6f;
 constexpr float kMixEps = 1e-8f;
 
@@ -66,127 +70,211 @@ __device__ __forceinline__ TokenPlace find_place(const PagedAppendParams& p, int
   return w;
 }
 
-// Loads of one item, issued before anything is known about where the token goes.
-struct Item {
-  bf16x8 x1, x2, u1, u2;
-};
-
-template <int HD, int kItems>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppendParams p, int tokens_per_cta) {
-  constexpr int HALF = HD / 2, LPH = HD / 16;
-  __shared__ TokenPlace place[kMaxTokens];
-  const int nslots = p.H + 2 * p.Hkv, nrot = p.H + p.Hkv;
-  const int t0 = blockIdx.x * tokens_per_cta;
-  const int n_tok = min(tokens_per_cta, p.T - t0);
-  const int n_items = n_tok * nslots * LPH;
-  const __nv_bfloat16* qkv = static_cast<const __nv_bfloat16*>(p.qkv);
-  const __nv_bfloat16* v1 = static_cast<const __nv_bfloat16*>(p.v1);
-  const float a1 = *p.alpha1, a2 = *p.alpha2, vs = *p.vscale, qg = *p.qgain;
-  const float c = vs * rsqrtf(a1 * a1 + a2 * a2 + kMixEps);
-  for (int base = 0; base < n_items; base += kItems * kThreads) {
-    Item it[kItems];
+// An item's 16 elements -> the finished query, key or value elements.  u1, u2: the first block's values (or nullptr).
+template <int HD>
+__device__ __forceinline__ void finish(const PagedAppendParams& p, int slot, const float* cos, const float* sin, const bf16x8* u1, const bf16x8* u2, float c,
+                                       float a1, float a2, float qg, float* x1, float* x2) {
+  if (slot < p.H + p.Hkv) {
+    float cs[8], sn[8];
+    load8<float>(cos, cs);
+    load8<float>(sin, sn);
+    float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const int item = base + i * kThreads + threadIdx.x;
-      if (item < n_items) {
-        const int sub = item % LPH, rest = item / LPH, tok = rest / nslots, slot = rest - tok * nslots;
-        const __nv_bfloat16* src = qkv + (int64_t)(t0 + tok) * p.qkv_stride + slot * HD + sub * 8;
-        it[i].x1 = *reinterpret_cast<const bf16x8*>(src);
-        it[i].x2 = *reinterpret_cast<const bf16x8*>(src + HALF);
-        if (slot >= nrot && v1 != nullptr) {
-          const __nv_bfloat16* u = v1 + ((int64_t)(t0 + tok) * p.Hkv + (slot - nrot)) * HD + sub * 8;
-          it[i].u1 = *reinterpret_cast<const bf16x8*>(u);
-          it[i].u2 = *reinterpret_cast<const bf16x8*>(u + HALF);
-        }
+    for (int j = 0; j < 8; ++j) {
+      const float r1 = x1[j] * cs[j] - x2[j] * sn[j], r2 = x1[j] * sn[j] + x2[j] * cs[j];
+      x1[j] = r1;
+      x2[j] = r2;
+      ss += r1 * r1 + r2 * r2;
+    }
+    if (p.qknorm) {
+      ss = head_sum<HD / 16>(ss);
+      const float mul = rsqrtf(ss / HD + kQkEps) * (slot < p.H ? qg : 1.f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x1[j] *= mul;
+        x2[j] *= mul;
       }
     }
+  } else {
+    float w1[8], w2[8];
+    if (u1 != nullptr) {
+      unpack8(*u1, w1);
+      unpack8(*u2, w2);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x1[j] = c * (a1 * x1[j] + a2 * (u1 != nullptr ? w1[j] : x1[j]));
+      x2[j] = c * (a1 * x2[j] + a2 * (u1 != nullptr ? w2[j] : x2[j]));
+    }
+  }
+}
+
+// Stores an item where it belongs; tokens without a place give zeros and leave the cache alone.
+template <int HD>
+__device__ __forceinline__ void store_item(const PagedAppendParams& p, int64_t t, const TokenPlace& w, int slot, int sub, const float* x1, const float* x2) {
+  constexpr int HALF = HD / 2;
+  const bf16x8 y1 = pack8(x1), y2 = pack8(x2);
+  if (slot < p.H) {
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.q) + (t * p.H + slot) * HD + sub * 8;
+    *reinterpret_cast<bf16x8*>(dst) = y1;
+    *reinterpret_cast<bf16x8*>(dst + HALF) = y2;
+    return;
+  }
+  const bool is_k = slot < p.H + p.Hkv;
+  const int h = slot - (is_k ? p.H : p.H + p.Hkv);
+  if (w.page >= 0) {
+    __nv_bfloat16* dst = is_k ? static_cast<__nv_bfloat16*>(p.pool.k) + w.page * p.pool.k_page + w.slot * p.pool.k_slot + h * p.pool.k_head
+                              : static_cast<__nv_bfloat16*>(p.pool.v) + w.page * p.pool.v_page + w.slot * p.pool.v_slot + h * p.pool.v_head;
+    *reinterpret_cast<bf16x8*>(dst + sub * 8) = y1;
+    *reinterpret_cast<bf16x8*>(dst + HALF + sub * 8) = y2;
+  }
+  void* out = is_k ? p.k_out : p.v_out;
+  if (out != nullptr) {
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(out) + (t * p.Hkv + h) * HD + sub * 8;
+    *reinterpret_cast<bf16x8*>(dst) = y1;
+    *reinterpret_cast<bf16x8*>(dst + HALF) = y2;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- a CTA per token
+template <int HD>
+__global__ void __launch_bounds__(kThreads) paged_append_few_kernel(const PagedAppendParams p) {
+  constexpr int HALF = HD / 2, LPH = HD / 16;
+  __shared__ TokenPlace place;
+  const int64_t t = blockIdx.x;
+  const int nslots = p.H + 2 * p.Hkv, nrot = p.H + p.Hkv, n_items = nslots * LPH;
+  const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.qkv) + t * p.qkv_stride;
+  for (int base = 0; base < n_items; base += kThreads) {
+    const int item = base + threadIdx.x, sub = item % LPH, slot = item / LPH;
+    const bool live = item < n_items;
+    bf16x8 x[2], u[2];
+    if (live) {  // on their way before anything is known about where the token goes
+      x[0] = *reinterpret_cast<const bf16x8*>(row + slot * HD + sub * 8);
+      x[1] = *reinterpret_cast<const bf16x8*>(row + slot * HD + HALF + sub * 8);
+      if (slot >= nrot && p.v1 != nullptr) {
+        const __nv_bfloat16* v1 = static_cast<const __nv_bfloat16*>(p.v1) + (t * p.Hkv + (slot - nrot)) * HD + sub * 8;
+        u[0] = *reinterpret_cast<const bf16x8*>(v1);
+        u[1] = *reinterpret_cast<const bf16x8*>(v1 + HALF);
+      }
+    }
+    const float a1 = *p.alpha1, a2 = *p.alpha2, qg = *p.qgain, c = *p.vscale * rsqrtf(a1 * a1 + a2 * a2 + kMixEps);
     if (base == 0) {
-      if ((int)threadIdx.x < n_tok) place[threadIdx.x] = find_place(p, t0 + threadIdx.x);
+      if (threadIdx.x == 0) place = find_place(p, (int)t);
       __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const int item = base + i * kThreads + threadIdx.x;
-      if (item >= n_items) continue;  // the LPH lanes of a head leave together: n_items is a multiple of LPH
-      const int sub = item % LPH, rest = item / LPH, tok = rest / nslots, slot = rest - tok * nslots;
-      const int64_t t = t0 + tok;
-      const TokenPlace w = place[tok];
-      float x1[8], x2[8];
-      unpack8(it[i].x1, x1);
-      unpack8(it[i].x2, x2);
-      if (w.page < 0) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x1[j] = x2[j] = 0.f;
-      } else if (slot < nrot) {
-        float cs[8], sn[8];
-        load8<float>(p.cos + (int64_t)w.pos * HALF + sub * 8, cs);
-        load8<float>(p.sin + (int64_t)w.pos * HALF + sub * 8, sn);
-        float ss = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float r1 = x1[j] * cs[j] - x2[j] * sn[j], r2 = x1[j] * sn[j] + x2[j] * cs[j];
-          x1[j] = r1;
-          x2[j] = r2;
-          ss += r1 * r1 + r2 * r2;
-        }
-        if (p.qknorm) {
-          ss = head_sum<LPH>(ss);
-          const float mul = rsqrtf(ss / HD + kQkEps) * (slot < p.H ? qg : 1.f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            x1[j] *= mul;
-            x2[j] *= mul;
-          }
-        }
-      } else {
-        float u1[8], u2[8];
-        if (v1 != nullptr) {
-          unpack8(it[i].u1, u1);
-          unpack8(it[i].u2, u2);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x1[j] = c * (a1 * x1[j] + a2 * (v1 != nullptr ? u1[j] : x1[j]));
-          x2[j] = c * (a1 * x2[j] + a2 * (v1 != nullptr ? u2[j] : x2[j]));
-        }
-      }
-      const bf16x8 y1 = pack8(x1), y2 = pack8(x2);
-      if (slot < p.H) {
-        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.q) + (t * p.H + slot) * HD + sub * 8;
-        *reinterpret_cast<bf16x8*>(dst) = y1;
-        *reinterpret_cast<bf16x8*>(dst + HALF) = y2;
-        continue;
-      }
-      const bool is_k = slot < nrot;
-      const int h = slot - (is_k ? p.H : nrot);
-      if (w.page >= 0) {
-        __nv_bfloat16* dst =
-            is_k ? static_cast<__nv_bfloat16*>(p.pool.k) + w.page * p.pool.k_page + w.slot * p.pool.k_slot + h * p.pool.k_head
-                 : static_cast<__nv_bfloat16*>(p.pool.v) + w.page * p.pool.v_page + w.slot * p.pool.v_slot + h * p.pool.v_head;
-        *reinterpret_cast<bf16x8*>(dst + sub * 8) = y1;
-        *reinterpret_cast<bf16x8*>(dst + HALF + sub * 8) = y2;
-      }
-      void* out = is_k ? p.k_out : p.v_out;
-      if (out != nullptr) {
-        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(out) + (t * p.Hkv + h) * HD + sub * 8;
-        *reinterpret_cast<bf16x8*>(dst) = y1;
-        *reinterpret_cast<bf16x8*>(dst + HALF) = y2;
+    if (!live) continue;  // the LPH lanes of a head leave together: n_items is a multiple of LPH
+    const TokenPlace w = place;
+    float x1[8] = {}, x2[8] = {};
+    if (w.page >= 0) {
+      unpack8(x[0], x1);
+      unpack8(x[1], x2);
+      const int64_t rot = (int64_t)w.pos * HALF + sub * 8;
+      finish<HD>(p, slot, p.cos + rot, p.sin + rot, p.v1 != nullptr ? &u[0] : nullptr, &u[1], c, a1, a2, qg, x1, x2);
+    }
+    store_item<HD>(p, t, w, slot, sub, x1, x2);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- a ring of token groups
+constexpr int kRing = 3;
+constexpr int kMaxTokens = 16;      // tokens of a group
+constexpr int kSmemCta = 110 * 1024;  // two CTAs share an SM
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// A stage: for each token its projection row, its v1 row, its cos and sin rows (token_bytes in all).
+template <int HD>
+__global__ void __launch_bounds__(kThreads + 32) paged_append_ring_kernel(const PagedAppendParams p, int tokens, int token_bytes) {
+  constexpr int HALF = HD / 2, LPH = HD / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ TokenPlace place[kRing][kMaxTokens];
+  __shared__ uint64_t full[kRing], empty[kRing];
+  __shared__ int abort_flag;
+  const int nslots = p.H + 2 * p.Hkv, nrot = p.H + p.Hkv;
+  const int row_bytes = nslots * HD * 2, v1_bytes = p.v1 != nullptr ? p.Hkv * HD * 2 : 0;
+  const int n_groups = (p.T + tokens - 1) / tokens, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const AbortState ab{&abort_flag, p.status};
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(smem_u32(&full[i]), 1);
+      mbar_init(smem_u32(&empty[i]), kThreads / 32);
+    }
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (warp == kThreads / 32) {
+    // a lane per token: finds its place and fetches its rows
+    int i = 0;
+    for (int g = blockIdx.x; g < n_groups; g += gridDim.x, ++i) {
+      const int st = i % kRing, t = g * tokens + lane;
+      const bool live = lane < tokens && t < p.T;
+      TokenPlace w{-1, 0, 0};
+      if (live) w = find_place(p, t);
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[st]), ((i / kRing) & 1) ^ 1, ab, 81))) break;
+      if (live) place[st][lane] = w;
+      const int n = __popc(__ballot_sync(0xffffffffu, live && w.page >= 0));
+      __syncwarp();  // the places of all lanes are written before lane 0 arrives
+      const uint32_t bar = smem_u32(&full[st]);
+      if (lane == 0) mbar_expect_tx(bar, n * (row_bytes + v1_bytes + HD * 4));
+      __syncwarp();
+      if (live && w.page >= 0) {
+        const uint32_t dst = smem_u32(smem) + (st * tokens + lane) * token_bytes;
+        bulk_load(dst, static_cast<const __nv_bfloat16*>(p.qkv) + (int64_t)t * p.qkv_stride, row_bytes, bar);
+        if (v1_bytes != 0) bulk_load(dst + row_bytes, static_cast<const __nv_bfloat16*>(p.v1) + (int64_t)t * p.Hkv * HD, v1_bytes, bar);
+        bulk_load(dst + row_bytes + v1_bytes, p.cos + (int64_t)w.pos * HALF, HD * 2, bar);
+        bulk_load(dst + row_bytes + v1_bytes + HD * 2, p.sin + (int64_t)w.pos * HALF, HD * 2, bar);
       }
     }
+  } else {
+    const float a1 = *p.alpha1, a2 = *p.alpha2, qg = *p.qgain, c = *p.vscale * rsqrtf(a1 * a1 + a2 * a2 + kMixEps);
+    int i = 0;
+    for (int g = blockIdx.x; g < n_groups; g += gridDim.x, ++i) {
+      const int st = i % kRing, t0 = g * tokens, n_items = min(tokens, p.T - t0) * nslots * LPH;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full[st]), (i / kRing) & 1, ab, 82))) break;
+      for (int item = threadIdx.x; item < n_items; item += kThreads) {  // the LPH lanes of a head stay together
+        const int sub = item % LPH, rest = item / LPH, tok = rest / nslots, slot = rest - tok * nslots;
+        const TokenPlace w = place[st][tok];
+        float x1[8] = {}, x2[8] = {};
+        if (w.page >= 0) {
+          const uint8_t* src = smem + (st * tokens + tok) * token_bytes;
+          unpack8(*reinterpret_cast<const bf16x8*>(src + (slot * HD + sub * 8) * 2), x1);
+          unpack8(*reinterpret_cast<const bf16x8*>(src + (slot * HD + HALF + sub * 8) * 2), x2);
+          const bf16x8* u = reinterpret_cast<const bf16x8*>(src + row_bytes + ((slot - nrot) * HD + sub * 8) * 2);
+          const float* cos = reinterpret_cast<const float*>(src + row_bytes + v1_bytes) + sub * 8;
+          finish<HD>(p, slot, cos, cos + HALF, v1_bytes != 0 ? u : nullptr, u + HALF / 8, c, a1, a2, qg, x1, x2);
+        }
+        store_item<HD>(p, t0 + tok, w, slot, sub, x1, x2);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&empty[st]));
+    }
+  }
+  if (*static_cast<volatile int*>(&abort_flag) != 0) {
+    for (int i = 0; i < 2000; ++i) __nanosleep(100);  // copies in flight land before the CTA's memory is given away
   }
 }
 
 template <int HD>
 int launch(const PagedAppendParams& p, cudaStream_t st) {
-  const int per_token = (p.H + 2 * p.Hkv) * (HD / 16);
-  // Few tokens: a token per CTA and an item per thread, so that the call lasts as long as one chain of dependent loads.
-  // Many: four items per thread keep enough loads in flight to saturate the memory.
-  if ((int64_t)p.T * per_token <= 148 * 2 * kThreads) {
-    paged_append_kernel<HD, 1><<<p.T, kThreads, 0, st>>>(p, 1);
+  const int nslots = p.H + 2 * p.Hkv, per_token = nslots * (HD / 16);
+  const int token_bytes = nslots * HD * 2 + (p.v1 != nullptr ? p.Hkv * HD * 2 : 0) + HD * 4;
+  int tokens = kSmemCta / kRing / token_bytes;
+  if ((int64_t)p.T * per_token <= 148 * 2 * kThreads || tokens == 0) {
+    paged_append_few_kernel<HD><<<p.T, kThreads, 0, st>>>(p);
   } else {
-    int n = 4 * kThreads / per_token;
-    n = n < 1 ? 1 : n > kMaxTokens ? kMaxTokens : n;
-    paged_append_kernel<HD, 4><<<(p.T + n - 1) / n, kThreads, 0, st>>>(p, n);
+    if (tokens > kMaxTokens) tokens = kMaxTokens;
+    static bool configured[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
+    if (!configured[dev]) {
+      if (cudaFuncSetAttribute(paged_append_ring_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemCta) != cudaSuccess) return -2;
+      configured[dev] = true;
+    }
+    const int groups = (p.T + tokens - 1) / tokens;
+    paged_append_ring_kernel<HD><<<groups < 148 * 2 ? groups : 148 * 2, kThreads + 32, kRing * tokens * token_bytes, st>>>(p, tokens, token_bytes);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
