@@ -10,30 +10,36 @@
 // leaves (m, l, unnormalised o) in fp32, and a second kernel joins the parts of every row in a fixed order (no atomics: the
 // result does not depend on timing).
 //
-// Inside a CTA each of the four warps walks over its own 16 keys of every tile, with its own ring of asynchronous copies and
-// its own running maximum and sum: no barrier is crossed until the item ends.  Scores and the weighted sum are m16n8k16 tensor
-// core products with the query heads as (padded) rows; the bound is the bytes of the cache, not the products.  Keys behind the
-// length are filled with zeros by the copy and masked by index: what lies in those slots is never read.
+// Inside a CTA each of the four warps walks over its own share of every tile, with its own ring of asynchronous copies (TMA
+// boxes that never leave a page; 16-byte copies by all lanes where the page size is no multiple of 8) and its own running
+// reference and sum: no barrier is crossed until the item ends.  Scores and the weighted sum are m16n8k16 tensor core products
+// with the query heads as (padded) rows; the bound is the bytes of the cache, so what counts is few instructions a byte.  The
+// exponentials are taken relative to a reference that is only moved when a score exceeds it by more than 2^8, which a vote
+// finds without reducing the maximum over lanes; weights are then at most 256, harmless for bf16 operands and fp32 sums.
+// Keys behind the length are masked by index and their values set to zero: what lies in those slots does not count.
 #include "paged_common.cuh"
+#include "sm100.cuh"
 
 namespace seg {
+
+using namespace sm100;
 
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kKeys = 16;               // keys per warp and step
-constexpr int kTile = kWarps * kKeys;   // keys per tile
 constexpr int kRows = 16;               // query rows per item
 constexpr int kThreads = kWarps * 32;
 
 template <int HD> struct Cfg {
-  static constexpr int kStages = HD == 128 ? 3 : 4;
+  static constexpr int kKeys = HD == 128 ? 16 : 32;        // keys per warp and step
+  static constexpr int kTile = kWarps * kKeys;             // keys per tile
+  static constexpr int kStages = HD == 128 ? 3 : HD == 64 ? 2 : 4;
   static constexpr int kChunks = HD / 8;                   // 16-byte chunks of a row
-  static constexpr int kStageBytes = 2 * kKeys * HD * 2;   // K and V of one step
+  static constexpr int kMat = kKeys * HD * 2;              // K or V of one step
+  static constexpr int kStageBytes = 2 * kMat;
   static constexpr int kRing = kStages * kStageBytes;      // per warp
 };
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
@@ -58,137 +64,220 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 // made l NaN: then the row becomes NaN, as the formula says.
 __device__ __forceinline__ float part_weight(float m, float l, float mm) { return m == -INFINITY ? l : exp2_(m - mm); }
 __device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f; }
-// Byte offset of 16-byte chunk c of row r in a [rows][HD] bf16 tile; the chunks of neighbouring rows are permuted so that the
-// eight rows that one ldmatrix phase reads fall on eight different bank groups.
+// Byte offset of 16-byte chunk c of row r in a step's K or V: blocks of 64 dims (hd 32: 32), chunks of neighbouring rows permuted
+// (the pattern that TMA writes) so that the eight rows of an ldmatrix phase fall on different banks.
 template <int HD> __device__ __forceinline__ uint32_t swz(int r, int c) {
   if (HD == 32) return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
-  return r * (HD * 2) + ((c ^ (r & 7)) << 4);
+  return (c >> 3) * (Cfg<HD>::kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
 // Addresses of one walk's keys: a list of pages and the kv head inside them.
 struct KeyWalk {
   const int* pages;
   const __nv_bfloat16 *k, *v;  // pools at the item's kv head
-  int len;
+  int kvh, len;
 };
 
-template <int HD>
-__device__ __forceinline__ void load_step(const PagedAttnParams& p, const KeyWalk& w, int key0, uint32_t stage) {
+__device__ __forceinline__ int64_t checked_page(const PagedAttnParams& p, const int* pages, int j) {
+  const int page = __ldg(pages + j);
+  if ((unsigned)page < (unsigned)p.pool.n_pages) return page;
+  atomicCAS(p.status, 0, kStatusAttnPage);
+  return -1;
+}
+
+// What a warp keeps of its ring between items: steps taken so far.
+struct Ring {
+  uint32_t base;    // shared memory of the stages
+  uint32_t full;    // mbarriers of the stages (TMA)
+  int it;
+};
+
+template <int HD, bool kTma>
+__device__ __forceinline__ void load_step(const PagedAttnParams& p, const CUtensorMap* map_k, const CUtensorMap* map_v, int box, const KeyWalk& w, int key0,
+                                          const Ring& ring, int it) {
   using C = Cfg<HD>;
   const int lane = threadIdx.x & 31;
-  constexpr int kRowsPer = 32 / C::kChunks;  // rows that the warp covers at once
-#pragma unroll
-  for (int i = 0; i < kKeys / kRowsPer; ++i) {
-    const int r = i * kRowsPer + lane / C::kChunks, c = lane % C::kChunks;
-    const int key = key0 + r;
-    bool live = key < w.len;
-    int64_t page = 0;
-    int slot = 0;
-    if (live) {
-      const int j = p.pool.shift >= 0 ? key >> p.pool.shift : key / p.pool.P;
-      slot = key - j * p.pool.P;
-      page = __ldg(w.pages + j);
-      if ((uint64_t)page >= (uint64_t)p.pool.n_pages) {
-        atomicCAS(p.status, 0, kStatusAttnPage);
-        live = false;
-        page = 0;
-        slot = 0;
+  const int st = it % C::kStages;
+  const uint32_t stage = ring.base + st * C::kStageBytes;
+  if constexpr (kTma) {
+    // a lane per box: K or V, block of dims, tokens
+    constexpr int kBlocks = HD / 64 > 0 ? HD / 64 : 1;
+    const uint32_t bar = ring.full + st * 8;
+    if (lane == 0) mbar_expect_tx(bar, C::kStageBytes);
+    __syncwarp();
+    if (lane < 2 * kBlocks * (C::kKeys / box)) {
+      const int kv = lane & 1, blk = (lane >> 1) % kBlocks, b = (lane >> 1) / kBlocks, key = key0 + b * box;
+      int page = p.pool.n_pages, slot = 0;  // outside the pool: zeros
+      if (key < w.len) {
+        const int j = p.pool.shift >= 0 ? key >> p.pool.shift : key / p.pool.P;
+        const int64_t found = checked_page(p, w.pages, j);
+        if (found >= 0) {
+          page = (int)found;
+          slot = key - j * p.pool.P;
+        }
       }
+      tma_load_4d(stage + kv * C::kMat + blk * (C::kKeys * 128) + b * box * (HD < 64 ? 64 : 128), kv ? map_v : map_k, bar, blk * 64, w.kvh, slot, page);
     }
-    copy16(stage + swz<HD>(r, c), w.k + page * p.pool.k_page + slot * p.pool.k_slot + c * 8, live);
-    copy16(stage + kKeys * HD * 2 + swz<HD>(r, c), w.v + page * p.pool.v_page + slot * p.pool.v_slot + c * 8, live);
+  } else {
+    constexpr int kRowsPer = 32 / C::kChunks;  // rows that the warp covers at once
+#pragma unroll
+    for (int i = 0; i < C::kKeys / kRowsPer; ++i) {
+      const int r = i * kRowsPer + lane / C::kChunks, c = lane % C::kChunks, key = key0 + r;
+      int64_t page = -1;
+      int slot = 0;
+      if (key < w.len) {
+        const int j = key / p.pool.P;
+        page = checked_page(p, w.pages, j);
+        slot = key - j * p.pool.P;
+      }
+      const bool live = page >= 0;
+      if (!live) page = slot = 0;
+      copy16(stage + swz<HD>(r, c), w.k + page * p.pool.k_page + slot * p.pool.k_slot + c * 8, live);
+      copy16(stage + C::kMat + swz<HD>(r, c), w.v + page * p.pool.v_page + slot * p.pool.v_slot + c * 8, live);
+    }
+    copy_commit();
   }
 }
 
 // kHalf: at most eight of the item's sixteen rows exist; the products' upper rows are zero and their softmax is left out.
-template <int HD, bool kHalf>
-__device__ __forceinline__ void walk(const PagedAttnParams& p, const KeyWalk& w, const uint32_t (*qf)[4], int key0, int steps, uint32_t ring, float (*o)[4],
-                                     float* m, float* l) {
+// Returns false when a wait gave up.
+template <int HD, bool kTma, bool kHalf>
+__device__ __forceinline__ bool walk(const PagedAttnParams& p, const CUtensorMap* map_k, const CUtensorMap* map_v, int box, const KeyWalk& w,
+                                     const uint32_t (*qf)[4], int key0, int steps, Ring& ring, const AbortState& ab, float (*o)[4], float* m, float* l) {
   using C = Cfg<HD>;
+  constexpr int kN = C::kKeys / 8;      // 8-key columns of the score tile
+  constexpr int kE = kHalf ? 2 : 4;     // scores of a lane per column tile that count
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int s = 0; s < C::kStages - 1; ++s) {
-    if (s < steps) load_step<HD>(p, w, key0 + s * kTile, ring + s * C::kStageBytes);
-    copy_commit();
+    if (s < steps) load_step<HD, kTma>(p, map_k, map_v, box, w, key0 + s * C::kTile, ring, ring.it + s);
+    else if (!kTma) copy_commit();
   }
-  for (int s = 0; s < steps; ++s) {
-    copy_wait<C::kStages - 2>();
-    __syncwarp();
-    const int ahead = s + C::kStages - 1;
-    if (ahead < steps) load_step<HD>(p, w, key0 + ahead * kTile, ring + (ahead % C::kStages) * C::kStageBytes);
-    copy_commit();
-    const uint32_t sk = ring + (s % C::kStages) * C::kStageBytes, sv = sk + kKeys * HD * 2;
-    float sc[2][4] = {};
+  for (int s = 0; s < steps; ++s, ++ring.it) {
+    const int st = ring.it % C::kStages;
+    if constexpr (kTma) {
+      if (!__all_sync(0xffffffffu, mbar_wait(ring.full + st * 8, (ring.it / C::kStages) & 1, ab, 59))) return false;
+    } else {
+      copy_wait<C::kStages - 2>();
+      __syncwarp();
+    }
+    if (s + C::kStages - 1 < steps) load_step<HD, kTma>(p, map_k, map_v, box, w, key0 + (s + C::kStages - 1) * C::kTile, ring, ring.it + C::kStages - 1);
+    else if (!kTma) copy_commit();
+    const int left = w.len - (key0 + s * C::kTile);  // keys of this step that exist
+    if (left <= 0) continue;                         // none (the item's last tile)
+    const uint32_t sk = ring.base + st * C::kStageBytes, sv = sk + C::kMat;
+    float sc[kN][4] = {};
 #pragma unroll
     for (int kk = 0; kk < HD / 16; ++kk) {
-      uint32_t b[4];
-      ldsm4(b, sk + swz<HD>((lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
-      mma(sc[0], qf[kk], b[0], b[1]);
-      mma(sc[1], qf[kk], b[2], b[3]);
-    }
-    // scaled before the mask and the maximum: the scale may be zero or negative
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < (kHalf ? 2 : 4); ++e) sc[n][e] *= p.scale_log2;
-    const int left = w.len - (key0 + s * kTile);  // keys of this step that exist
-    if (left < kKeys) {
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n * 8 + (lane & 3) * 2 + (e & 1) >= left) sc[n][e] = -INFINITY;
-    }
-    uint32_t pf[4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (kHalf && h == 1) {
-        pf[1] = pf[3] = 0u;
-        continue;
+      for (int n = 0; n < kN; n += 2) {
+        uint32_t b[4];
+        ldsm4(b, sk + swz<HD>(n * 8 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
+        mma(sc[n], qf[kk], b[0], b[1]);
+        mma(sc[n + 1], qf[kk], b[2], b[3]);
       }
-      float mx = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float m_new = fmaxf(m[h], mx);
-      if (__any_sync(0xffffffffu, m_new > m[h])) {
-        const float a = m_new == -INFINITY ? 1.f : exp2_(m[h] - m_new);
+    }
+    // relative to the reference; scaled before the mask and the maximum, for the scale may be zero or negative
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int e = 0; e < kE; ++e) sc[n][e] = fmaf(sc[n][e], p.scale_log2, -ref[e >> 1]);
+    if (left < C::kKeys) {
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int e = 0; e < kE; ++e)
+          if (n * 8 + (lane & 3) * 2 + (e & 1) >= left) sc[n][e] = -INFINITY;
+      if (kTma) {  // a box may bring slots behind the length: their values must not meet the weights of zero
+        for (int i = left * C::kChunks + lane; i < C::kKeys * C::kChunks; i += 32)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + swz<HD>(i / C::kChunks, i % C::kChunks)), "r"(0) : "memory");
+        fence_proxy_async();
+        __syncwarp();
+      }
+    }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int e = 0; e < kE; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], sc[n][e]);
+    bool low = mx[0] > 8.f || (m[0] == -INFINITY && mx[0] > -INFINITY);
+    if (!kHalf) low = low || mx[1] > 8.f || (m[1] == -INFINITY && mx[1] > -INFINITY);
+    if (__any_sync(0xffffffffu, low)) {  // move the references to the maxima (always in an item's first step, rarely after it)
+#pragma unroll
+      for (int h = 0; h < (kHalf ? 1 : 2); ++h) {
+        float t = mx[h];
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+        const float m_new = fmaxf(m[h], ref[h] + t);
+        if (m_new == -INFINITY) continue;
+        const float a = m[h] == -INFINITY ? 1.f : exp2_(m[h] - m_new), down = m_new - ref[h];
         l[h] *= a;
 #pragma unroll
         for (int d = 0; d < HD / 8; ++d) {
           o[d][2 * h] *= a;
           o[d][2 * h + 1] *= a;
         }
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          sc[n][2 * h] -= down;
+          sc[n][2 * h + 1] -= down;
+        }
         m[h] = m_new;
       }
-      const float base = m_new == -INFINITY ? 0.f : m_new;  // nothing seen yet: every score is -inf and its weight exp2(-inf) = 0
-      float e[4];
+    }
+    uint32_t pf[kN / 2][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = exp2_(sc[i >> 1][2 * h + (i & 1)] - base);
-      l[h] += (e[0] + e[1]) + (e[2] + e[3]);
-      pf[h] = pack_bf16(e[0], e[1]);      // weights <= 1 rounded to bf16 (2^-9 relative), as operands of the tensor core
-      pf[2 + h] = pack_bf16(e[2], e[3]);
+    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (kHalf && h == 1) {
+          pf[n / 2][(n & 1) * 2 + 1] = 0u;
+          continue;
+        }
+        const float e0 = exp2_(sc[n][2 * h]), e1 = exp2_(sc[n][2 * h + 1]);
+        l[h] += e0 + e1;
+        pf[n / 2][(n & 1) * 2 + h] = pack_bf16(e0, e1);  // weights rounded to bf16 (2^-9 relative), as operands of the tensor core
+      }
     }
 #pragma unroll
-    for (int dd = 0; dd < HD / 16; ++dd) {
-      uint32_t b[4];
-      ldsm4t(b, sv + swz<HD>((lane & 7) + ((lane >> 3) & 1) * 8, dd * 2 + (lane >> 4)));
-      mma(o[2 * dd], pf, b[0], b[1]);
-      mma(o[2 * dd + 1], pf, b[2], b[3]);
+    for (int kk = 0; kk < kN / 2; ++kk) {
+#pragma unroll
+      for (int dd = 0; dd < HD / 16; ++dd) {
+        uint32_t b[4];
+        ldsm4t(b, sv + swz<HD>(kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, dd * 2 + (lane >> 4)));
+        mma(o[2 * dd], pf[kk], b[0], b[1]);
+        mma(o[2 * dd + 1], pf[kk], b[2], b[3]);
+      }
     }
     __syncwarp();
   }
-  copy_wait<0>();
+  if (!kTma) copy_wait<0>();
+  return true;
 }
 
-template <int HD>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnParams p, const Plan n, const Work ws) {
+// hd 64: at most 128 registers, so that a CTA fits next to one of the prefix kernel's
+template <int HD, bool kTma>
+__global__ void __launch_bounds__(kThreads, HD == 128 ? 2 : 4)
+paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedAttnParams p, const Plan n, const Work ws,
+                  const int box) {
   using C = Cfg<HD>;
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int kTile = C::kTile;
+  extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int warp_tot[kWarps];
+  __shared__ uint64_t full[kWarps][C::kStages];
+  __shared__ int abort_flag;
   int* sum_s = reinterpret_cast<int*>(smem + kWarps * C::kRing);
   int* sum_p = sum_s + p.B + 1;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const AbortState ab{&abort_flag, p.status};
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < kWarps * C::kStages; ++i) mbar_init(smem_u32(&full[0][0] + i), 1);
+    fence_barrier_init();
+  }
+  Ring ring{smem_u32(smem + warp * C::kRing), smem_u32(full[warp]), 0};
   scan_tiles<kThreads>(sum_s, p.B, [&](int b) { return (clamp_len(p.lens[b], p.table_width, p.pool.P, p.status) + kTile - 1) / kTile; }, warp_tot);
   const int n_groups = n.form == kPrefixSmall ? p.G : 0;
   scan_tiles<kThreads>(sum_p, n_groups, [&](int g) {
@@ -236,6 +325,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnPar
     }
     w.k = static_cast<const __nv_bfloat16*>(p.pool.k) + kvh * p.pool.k_head;
     w.v = static_cast<const __nv_bfloat16*>(p.pool.v) + kvh * p.pool.v_head;
+    w.kvh = kvh;
     const int steps = (int)min(t_end - t, (int64_t)(n_tiles - tile0));
     if (tile0 == 0 && threadIdx.x == 0) ws.meta[item] = item_parts(own ? item : item - n.items_s, t, n_tiles, ctas, total);
 
@@ -258,14 +348,14 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnPar
     // ---- this warp's keys
     float o[HD / 8][4] = {};
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    uint8_t* ring = smem + warp * C::kRing;
-    const int key0 = tile0 * kTile + warp * kKeys;
-    if (rows <= 8) walk<HD, true>(p, w, qf, key0, steps, smem_addr(ring), o, m, l);
-    else walk<HD, false>(p, w, qf, key0, steps, smem_addr(ring), o, m, l);
+    uint8_t* mine = smem + warp * C::kRing;
+    const int key0 = tile0 * kTile + warp * C::kKeys;
+    if (rows <= 8) walk<HD, kTma, true>(p, &map_k, &map_v, box, w, qf, key0, steps, ring, ab, o, m, l);
+    else walk<HD, kTma, false>(p, &map_k, &map_v, box, w, qf, key0, steps, ring, ab, o, m, l);
 
     // ---- join the four warps: every warp's (m, l, o) into its own ring, then each thread sums its columns
-    float* part = reinterpret_cast<float*>(ring);                      // [16][HD]
-    float2* part_ml = reinterpret_cast<float2*>(ring + kRows * HD * 4);  // [16]
+    float* part = reinterpret_cast<float*>(mine);                      // [16][HD]
+    float2* part_ml = reinterpret_cast<float2*>(mine + kRows * HD * 4);  // [16]
     static_assert(kRows * HD * 4 + kRows * 8 <= C::kRing, "a warp's part must fit into its ring");
     __syncwarp();
 #pragma unroll
@@ -316,12 +406,16 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnPar
         if (c == 0) (own ? ws.ml_s : ws.ml_p)[slot * slot_rows + r] = make_float2(mm, ll);
       }
     }
+    fence_proxy_async();  // these reads and writes, before the next item's copies
     __syncthreads();
     t += steps;
   }
   // The prefix kernel before this one let it start early.  It must have ended when this one ends, for the join waits for this
   // one alone.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (*static_cast<volatile int*>(&abort_flag) != 0) {
+    for (int i = 0; i < 2000; ++i) __nanosleep(100);  // copies in flight land before the CTA's memory is given away
+  }
 }
 
 // Joins the parts of one (row, head): the prefix's, then the sequence's own, in order.
@@ -422,7 +516,7 @@ Plan make_plan(const PagedAttnParams& p) {
   n.items_p = p.G > 0 ? p.Hkv * (int)((int64_t)p.B * n.gqa / n.rows_p + p.G + 1) : 0;
   // one resident wave, but no more CTAs than there can be tiles
   const int per_sm = p.hd == 128 || p.B + p.G > 2048 ? 2 : 3;
-  const int64_t P = p.pool.P;
+  const int64_t P = p.pool.P, kTile = p.hd == 128 ? Cfg<128>::kTile : Cfg<64>::kTile;
   int64_t tiles = (int64_t)n.items_s * ((p.table_width * P + kTile - 1) / kTile), tiles_p = 0;
   if (n.form == kPrefixSmall) tiles += (int64_t)n.items_p * ((p.ptable_width * P + kTile - 1) / kTile);
   else tiles_p = (int64_t)n.items_p * ((p.ptable_width * P + 127) / 128);
@@ -433,13 +527,18 @@ Plan make_plan(const PagedAttnParams& p) {
 
 int64_t round_up(int64_t n) { return (n + 255) / 256 * 256; }
 
-template <int HD>
+template <int HD, bool kTma>
 int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t st) {
+  const int box = pool_box(p.pool.P, Cfg<HD>::kKeys);
+  CUtensorMap mk = {}, mv = {};
+  if (kTma && (make_pool_map(&mk, p.pool.k, p, p.pool.k_page, p.pool.k_slot, p.pool.k_head, box) != 0 ||
+               make_pool_map(&mv, p.pool.v, p, p.pool.v_page, p.pool.v_slot, p.pool.v_head, box) != 0))
+    return -5;
   static bool configured[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
   if (!configured[dev]) {
-    if (cudaFuncSetAttribute(paged_attn_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * Cfg<HD>::kRing + (kMaxLists + 2) * 4) != cudaSuccess) return -2;
+    if (cudaFuncSetAttribute(paged_attn_kernel<HD, kTma>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * Cfg<HD>::kRing + (kMaxLists + 2) * 4) != cudaSuccess) return -2;
     configured[dev] = true;
   }
   // The kernels after the first may be brought in while the one before still runs: the walk over own pages needs nothing of the
@@ -459,7 +558,7 @@ int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t
   }
   cfg.gridDim = dim3(n.ctas);
   cfg.dynamicSmemBytes = smem_bytes<HD>(p);
-  if (cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD>, p, n, ws) != cudaSuccess) return -3;
+  if (cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD, kTma>, mk, mv, p, n, ws, box) != cudaSuccess) return -3;
   cfg.numAttrs = 1;
   cfg.gridDim = dim3(p.B, p.H);
   cfg.dynamicSmemBytes = 0;
@@ -492,10 +591,11 @@ int paged_attn(const PagedAttnParams& p, void* workspace, cudaStream_t st) {
   ws.ml_p = reinterpret_cast<float2*>(at);
   at += round_up(sp * 8);
   ws.meta = reinterpret_cast<int2*>(at);
+  const bool tma = pool_box(p.pool.P, 8) == 8;  // whole 8-row groups of the swizzle pattern
   switch (p.hd) {
-    case 32: return launch<32>(p, n, ws, st);
-    case 64: return launch<64>(p, n, ws, st);
-    case 128: return launch<128>(p, n, ws, st);
+    case 32: return tma ? launch<32, true>(p, n, ws, st) : launch<32, false>(p, n, ws, st);
+    case 64: return tma ? launch<64, true>(p, n, ws, st) : launch<64, false>(p, n, ws, st);
+    case 128: return tma ? launch<128, true>(p, n, ws, st) : launch<128, false>(p, n, ws, st);
   }
   return -10;
 }

@@ -1,6 +1,8 @@
 // What the kernels of the paged attention share: the plan of a call, the checked reads of lengths and group borders, and the
 // dealing of key tiles to CTAs.
 #pragma once
+#include <cuda.h>
+
 #include "common.cuh"
 #include "paged.h"
 
@@ -102,6 +104,34 @@ __device__ __forceinline__ int2 item_parts(int item, int64_t first_tile, int n_t
 }
 
 constexpr int kMaxLists = 8192;  // sequences + groups of a call (their cumulative tile counts live in shared memory)
+
+// ---- reading a pool with TMA
+// Tokens of a box: the largest power of two that divides the page (so that a box never leaves its page), at most `most`.
+inline int pool_box(int P, int most) {
+  const int box = P & -P;
+  return box < most ? box : most;
+}
+// 4-D bf16 map over a pool [pages, P, Hkv, hd] with any strides; box of (up to 64 dims) x `box` tokens, swizzled over the
+// box's rows of 128 (hd 32: 64) bytes.  A box of page n_pages lies outside and reads as zeros.
+inline int make_pool_map(CUtensorMap* map, void* base, const PagedAttnParams& p, int64_t page, int64_t slot, int64_t head, int box) {
+  typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static EncodeFn fn = nullptr;
+  if (fn == nullptr) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess) return -1;
+    fn = reinterpret_cast<EncodeFn>(ptr);
+  }
+  // a dimension of one element may have any stride in the framework; the map wants a multiple of 16 bytes
+  const cuuint64_t dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)p.Hkv, (cuuint64_t)p.pool.P, (cuuint64_t)p.pool.n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)(p.Hkv == 1 ? p.hd : head) * 2, (cuuint64_t)(p.pool.P == 1 ? p.hd : slot) * 2,
+                                 (cuuint64_t)(p.pool.n_pages == 1 ? p.hd : page) * 2};
+  const cuuint32_t boxes[4] = {(cuuint32_t)(p.hd < 64 ? p.hd : 64), 1, (cuuint32_t)box, 1}, ones[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            p.hd < 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -1;
+}
 
 // ---- paged_prefix.cu: whether the pool can be read in the tcgen05 forms, and their launch
 bool paged_prefix_usable(const PagedAttnParams& p);

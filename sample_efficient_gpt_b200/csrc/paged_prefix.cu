@@ -403,37 +403,10 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
-// 4-D bf16 map over a pool [pages, P, Hkv, hd] with any strides, a box of 64 dims x `box` tokens, 128-byte swizzle.
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-int make_pool_map(CUtensorMap* map, void* base, const PagedAttnParams& p, int64_t page, int64_t slot, int64_t head, int box) {
-  static EncodeFn fn = nullptr;
-  if (fn == nullptr) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult res;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess) return -1;
-    fn = reinterpret_cast<EncodeFn>(ptr);
-  }
-  // a dimension of one element may have any stride in the framework; the map wants a multiple of 16 bytes
-  const cuuint64_t dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)p.Hkv, (cuuint64_t)p.pool.P, (cuuint64_t)p.pool.n_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)(p.Hkv == 1 ? p.hd : head) * 2, (cuuint64_t)(p.pool.P == 1 ? p.hd : slot) * 2,
-                                 (cuuint64_t)(p.pool.n_pages == 1 ? p.hd : page) * 2};
-  const cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1}, ones[4] = {1, 1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -1;
-}
-
-// Tokens of a box: the largest power of two that divides the page, so that a box never leaves its page; whole 8-row groups of
-// the swizzle pattern.
-int box_of(int P) {
-  int box = P & -P;
-  return box > kTileKeys ? kTileKeys : box;
-}
-
 template <int HD, bool kSplit>
 int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t st) {
   using L = Lay<HD, kSplit>;
-  const int box = box_of(p.pool.P);
+  const int box = pool_box(p.pool.P, kTileKeys);
   CUtensorMap mk, mv;
   if (make_pool_map(&mk, p.pool.k, p, p.pool.k_page, p.pool.k_slot, p.pool.k_head, box) != 0 ||
       make_pool_map(&mv, p.pool.v, p, p.pool.v_page, p.pool.v_slot, p.pool.v_head, box) != 0)
@@ -453,7 +426,7 @@ int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t
 
 bool paged_prefix_usable(const PagedAttnParams& p) {
   if (p.hd != 64 && p.hd != 128) return false;
-  if (box_of(p.pool.P) < 8) return false;
+  if (pool_box(p.pool.P, 8) < 8) return false;  // whole 8-row groups of the swizzle pattern
   const int smem = (p.hd == 128 ? Lay<128, true>::kSum : Lay<64, false>::kSum) + (p.G + 1) * 4;
   return smem <= 227 * 1024;
 }
