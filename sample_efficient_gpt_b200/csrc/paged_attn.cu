@@ -418,16 +418,24 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
 }
 
-// Joins the parts of one (row, head): the prefix's, then the sequence's own, in order.
-template <int HD>
-__global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const PagedAttnParams p, const Plan n, const Work ws) {
-  __shared__ float4 acc_w[kWarps][HD / 4];
+// Joins the parts of one (row, head) - the prefix's, then the sequence's own, in order - with kSplit warps: 1, or 4 where few
+// rows with many parts each would leave the machine empty.  A lane reads one part's (m, l) and the warp's common maximum turns
+// them into weights; the sums over o then have no dependent loads.
+template <int HD, int kSplit>
+__global__ void __launch_bounds__(kThreads, 8) paged_attn_join_kernel(const PagedAttnParams p, const Plan n, const Work ws) {
+  constexpr int kPer = HD / 32;  // columns of a lane
+  __shared__ float acc_w[kWarps][HD];
   __shared__ float2 ml_w[kWarps];
-  const int b = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = h / n.gqa, hl = h - kvh * n.gqa;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int bh = kSplit == 1 ? blockIdx.x * kWarps + warp : blockIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (bh >= p.B * p.H) return;  // kSplit 1 only: no barrier follows
+  const int b = bh / p.H, h = bh - b * p.H;
+  const int kvh = h / n.gqa, hl = h - kvh * n.gqa;
   const int len = clamp_len(p.lens[b], p.table_width, p.pool.P, p.status);
   int2 parts[2] = {make_int2(0, 0), make_int2(0, 0)};
+  if (len > 0) parts[1] = ws.meta[(b * p.Hkv + kvh) * n.RT + hl / kRows];
+  if (p.G == 0 && parts[1].y == 1) return;  // written by the CTA that held the whole item (the same for all warps of the row)
   int row_p = 0;
   if (p.G > 0) {
     int g = 0;
@@ -449,52 +457,65 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const PagedAt
       parts[0].y *= n.parts_p;
     }
   }
-  if (len > 0) {
-    parts[1] = ws.meta[(b * p.Hkv + kvh) * n.RT + hl / kRows];
-    if (p.G == 0 && parts[1].y == 1) return;  // written by the CTA that held the whole item
-  }
   const int total = parts[0].y + parts[1].y;
-  float m = -INFINITY, l = 0.f;
-  constexpr int kPer = HD / 32;  // columns of a lane
-  float acc[kPer] = {};
-  for (int i = warp; i < total; i += kWarps) {
-    const bool pre = i < parts[0].y;
-    const int64_t at = pre ? (int64_t)(parts[0].x + i) * n.part_rows_p + row_p : (int64_t)(parts[1].x + i - parts[0].y) * n.rows_s + hl % kRows;
-    const float2 ml = (pre ? ws.ml_p : ws.ml_s)[at];
-    const float* src = (pre ? ws.acc_p : ws.acc_s) + at * HD + lane * kPer;
-    float x[kPer];
+  const auto place = [&](int i) {
+    return i < parts[0].y ? (int64_t)(parts[0].x + i) * n.part_rows_p + row_p : (int64_t)(parts[1].x + i - parts[0].y) * n.rows_s + hl % kRows;
+  };
+  float m = -INFINITY, l = 0.f, acc[kPer] = {};
+  constexpr int kStep = 32 * kSplit;
+  for (int i0 = (kSplit == 1 ? 0 : warp * 32); i0 < total; i0 += kStep) {
+    const int count = min(32, total - i0), i = i0 + lane;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < count) ml = (i < parts[0].y ? ws.ml_p : ws.ml_s)[place(i)];
+    const float m_new = fmaxf(m, warp_max(ml.x));
+    const float w = part_weight(ml.x, ml.y, m_new), old = part_weight(m, l, m_new);
+    l = l * old + warp_sum(w * ml.y);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) x[j] = src[j];
-    if (ml.x == -INFINITY) {
-      l += ml.y;  // 0, or NaN
-      continue;
-    }
-    const float m_new = fmaxf(m, ml.x);
-    const float a = exp2_(m - m_new), c = exp2_(ml.x - m_new);
-    l = l * a + ml.y * c;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) acc[j] = acc[j] * a + x[j] * c;
+    for (int c = 0; c < kPer; ++c) acc[c] *= old;
     m = m_new;
+    const auto add = [&](int j) {
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      const float* src = (i0 + j < parts[0].y ? ws.acc_p : ws.acc_s) + place(i0 + j) * HD + lane * kPer;
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) {
+        const float x = src[c];
+        acc[c] += wj != 0.f ? wj * x : 0.f;  // a part without weight may not have been written
+      }
+    };
+    int j = 0;
+    for (; j + 4 <= count; j += 4) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) add(j + k);
+    }
+    for (; j < count; ++j) add(j);
   }
-  float* mine = reinterpret_cast<float*>(acc_w[warp]);
+  if constexpr (kSplit > 1) {
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) mine[lane * kPer + j] = acc[j];
-  if (lane == 0) ml_w[warp] = make_float2(m, l);
-  __syncthreads();
-  const int c = threadIdx.x;
-  if (c >= HD) return;
-  float mm = -INFINITY, ll = 0.f, out = 0.f;
+    for (int c = 0; c < kPer; ++c) acc_w[warp][lane * kPer + c] = acc[c];
+    if (lane == 0) ml_w[warp] = make_float2(m, l);
+    __syncthreads();
+    if (warp != 0) return;
+    float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml_w[w].x);
+    for (int v = 0; v < kWarps; ++v) mm = fmaxf(mm, ml_w[v].x);
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const float a = part_weight(ml_w[w].x, ml_w[w].y, mm);
-    ll += a * ml_w[w].y;
-    out += a * reinterpret_cast<const float*>(acc_w[w])[c];
+    for (int c = 0; c < kPer; ++c) acc[c] = 0.f;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) {
+      const float a = part_weight(ml_w[v].x, ml_w[v].y, mm);
+      ll += a * ml_w[v].y;
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) acc[c] += a * acc_w[v][lane * kPer + c];
+    }
+    m = mm;
+    l = ll;
   }
   const int64_t at = (int64_t)b * p.H + h;
-  static_cast<__nv_bfloat16*>(p.o)[at * HD + c] = __float2bfloat16_rn(ll == 0.f ? 0.f : out / ll);
-  if (c == 0) p.lse[at] = row_lse(mm, ll);
+  __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.o) + at * HD + lane * kPer;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int c = 0; c < kPer; ++c) dst[c] = __float2bfloat16_rn(acc[c] * inv);
+  if (lane == 0) p.lse[at] = row_lse(m, l);
 }
 
 template <int HD> int smem_bytes(const PagedAttnParams& p) { return kWarps * Cfg<HD>::kRing + (p.B + p.G + 2) * (int)sizeof(int); }
@@ -519,7 +540,7 @@ Plan make_plan(const PagedAttnParams& p) {
   const int64_t P = p.pool.P, kTile = p.hd == 128 ? Cfg<128>::kTile : Cfg<64>::kTile;
   int64_t tiles = (int64_t)n.items_s * ((p.table_width * P + kTile - 1) / kTile), tiles_p = 0;
   if (n.form == kPrefixSmall) tiles += (int64_t)n.items_p * ((p.ptable_width * P + kTile - 1) / kTile);
-  else tiles_p = (int64_t)n.items_p * ((p.ptable_width * P + 127) / 128);
+  else tiles_p = (int64_t)n.items_p * ((p.ptable_width * P + 63) / 64);
   n.ctas = (int)(tiles < 148 * per_sm ? (tiles < 1 ? 1 : tiles) : 148 * per_sm);
   n.ctas_p = n.form == kPrefixSmall ? n.ctas : (int)(tiles_p < 148 ? tiles_p : 148);
   return n;
@@ -560,9 +581,10 @@ int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t
   cfg.dynamicSmemBytes = smem_bytes<HD>(p);
   if (cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD, kTma>, mk, mv, p, n, ws, box) != cudaSuccess) return -3;
   cfg.numAttrs = 1;
-  cfg.gridDim = dim3(p.B, p.H);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<HD>, p, n, ws) == cudaSuccess ? 0 : -3;
+  const bool few = p.B * p.H <= 148 * 8;
+  cfg.gridDim = dim3(few ? p.B * p.H : (p.B * p.H + kWarps - 1) / kWarps);
+  return cudaLaunchKernelEx(&cfg, few ? paged_attn_join_kernel<HD, kWarps> : paged_attn_join_kernel<HD, 1>, p, n, ws) == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace

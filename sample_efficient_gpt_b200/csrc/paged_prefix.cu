@@ -7,18 +7,22 @@
 //
 // Work: items of 256 rows (two tiles of 128 that share every key tile; kRows form) or of 128 rows whose key tiles are dealt to
 // the CTA's two halves alternately (kKeys form: fewer rows, or head_dim 128, where two query tiles would not fit into shared
-// memory).  The key tiles (128 keys) of all items in one row are dealt to one CTA per SM in equal, contiguous ranges.
+// memory).  The key tiles (128 keys; 64 in the kKeys form, which is bound by the latency of its loads and wants more of them in
+// flight) of all items in one row are dealt to one CTA per SM in equal, contiguous ranges.
 //
-// Roles of a CTA (384 threads): warp 0 loads, every lane one box of a page (2 to 16 boxes of 8 to 64 or 128 keys a tile, K and V
-// each in a ring of two; the last tile's missing keys are set to zero before the products see them); warps 1 and 2 issue the
-// products of half 0 / 1; warps 4-7 and 8-11 are the softmax of half 0 / 1, a row per thread.
+// Roles of a CTA (384 threads): warp 0 loads, every lane one box of a page (1 to 16 boxes of 8 to 128 keys a tile) into rings
+// of K and V tiles; keys behind the length come as zeros or are masked, their values are set to zero before the products see
+// them; warps 1 and 2 issue the products of half 0 / 1; warps 4-7 and 8-11 are the softmax of half 0 / 1, a row per thread.
 //
-// Bound: one exp2 per score on the special-function unit, 16 a cycle and SM: 2048 cycles for 256 x 128 scores against 1024 of
-// the tensor core at head_dim 64.  The softmax therefore takes the maximum off its critical path: the exponentials use the
-// maximum of the tiles before, and only when a new score exceeds it by more than 2^8 (rare after the first tile) is the row's
-// sum rescaled and the tile repeated from tensor memory.  Scores pass through the registers 32 columns at a time, the next
-// load in flight, which leaves room on the SM for a CTA of the kernel over own pages.
+// Bound: one exp2 per score, 16 a cycle and SM on the special-function unit: 2048 cycles for 256 x 128 scores against 1024 of
+// the tensor core at head_dim 64.  A quarter of the exponentials therefore runs as a polynomial on the FMA pipe, and the
+// softmax keeps the maximum off its critical path: the exponentials use the reference of the tiles before, and only when a
+// new score exceeds it by more than 2^8 (rare after the first tile) is the row's sum rescaled and the tile repeated from tensor
+// memory.  Scores pass through the registers 32 columns at a time, the next load in flight, which leaves room on the SM for a
+// CTA of the kernel over own pages.
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "paged_common.cuh"
 #include "sm100.cuh"
@@ -30,15 +34,40 @@ using namespace sm100;
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kTileKeys = 128;
-constexpr int kBlock = kTileKeys * 128;  // bytes of 128 rows of 64 bf16: the unit of all operand tiles
-constexpr int kPBytes = 2 * kBlock;      // P of one half: 128 x 128
+constexpr int kBlock = 128 * 128;  // bytes of 128 rows of 64 bf16: the unit of the query and P tiles
 
 template <int HD, bool kSplit> struct Lay {
-  static constexpr int kTile = HD / 64 * kBlock;        // a K or V tile
-  static constexpr int kQ = (kSplit ? 1 : 2) * kTile;   // query tiles
-  static constexpr int kK = kQ, kV = kK + 2 * kTile, kP = kV + 2 * kTile, kBars = kP + 2 * kPBytes, kSum = kBars + 256;
+  static constexpr int kKeys = kSplit ? 64 : 128;              // keys per tile
+  static constexpr int kDepth = !kSplit || HD == 128 ? 2 : 3;  // places of a ring
+  static constexpr int kRings = kSplit ? 2 : 1;                // rings: one for both halves, or one each
+  static constexpr int kSlots = kDepth * kRings;
+  static constexpr int kTileBlock = kKeys * 128;               // 64 dims of a K or V tile
+  static constexpr int kTile = HD / 64 * kTileBlock;
+  static constexpr int kQTile = HD / 64 * kBlock;
+  static constexpr int kPTile = kKeys / 64 * kBlock;           // P of one half
+  static constexpr int kK = (kSplit ? 1 : 2) * kQTile, kV = kK + kSlots * kTile, kP = kV + kSlots * kTile, kBars = kP + 2 * kPTile, kSum = kBars + 512;
 };
+
+constexpr int kPolyPairs = 1;  // of four pairs of exponentials, one takes the polynomial
+
+// 2^x for a pair on the FMA and integer pipes: x = n + f with n the nearest integer (rounding by a large constant), |f| <= 1/2, a
+// polynomial of degree 4 for 2^f (minimax of the relative error, 2.6e-6; a weight is rounded to bf16 anyway), n added to the
+// exponent.  x <= 100; below -126 the result is 2^-126 instead of 0.
+__device__ __forceinline__ void exp2_pair(uint64_t x, float& p0, float& p1) {
+  float x0, x1;
+  unpack2(x, x0, x1);
+  const uint64_t xc = pack2(fmaxf(x0, -126.f), fmaxf(x1, -126.f)), magic = pack2(12582912.f, 12582912.f);  // 1.5 * 2^23
+  const uint64_t t = add2(xc, magic), f = sub2(xc, sub2(t, magic));
+  uint64_t q = fma2(pack2(0.009570102207362652f, 0.009570102207362652f), f, pack2(0.05591785907745361f, 0.05591785907745361f));
+  q = fma2(q, f, pack2(0.240247443318367f, 0.240247443318367f));
+  q = fma2(q, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+  q = fma2(q, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+  uint32_t t0, t1, q0, q1;
+  unpack2(t, t0, t1);
+  unpack2(q, q0, q1);
+  p0 = __uint_as_float(q0 + (t0 << 23));
+  p1 = __uint_as_float(q1 + (t1 << 23));
+}
 
 struct Seg {
   int item, kvh, rows, row0, x0;  // rows r = x0 .. x0 + rows - 1 of the group: sequence row0 + r / gqa, head kvh * gqa + r % gqa
@@ -46,6 +75,7 @@ struct Seg {
   const int* pages;
 };
 
+template <int kTileKeys>
 __device__ __forceinline__ Seg find_seg(const PagedAttnParams& p, const Plan& n, const int* sum, int64_t t, int64_t t_end) {
   Seg s;
   const int g = find_list(sum, p.G, (int)(t / p.Hkv));
@@ -69,6 +99,7 @@ __global__ void __maxnreg__(128)  // of 384 threads: leaves 16384 registers for 
 paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedAttnParams p, const Plan n, const Work ws,
                     const int box) {
   using L = Lay<HD, kSplit>;
+  constexpr int kTileKeys = L::kKeys;
   extern __shared__ __align__(1024) uint8_t smem[];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need a 1024-byte aligned base
@@ -76,11 +107,12 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     return;
   }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
-  uint64_t *q_full = bars, *k_full = bars + 2, *k_empty = bars + 4, *v_full = bars + 6, *v_empty = bars + 8, *s_full = bars + 10, *s_empty = bars + 12,
-           *p_full = bars + 14, *pv_full = bars + 16, *tail = bars + 18, *q_free = bars + 19;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t *q_full = bars, *s_full = bars + 2, *s_empty = bars + 4, *p_full = bars + 6, *pv_full = bars + 8, *tail = bars + 10, *q_free = bars + 11,
+           *k_full = bars + 12, *k_empty = k_full + L::kSlots, *v_full = k_empty + L::kSlots, *v_empty = v_full + L::kSlots;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + L::kSlots);
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* warp_tot = reinterpret_cast<int*>(bars + 21);
+  int* warp_tot = reinterpret_cast<int*>(tmem_slot + 2);
+  static_assert((12 + 4 * L::kSlots) * 8 + 8 + kThreads / 32 * 4 <= 512, "the barriers must fit into their region");
   int* sum = reinterpret_cast<int*>(smem + L::kSum);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const AbortState ab{cta_abort, p.status};
@@ -89,14 +121,16 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     *cta_abort = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&q_full[i]), 4);
-      mbar_init(smem_u32(&k_full[i]), 1);
-      mbar_init(smem_u32(&v_full[i]), 1);
-      mbar_init(smem_u32(&k_empty[i]), kSplit ? 1 : 2);  // released by the products of every half that reads the tile
-      mbar_init(smem_u32(&v_empty[i]), kSplit ? 1 : 2);
       mbar_init(smem_u32(&s_full[i]), 1);
       mbar_init(smem_u32(&s_empty[i]), 4);
       mbar_init(smem_u32(&p_full[i]), 4);
       mbar_init(smem_u32(&pv_full[i]), 1);
+    }
+    for (int i = 0; i < L::kSlots; ++i) {
+      mbar_init(smem_u32(&k_full[i]), 1);
+      mbar_init(smem_u32(&v_full[i]), 1);
+      mbar_init(smem_u32(&k_empty[i]), kSplit ? 1 : 2);  // released by the products of every half that reads the tile
+      mbar_init(smem_u32(&v_empty[i]), kSplit ? 1 : 2);
     }
     mbar_init(smem_u32(tail), 1);
     mbar_init(smem_u32(q_free), 5);  // the second half's softmax warps and its issuer
@@ -123,51 +157,47 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
   if (warp == 0) {
     // ------------------------------------------------------------------------------------------------ loads
-    const int boxes = kTileKeys / box;
-    int c = 0, tails = 0, used[2] = {0, 0};  // rows form: tiles so far; keys form: tiles so far of each half, whose ring slot is its own
+    int used[2] = {0, 0}, tails = 0;  // tiles so far of each ring
     bool ok = true;
     for (int64_t t = t_begin; t < t_end && ok;) {
-      const Seg s = find_seg(p, n, sum, t, t_end);
-      for (int j = 0; j < s.steps && ok; ++j, ++c) {
-        const int st = kSplit ? j & 1 : c & 1, ph = (kSplit ? (j & 1 ? used[1]++ : used[0]++) : c >> 1) & 1;
+      const Seg s = find_seg<kTileKeys>(p, n, sum, t, t_end);
+      for (int j = 0; j < s.steps && ok; ++j) {
+        const int ring = kSplit ? j & 1 : 0, c = ring ? used[1]++ : used[0]++, st = ring * L::kDepth + c % L::kDepth, ph = (c / L::kDepth) & 1;
         const int first = (s.tile0 + j) * kTileKeys, key = first + lane * box;
-        int page = 0, slot = 0;
-        bool live = lane < boxes && key < s.len;
-        if (live) {
-          const int i = p.pool.shift >= 0 ? key >> p.pool.shift : key / p.pool.P;
-          page = s.pages[i];
-          slot = key - i * p.pool.P;
-          if ((unsigned)page >= (unsigned)p.pool.n_pages) {
+        int page = p.pool.n_pages, slot = 0;  // a box outside the pool reads as zeros
+        if (lane * box < kTileKeys && key < s.len) {
+          const int i = p.pool.shift >= 0 ? key >> p.pool.shift : key / p.pool.P, found = s.pages[i];
+          if ((unsigned)found < (unsigned)p.pool.n_pages) {
+            page = found;
+            slot = key - i * p.pool.P;
+          } else {
             atomicCAS(p.status, 0, kStatusAttnPage);
-            live = false;
           }
         }
-        const unsigned live_boxes = __ballot_sync(0xffffffffu, live);
-        const bool full = first + kTileKeys <= s.len && __popc(live_boxes) == boxes;
+        const bool cut = s.len < first + kTileKeys && s.len % box != 0;  // the last box brings slots behind the length
         // K before V: the issuer wants the next scores before it issues the products that free the place of the V tile.
 #pragma unroll
         for (int kv = 0; kv < 2 && ok; ++kv) {
           uint64_t* tile_full = kv == 0 ? &k_full[st] : &v_full[st];
-          const uint32_t dst = (kv == 0 ? L::kK : L::kV) + st * L::kTile, bar = smem_u32(full ? tile_full : tail);
+          const bool mend = kv == 1 && cut;
+          const uint32_t dst = (kv == 0 ? L::kK : L::kV) + st * L::kTile, bar = smem_u32(mend ? tail : tile_full);
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(kv == 0 ? &k_empty[st] : &v_empty[st]), ph ^ 1, ab, 61 + kv));
           if (!ok) break;
-          if (lane == 0) mbar_expect_tx(bar, __popc(live_boxes) * box * HD * 2);
+          if (lane == 0) mbar_expect_tx(bar, L::kTile);
           __syncwarp();
-          if (live) {
+          if (lane * box < kTileKeys) {
 #pragma unroll
             for (int b = 0; b < HD / 64; ++b)
-              tma_load_4d(smem_u32(smem) + dst + b * kBlock + lane * box * 128, kv == 0 ? &map_k : &map_v, bar, b * 64, s.kvh, slot, page);
+              tma_load_4d(smem_u32(smem) + dst + b * L::kTileBlock + lane * box * 128, kv == 0 ? &map_k : &map_v, bar, b * 64, s.kvh, slot, page);
           }
-          if (full) continue;
-          // Keys behind the length, and pages that do not exist: zeros, so that no weight of zero meets what lies there.
+          if (!mend) continue;
+          // values behind the length: zeros, so that no weight of zero meets what lies there
           ok = __all_sync(0xffffffffu, mbar_wait(bar, tails & 1, ab, 63));
           if (!ok) break;
           ++tails;
-          for (int i = lane; i < kTileKeys * 8; i += 32) {
-            const int r = i >> 3;
-            if (first + r < s.len && ((live_boxes >> (r / box)) & 1)) continue;
+          for (int i = (s.len - first) * 8 + lane; i < kTileKeys * 8; i += 32) {
 #pragma unroll
-            for (int b = 0; b < HD / 64; ++b) *reinterpret_cast<uint4*>(smem + dst + b * kBlock + i * 16) = make_uint4(0, 0, 0, 0);
+            for (int b = 0; b < HD / 64; ++b) *reinterpret_cast<uint4*>(smem + dst + b * L::kTileBlock + i * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async();
           __syncwarp();
@@ -182,26 +212,26 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (elect_one()) {
       constexpr uint32_t idesc_s = make_idesc_bf16(128, kTileKeys, false, false);  // Q (K-major) x K (K-major)
       constexpr uint32_t idesc_o = make_idesc_bf16(128, HD, false, true);          // P (K-major) x V (MN-major)
-      const uint64_t d_q = make_smem_desc(smem_u32(smem) + (kSplit ? 0 : x * L::kTile), 16, 1024);
-      const uint64_t d_p = make_smem_desc(smem_u32(smem + L::kP) + x * kPBytes, 16, 1024);
-      const uint32_t t_s = tmem + x * kTileKeys, t_o = tmem + 256 + x * HD;
+      const uint64_t d_q = make_smem_desc(smem_u32(smem) + (kSplit ? 0 : x * L::kQTile), 16, 1024);
+      const uint64_t d_p = make_smem_desc(smem_u32(smem + L::kP) + x * L::kPTile, 16, 1024);
+      const uint32_t t_s = tmem + x * 128, t_o = tmem + 256 + x * HD;
       int cx = 0, seg = 0;  // tiles of this half, segments
       bool ok = true;
       for (int64_t t = t_begin; t < t_end && ok; ++seg) {
-        const Seg s = find_seg(p, n, sum, t, t_end);
+        const Seg s = find_seg<kTileKeys>(p, n, sum, t, t_end);
         const int mine = kSplit ? (s.steps + 1 - x) / 2 : s.steps;
         ok = mbar_wait(smem_u32(&q_full[kSplit ? 0 : x]), seg & 1, ab, 64);  // in every segment, so that no phase is missed
         if (kSplit && x == 1 && ok) mbar_arrive(smem_u32(q_free));
         auto scores = [&](int i) {
-          const int at = cx + i, st = kSplit ? x : at & 1, ph = (kSplit ? at : at >> 1) & 1;
+          const int at = cx + i, st = (kSplit ? x * L::kDepth : 0) + at % L::kDepth, ph = (at / L::kDepth) & 1;
           if (!mbar_wait(smem_u32(&k_full[st]), ph, ab, 65)) return false;
           if (at > 0 && !mbar_wait(smem_u32(&s_empty[x]), (at - 1) & 1, ab, 66)) return false;
           const uint64_t d_k = make_smem_desc(smem_u32(smem + L::kK + st * L::kTile), 16, 1024);
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k) {
-            const uint64_t off = (uint64_t)(((k >> 2) * kBlock + (k & 3) * 32) >> 4);
-            umma_bf16(t_s, d_q + off, d_k + off, idesc_s, k > 0);
+            const uint64_t oq = (uint64_t)(((k >> 2) * kBlock + (k & 3) * 32) >> 4), ok_ = (uint64_t)(((k >> 2) * L::kTileBlock + (k & 3) * 32) >> 4);
+            umma_bf16(t_s, d_q + oq, d_k + ok_, idesc_s, k > 0);
           }
           umma_commit(smem_u32(&s_full[x]));
           umma_commit(smem_u32(&k_empty[st]));
@@ -210,9 +240,9 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (ok && mine > 0) ok = scores(0);
         for (int i = 0; i < mine && ok; ++i) {
           if (i + 1 < mine && !scores(i + 1)) { ok = false; break; }
-          const int at = cx + i, st = kSplit ? x : at & 1, ph = (kSplit ? at : at >> 1) & 1;
+          const int at = cx + i, st = (kSplit ? x * L::kDepth : 0) + at % L::kDepth, ph = (at / L::kDepth) & 1;
           if (!mbar_wait(smem_u32(&v_full[st]), ph, ab, 67) || !mbar_wait(smem_u32(&p_full[x]), at & 1, ab, 68)) { ok = false; break; }
-          const uint64_t d_v = make_smem_desc(smem_u32(smem + L::kV + st * L::kTile), kBlock, 1024);
+          const uint64_t d_v = make_smem_desc(smem_u32(smem + L::kV + st * L::kTile), L::kTileBlock, 1024);
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kTileKeys / 16; ++k)
@@ -229,15 +259,15 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     // ------------------------------------------------------------------------------------------------ softmax of half x
     const int x = (warp >> 2) - 1, sub = warp & 3, r = sub * 32 + lane;  // r: row of the half's tile == TMEM lane
     const uint32_t lane_addr = (uint32_t)(sub * 32) << 16;
-    const uint32_t t_s = tmem + x * kTileKeys + lane_addr, t_o = tmem + 256 + x * HD + lane_addr;
-    uint8_t* sP = smem + L::kP + x * kPBytes + r * 128;
+    const uint32_t t_s = tmem + x * 128 + lane_addr, t_o = tmem + 256 + x * HD + lane_addr;
+    uint8_t* sP = smem + L::kP + x * L::kPTile + r * 128;
     const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
     int cx = 0, seg = 0;
     bool ok = true;
     // tensor memory is read by whole warps: when a wait gives up, all lanes leave together
     auto wait = [&](uint64_t* bar, int parity, int code) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, ab, code)) != 0; };
     for (int64_t t = t_begin; t < t_end && ok; ++seg) {
-      const Seg s = find_seg(p, n, sum, t, t_end);
+      const Seg s = find_seg<kTileKeys>(p, n, sum, t, t_end);
       const int mine = kSplit ? (s.steps + 1 - x) / 2 : s.steps;
       if (s.tile0 == 0 && threadIdx.x == 128) ws.meta[s.item] = item_parts(s.item - n.items_s, t, s.n_tiles, ctas, total);
       const int row = (kSplit ? 0 : x * 128) + r;
@@ -248,7 +278,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (!ok) break;
       }
       if (!kSplit || x == 0) {
-        uint8_t* sQ = smem + (kSplit ? 0 : x * L::kTile) + r * 128;
+        uint8_t* sQ = smem + (kSplit ? 0 : x * L::kQTile) + r * 128;
         const int q = s.x0 + row;
         const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.q) + (s.row0 + q / n.gqa) * p.q_row + (s.kvh * n.gqa + q % n.gqa) * p.q_head;
         const bool live = row < s.rows;
@@ -271,92 +301,112 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         ok = wait(&s_full[x], at & 1, 69);
         if (!ok) break;
         tc_fence_after();
-        // The first pass uses the reference that there is (on a segment's first tile it only finds the maximum); a pass with a
-        // new reference follows where it was too low.  A third one is for scores so large that their own rounding exceeds 8.
-        for (int pass = 0;; ++pass) {
-          const bool only_max = i == 0 && pass == 0;
-          const float base = m == -INFINITY ? 0.f : m;
-          const uint64_t neg2 = pack2(-base, -base);
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          uint64_t l2[2] = {0ull, 0ull};
-          uint32_t v[2][32];
-          bool redo = false;
-          tmem_ld_32x32(t_s, v[0]);
+        // The scores of chunk c relative to the reference, and the row's running maximum of them.
+        auto scaled = [&](auto tail_tile, const uint32_t* w, int c, uint64_t neg2, uint64_t* y, float* mx) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t* w = v[c & 1];
-            tmem_ld_wait_regs(w);
-            if (c < 3) tmem_ld_32x32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
-            uint64_t y[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              y[e] = fma2(pack2(w[2 * e], w[2 * e + 1]), scale2, neg2);
-              float a, b;
-              unpack2(y[e], a, b);
-              if (left < kTileKeys) {
-                if (c * 32 + 2 * e >= left) a = -INFINITY;
-                if (c * 32 + 2 * e + 1 >= left) b = -INFINITY;
-                y[e] = pack2(a, b);
-              }
-              mx4[e & 3] = max3(mx4[e & 3], a, b);
+          for (int e = 0; e < 16; ++e) {
+            y[e] = fma2(pack2(w[2 * e], w[2 * e + 1]), scale2, neg2);
+            float a, b;
+            unpack2(y[e], a, b);
+            if (decltype(tail_tile)::value) {
+              if (c * 32 + 2 * e >= left) a = -INFINITY;
+              if (c * 32 + 2 * e + 1 >= left) b = -INFINITY;
+              y[e] = pack2(a, b);
             }
-            if (c == 3) {
-              const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-              const bool low = mx > 8.f || (m == -INFINITY && mx > -INFINITY);
-              redo = only_max || (pass < 2 && __any_sync(0xffffffffu, low));
-              if (redo) {
-                const float m_new = low ? mx + base : m;
-                if (i > 0) {  // what was summed so far is rescaled (P V of the tile before is complete: waited for at c == 0)
-                  const float a = low && m != -INFINITY ? exp2_(m - m_new) : 1.f;
-                  l *= a;
-#pragma unroll
-                  for (int o = 0; o < HD / 32; ++o) {
-                    uint32_t f[32];
-                    tmem_ld_32x32(t_o + o * 32, f);
-                    tmem_ld_wait_regs(f);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) f[e] = __float_as_uint(__uint_as_float(f[e]) * a);
-                    tmem_st_32x32(t_o + o * 32, f);
-                  }
-                  tmem_st_wait();
-                }
-                m = m_new;
-                break;
-              }
-              // the scores are in registers: the next product may overwrite them
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(smem_u32(&s_empty[x]));
-            }
-            if (only_max) continue;
-            if (c == 0 && i > 0 && pass == 0) {  // P V of the tile before has read the P tile
-              ok = wait(&pv_full[x], (at - 1) & 1, 71);
-              if (!ok) break;
-              tc_fence_after();
-            }
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-              float e[8];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                float a, b;
-                unpack2(y[q4 * 4 + k], a, b);
-                e[2 * k] = exp2_(a);
-                e[2 * k + 1] = exp2_(b);
-                l2[k & 1] = add2(l2[k & 1], pack2(e[2 * k], e[2 * k + 1]));
-              }
-              const int c16 = c * 4 + q4;  // bf16 operand tile: 16-byte chunk c16 of row r at c16 ^ (r & 7) inside its 64-column block
-              *reinterpret_cast<bf16x8*>(sP + (c16 >> 3) * kBlock + (((c16 & 7) ^ (r & 7)) << 4)) = pack8(e);
-            }
+            mx[e & 3] = max3(mx[e & 3], a, b);
           }
-          if (!ok) break;
-          if (redo) continue;
-          float a0, a1, a2, a3;
-          unpack2(l2[0], a0, a1);
-          unpack2(l2[1], a2, a3);
-          l += (a0 + a1) + (a2 + a3);
-          break;
-        }
+        };
+        constexpr int kChunks = kTileKeys / 32;
+        auto one_tile = [&](auto tail_tile) {
+          uint32_t v[2][32];
+          uint64_t y[16];
+          if (i == 0) {  // no reference yet: the tile's maximum
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld_32x32(t_s, v[0]);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              tmem_ld_wait_regs(v[c & 1]);
+              if (c + 1 < kChunks) tmem_ld_32x32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
+              scaled(tail_tile, v[c & 1], c, 0ull, y, mx);
+            }
+            m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          }
+          // A second pass where the reference was too low; a third is for scores so large that their own rounding exceeds 8.
+          for (int pass = 0;; ++pass) {
+            const float base = m == -INFINITY ? 0.f : m;
+            const uint64_t neg2 = pack2(-base, -base);
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            uint64_t l2[2] = {0ull, 0ull};
+            bool redo = false;
+            tmem_ld_32x32(t_s, v[0]);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              tmem_ld_wait_regs(v[c & 1]);
+              if (c + 1 < kChunks) tmem_ld_32x32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
+              scaled(tail_tile, v[c & 1], c, neg2, y, mx);
+              if (c == 0 && i > 0 && pass == 0) {  // P V of the tile before has read the P tile
+                if (!wait(&pv_full[x], (at - 1) & 1, 71)) {
+                  tmem_ld_wait();
+                  return false;
+                }
+                tc_fence_after();
+              }
+              if (c == kChunks - 1) {
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool low = top > 8.f || (m == -INFINITY && top > -INFINITY);
+                redo = pass < 2 && __any_sync(0xffffffffu, low);
+                if (redo) {
+                  const float m_new = low ? top + base : m;
+                  if (i > 0) {  // what was summed so far is rescaled
+                    const float a = low && m != -INFINITY ? exp2_(m - m_new) : 1.f;
+                    l *= a;
+#pragma unroll
+                    for (int o = 0; o < HD / 32; ++o) {
+                      tmem_ld_32x32(t_o + o * 32, v[0]);
+                      tmem_ld_wait_regs(v[0]);
+#pragma unroll
+                      for (int e = 0; e < 32; ++e) v[0][e] = __float_as_uint(__uint_as_float(v[0][e]) * a);
+                      tmem_st_32x32(t_o + o * 32, v[0]);
+                    }
+                    tmem_st_wait();
+                  }
+                  m = m_new;
+                  break;
+                }
+                // the scores are in registers: the next product may overwrite them
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s_empty[x]));
+              }
+#pragma unroll
+              for (int q4 = 0; q4 < 4; ++q4) {
+                float e[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  if (k == 3 && kPolyPairs != 0 && !decltype(tail_tile)::value) {
+                    exp2_pair(y[q4 * 4 + k], e[2 * k], e[2 * k + 1]);
+                  } else {
+                    float a, b;
+                    unpack2(y[q4 * 4 + k], a, b);
+                    e[2 * k] = exp2_(a);
+                    e[2 * k + 1] = exp2_(b);
+                  }
+                  l2[k & 1] = add2(l2[k & 1], pack2(e[2 * k], e[2 * k + 1]));
+                }
+                const int c16 = c * 4 + q4;  // bf16 operand tile: 16-byte chunk c16 of row r at c16 ^ (r & 7) inside its 64-column block
+                *reinterpret_cast<bf16x8*>(sP + (c16 >> 3) * kBlock + (((c16 & 7) ^ (r & 7)) << 4)) = pack8(e);
+              }
+            }
+            if (redo) continue;
+            float a0, a1, a2, a3;
+            unpack2(l2[0], a0, a1);
+            unpack2(l2[1], a2, a3);
+            const float add = (a0 + a1) + (a2 + a3);
+            l += m == -INFINITY && add == add ? 0.f : add;  // only -inf scores so far: weights of zero (the polynomial's are 2^-126)
+            return true;
+          }
+        };
+        ok = left < kTileKeys ? one_tile(std::true_type{}) : one_tile(std::false_type{});
         if (!ok) break;
         tc_fence_before();
         fence_proxy_async();  // the P tile is visible to the tensor core
@@ -406,7 +456,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 template <int HD, bool kSplit>
 int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t st) {
   using L = Lay<HD, kSplit>;
-  const int box = pool_box(p.pool.P, kTileKeys);
+  const int box = pool_box(p.pool.P, L::kKeys);
   CUtensorMap mk, mv;
   if (make_pool_map(&mk, p.pool.k, p, p.pool.k_page, p.pool.k_slot, p.pool.k_head, box) != 0 ||
       make_pool_map(&mv, p.pool.v, p, p.pool.v_page, p.pool.v_slot, p.pool.v_head, box) != 0)
