@@ -4,19 +4,20 @@
 //   o = sum exp(s_n - m) v_n / l,  lse = m + log l;   a row that sees no token: o = 0, lse = -inf.
 //
 // Work items: (sequence, kv head, 16 of its query heads) over the sequence's own pages, and (group, kv head, 16 of the group's
-// rows x query heads) over the group's prefix, which is therefore read once per 16 rows and not once per sequence.  Items are
-// cut into tiles of 64 keys; the tiles of all items in one row are dealt to the CTAs of one resident wave in equal, contiguous
-// ranges, so that ragged lengths and single long sequences fill the machine alike.  A range that does not hold an item alone
-// leaves (m, l, unnormalised o) in fp32, and a second kernel joins the parts of every row in a fixed order (no atomics: the
-// result does not depend on timing).
+// rows x query heads) over the group's prefix, which is therefore read once per 16 rows and not once per sequence (groups
+// with many rows have a kernel of their own, paged_prefix.cu).  Items are cut into steps of 32 keys (16 at head_dim 128); the
+// steps of all items in one row are dealt to the warps of one resident wave in equal, contiguous ranges, so that ragged lengths
+// and single long sequences fill the machine alike.  A range that does not hold an item alone leaves (m, l, unnormalised o) in
+// fp32, and a second kernel joins the parts of every row in a fixed order (no atomics: the result does not depend on timing).
 //
-// Inside a CTA each of the four warps walks over its own share of every tile, with its own ring of asynchronous copies (TMA
-// boxes that never leave a page; 16-byte copies by all lanes where the page size is no multiple of 8) and its own running
-// reference and sum: no barrier is crossed until the item ends.  Scores and the weighted sum are m16n8k16 tensor core products
+// A warp works alone: its own ring of asynchronous copies (TMA boxes that never leave a page; 16-byte copies by all lanes where
+// the page size is no multiple of 8) runs ahead over the borders of items, and no barrier is crossed after the plan.  Scores and the weighted sum are m16n8k16 tensor core products
 // with the query heads as (padded) rows; the bound is the bytes of the cache, so what counts is few instructions a byte.  The
 // exponentials are taken relative to a reference that is only moved when a score exceeds it by more than 2^8, which a vote
 // finds without reducing the maximum over lanes; weights are then at most 256, harmless for bf16 operands and fp32 sums.
 // Keys behind the length are masked by index and their values set to zero: what lies in those slots does not count.
+#include <algorithm>
+
 #include "paged_common.cuh"
 #include "sm100.cuh"
 
@@ -26,13 +27,14 @@ using namespace sm100;
 
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 2;               // small CTAs: one or two fit next to a CTA of the prefix kernel
+constexpr int kJoinWarps = 4;
 constexpr int kRows = 16;               // query rows per item
+constexpr int kLeast = 2;               // steps of a worker where there are few
 constexpr int kThreads = kWarps * 32;
 
 template <int HD> struct Cfg {
   static constexpr int kKeys = HD == 128 ? 16 : 32;        // keys per warp and step
-  static constexpr int kTile = kWarps * kKeys;             // keys per tile
   static constexpr int kStages = HD == 128 ? 3 : HD == 64 ? 2 : 4;
   static constexpr int kChunks = HD / 8;                   // 16-byte chunks of a row
   static constexpr int kMat = kKeys * HD * 2;              // K or V of one step
@@ -85,11 +87,93 @@ __device__ __forceinline__ int64_t checked_page(const PagedAttnParams& p, const 
   return -1;
 }
 
-// What a warp keeps of its ring between items: steps taken so far.
+// An item, and the step of it that a cursor stands at.
+struct Cursor {
+  bool own;
+  int list, i;               // sequence or group; item of it
+  int item;                  // number of the item
+  int kvh, h0, rows, row0;   // query rows r = 0 .. rows-1: sequence row0 + (h0 + r) / gqa, head kvh * gqa + (h0 + r) % gqa
+  int step, n_steps;
+  KeyWalk w;
+};
+
+struct Lists {  // cumulative steps per item of the sequences, and steps per kv head of the groups
+  const int *sum_s, *sum_p;
+  int n_groups;
+};
+
+template <int HD>
+__device__ __forceinline__ void set_item(const PagedAttnParams& p, const Plan& n, Cursor& c) {
+  constexpr int kKeys = Cfg<HD>::kKeys;
+  if (c.own) {
+    const int b = c.list;
+    c.kvh = c.i / n.RT;
+    c.h0 = (c.i - c.kvh * n.RT) * kRows;
+    c.item = b * p.Hkv * n.RT + c.i;
+    c.row0 = b;
+    c.rows = min(kRows, n.gqa - c.h0);
+    c.w.len = clamp_len(p.lens[b], p.table_width, p.pool.P, p.status);
+    c.w.pages = p.table + b * p.table_stride;
+  } else {
+    const Group g = load_group(p, c.list);
+    const int rt = row_tiles(g, n);
+    c.kvh = c.i / rt;
+    c.h0 = (c.i - c.kvh * rt) * kRows;
+    c.item = first_item(n, p, c.list, g.r0) + c.i;
+    c.row0 = g.r0;
+    c.rows = min(kRows, (g.r1 - g.r0) * n.gqa - c.h0);
+    c.w.len = g.len;
+    c.w.pages = p.ptable + c.list * p.ptable_stride;
+  }
+  c.n_steps = (c.w.len + kKeys - 1) / kKeys;
+  c.w.kvh = c.kvh;
+  c.w.k = static_cast<const __nv_bfloat16*>(p.pool.k) + c.kvh * p.pool.k_head;
+  c.w.v = static_cast<const __nv_bfloat16*>(p.pool.v) + c.kvh * p.pool.v_head;
+}
+
+// The item of step t, and the step's place in it.
+template <int HD>
+__device__ __forceinline__ Cursor cursor_at(const PagedAttnParams& p, const Plan& n, const Lists& L, int64_t steps_s, int64_t t) {
+  Cursor c;
+  c.own = t < steps_s;
+  const int per = c.own ? p.Hkv * n.RT : p.Hkv;
+  const int64_t u = c.own ? t : t - steps_s;
+  const int* sum = c.own ? L.sum_s : L.sum_p;
+  c.list = find_list(sum, c.own ? p.B : L.n_groups, (int)(u / per));
+  const int local = (int)(u - (int64_t)sum[c.list] * per);
+  c.i = 0;
+  set_item<HD>(p, n, c);
+  c.i = local / c.n_steps;
+  c.step = local - c.i * c.n_steps;
+  set_item<HD>(p, n, c);
+  return c;
+}
+
+// To the next item; there is one.
+template <int HD>
+__device__ __forceinline__ void next_item(const PagedAttnParams& p, const Plan& n, const Lists& L, Cursor& c) {
+  const int per = c.own ? p.Hkv * n.RT : p.Hkv, last = c.own ? p.B : L.n_groups;
+  const int* sum = c.own ? L.sum_s : L.sum_p;
+  c.step = 0;
+  // items of the list: its steps (of all items, per kv head or head tile) over those of one item
+  const int items = (int)((int64_t)(sum[c.list + 1] - sum[c.list]) * per / c.n_steps);
+  if (++c.i == items) {
+    c.i = 0;
+    do ++c.list;
+    while (c.list < last && sum[c.list + 1] == sum[c.list]);
+    if (c.list == last) {  // from the sequences to the groups
+      c.own = false;
+      c.list = 0;
+      while (L.sum_p[c.list + 1] == L.sum_p[c.list]) ++c.list;
+    }
+  }
+  set_item<HD>(p, n, c);
+}
+
+// What a warp keeps of its ring: steps taken so far.
 struct Ring {
-  uint32_t base;    // shared memory of the stages
-  uint32_t full;    // mbarriers of the stages (TMA)
-  int it;
+  uint32_t base;  // shared memory of the stages
+  uint32_t full;  // mbarriers of the stages (TMA)
 };
 
 template <int HD, bool kTma>
@@ -139,32 +223,15 @@ __device__ __forceinline__ void load_step(const PagedAttnParams& p, const CUtens
   }
 }
 
-// kHalf: at most eight of the item's sixteen rows exist; the products' upper rows are zero and their softmax is left out.
-// Returns false when a wait gave up.
+// One step: the keys [key0, key0 + left) of a list in stage st.  kHalf: at most eight of the item's sixteen rows exist; the
+// products' upper rows are zero and their softmax is left out.
 template <int HD, bool kTma, bool kHalf>
-__device__ __forceinline__ bool walk(const PagedAttnParams& p, const CUtensorMap* map_k, const CUtensorMap* map_v, int box, const KeyWalk& w,
-                                     const uint32_t (*qf)[4], int key0, int steps, Ring& ring, const AbortState& ab, float (*o)[4], float* m, float* l) {
+__device__ __forceinline__ void attend(const PagedAttnParams& p, int left, const uint32_t (*qf)[4], const Ring& ring, int st, float (*o)[4], float* m, float* l) {
   using C = Cfg<HD>;
   constexpr int kN = C::kKeys / 8;      // 8-key columns of the score tile
   constexpr int kE = kHalf ? 2 : 4;     // scores of a lane per column tile that count
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int s = 0; s < C::kStages - 1; ++s) {
-    if (s < steps) load_step<HD, kTma>(p, map_k, map_v, box, w, key0 + s * C::kTile, ring, ring.it + s);
-    else if (!kTma) copy_commit();
-  }
-  for (int s = 0; s < steps; ++s, ++ring.it) {
-    const int st = ring.it % C::kStages;
-    if constexpr (kTma) {
-      if (!__all_sync(0xffffffffu, mbar_wait(ring.full + st * 8, (ring.it / C::kStages) & 1, ab, 59))) return false;
-    } else {
-      copy_wait<C::kStages - 2>();
-      __syncwarp();
-    }
-    if (s + C::kStages - 1 < steps) load_step<HD, kTma>(p, map_k, map_v, box, w, key0 + (s + C::kStages - 1) * C::kTile, ring, ring.it + C::kStages - 1);
-    else if (!kTma) copy_commit();
-    const int left = w.len - (key0 + s * C::kTile);  // keys of this step that exist
-    if (left <= 0) continue;                         // none (the item's last tile)
+  {
     const uint32_t sk = ring.base + st * C::kStageBytes, sv = sk + C::kMat;
     float sc[kN][4] = {};
 #pragma unroll
@@ -250,19 +317,15 @@ __device__ __forceinline__ bool walk(const PagedAttnParams& p, const CUtensorMap
         mma(o[2 * dd + 1], pf[kk], b[2], b[3]);
       }
     }
-    __syncwarp();
   }
-  if (!kTma) copy_wait<0>();
-  return true;
 }
 
-// hd 64: at most 128 registers, so that a CTA fits next to one of the prefix kernel's
+// hd 64: at most 128 registers, so that CTAs fit next to one of the prefix kernel's
 template <int HD, bool kTma>
-__global__ void __launch_bounds__(kThreads, HD == 128 ? 2 : 4)
+__global__ void __launch_bounds__(kThreads, HD == 128 ? 4 : 8)
 paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedAttnParams p, const Plan n, const Work ws,
                   const int box) {
   using C = Cfg<HD>;
-  constexpr int kTile = C::kTile;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int warp_tot[kWarps];
   __shared__ uint64_t full[kWarps][C::kStages];
@@ -277,138 +340,99 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (int i = 0; i < kWarps * C::kStages; ++i) mbar_init(smem_u32(&full[0][0] + i), 1);
     fence_barrier_init();
   }
-  Ring ring{smem_u32(smem + warp * C::kRing), smem_u32(full[warp]), 0};
-  scan_tiles<kThreads>(sum_s, p.B, [&](int b) { return (clamp_len(p.lens[b], p.table_width, p.pool.P, p.status) + kTile - 1) / kTile; }, warp_tot);
-  const int n_groups = n.form == kPrefixSmall ? p.G : 0;
-  scan_tiles<kThreads>(sum_p, n_groups, [&](int g) {
+  const Ring ring{smem_u32(smem + warp * C::kRing), smem_u32(full[warp])};
+  Lists L{sum_s, sum_p, n.form == kPrefixSmall ? p.G : 0};
+  scan_tiles<kThreads>(sum_s, p.B, [&](int b) { return (clamp_len(p.lens[b], p.table_width, p.pool.P, p.status) + C::kKeys - 1) / C::kKeys; }, warp_tot);
+  scan_tiles<kThreads>(sum_p, L.n_groups, [&](int g) {
     const Group w = load_group(p, g);
-    return (w.len + kTile - 1) / kTile * row_tiles(w, n);
+    return (w.len + C::kKeys - 1) / C::kKeys * row_tiles(w, n);
   }, warp_tot);
   __syncthreads();
-  const int per_seq = p.Hkv * n.RT;
-  const int64_t tiles_s = (int64_t)sum_s[p.B] * per_seq;
-  const int64_t total = tiles_s + (int64_t)sum_p[n_groups] * p.Hkv;
-  const int64_t ctas = min((int64_t)gridDim.x, total);  // every one of them has a tile: the parts of an item have consecutive numbers
-  const int64_t t_end = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
-  for (int64_t t = t_end > 0 ? total * blockIdx.x / ctas : 0; t < t_end;) {
-    // ---- the item that tile t belongs to
-    KeyWalk w;
-    int item, kvh, rows, row0, h0, n_tiles, tile0;  // rows r = 0 .. rows-1 are query row row0 + (h0 + r) / gqa, head kvh * gqa + (h0 + r) % gqa
-    const bool own = t < tiles_s;
-    if (own) {
-      const int b = find_list(sum_s, p.B, (int)(t / per_seq));
-      n_tiles = sum_s[b + 1] - sum_s[b];
-      const int local = (int)(t - (int64_t)sum_s[b] * per_seq), i = local / n_tiles;
-      tile0 = local - i * n_tiles;
-      kvh = i / n.RT;
-      h0 = (i - kvh * n.RT) * kRows;
-      item = b * per_seq + i;
-      row0 = b;
-      rows = min(kRows, n.gqa - h0);
-      w.len = clamp_len(p.lens[b], p.table_width, p.pool.P, p.status);
-      w.pages = p.table + b * p.table_stride;
-    } else {
-      const int64_t tp = t - tiles_s;
-      const int g = find_list(sum_p, n_groups, (int)(tp / p.Hkv));
-      const Group gr = load_group(p, g);
-      n_tiles = (gr.len + kTile - 1) / kTile;
-      const int local = (int)(tp - (int64_t)sum_p[g] * p.Hkv), i = local / n_tiles;
-      tile0 = local - i * n_tiles;
-      const int rt = row_tiles(gr, n);
-      kvh = i / rt;
-      h0 = (i - kvh * rt) * kRows;
-      item = first_item(n, p, g, gr.r0) + i;
-      row0 = gr.r0;
-      rows = min(kRows, (gr.r1 - gr.r0) * n.gqa - h0);
-      w.len = gr.len;
-      w.pages = p.ptable + g * p.ptable_stride;
+  const int64_t steps_s = (int64_t)sum_s[p.B] * p.Hkv * n.RT, total = steps_s + (int64_t)sum_p[L.n_groups] * p.Hkv;
+  // every worker has at least kLeast steps (one worker may have less), so the parts of an item have consecutive numbers
+  const int64_t workers = min((int64_t)gridDim.x * kWarps, (total + kLeast - 1) / kLeast);
+  const int64_t worker = (int64_t)warp * gridDim.x + blockIdx.x;  // few workers: on SMs of their own
+  int64_t t = worker < workers ? total * worker / workers : 0;
+  const int64_t t_end = worker < workers ? total * (worker + 1) / workers : 0;
+  if (t < t_end) {
+    Cursor ahead = cursor_at<HD>(p, n, L, steps_s, t);  // of the loads
+    Cursor c = ahead;
+    int64_t t_ahead = t;
+    int it = 0;  // steps so far: the ring's position
+    bool ok = true;
+    const auto load_next = [&](int at) {
+      if (t_ahead < t_end) {
+        if (ahead.step == ahead.n_steps) next_item<HD>(p, n, L, ahead);
+        load_step<HD, kTma>(p, &map_k, &map_v, box, ahead.w, ahead.step * C::kKeys, ring, at);
+        ++ahead.step;
+        ++t_ahead;
+      } else if (!kTma) {
+        copy_commit();
+      }
+    };
+#pragma unroll
+    for (int s = 0; s < C::kStages - 1; ++s) load_next(s);
+    while (t < t_end && ok) {
+      const int steps = (int)min(t_end - t, (int64_t)(c.n_steps - c.step));
+      if (c.step == 0 && lane == 0) ws.meta[c.item] = item_parts(c.own ? c.item : c.item - n.items_s, t, c.n_steps, workers, total);
+      // ---- queries: the A operand, straight from memory
+      uint32_t qf[HD / 16][4];
+      const __nv_bfloat16* qrow[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = (lane >> 2) + 8 * h, x = c.h0 + r;
+        qrow[h] = r < c.rows ? static_cast<const __nv_bfloat16*>(p.q) + (c.row0 + x / n.gqa) * p.q_row + (c.kvh * n.gqa + x % n.gqa) * p.q_head : nullptr;
+      }
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const __nv_bfloat16* src = qrow[e & 1];
+          qf[kk][e] = src != nullptr ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + (lane & 3) * 2 + (e >> 1) * 8) : 0u;
+        }
+      float o[HD / 8][4] = {};
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int s = 0; s < steps; ++s, ++it) {
+        const int st = it % C::kStages;
+        if constexpr (kTma) {
+          ok = __all_sync(0xffffffffu, mbar_wait(ring.full + st * 8, (it / C::kStages) & 1, ab, 59));
+          if (!ok) break;
+        } else {
+          copy_wait<C::kStages - 2>();
+          __syncwarp();
+        }
+        load_next(it + C::kStages - 1);
+        const int left = c.w.len - (c.step + s) * C::kKeys;
+        if (c.rows <= 8) attend<HD, kTma, true>(p, left, qf, ring, st, o, m, l);
+        else attend<HD, kTma, false>(p, left, qf, ring, st, o, m, l);
+        __syncwarp();
+      }
+      // ---- the row's result, or the part of it
+      const bool whole = c.own && p.G == 0 && steps == c.n_steps;
+      const int64_t part = ((c.own ? c.item : c.item - n.items_s) + worker) * (c.own ? n.rows_s : kRows);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = (lane >> 2) + 8 * h, x = c.h0 + r, col = (lane & 3) * 2;
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        if (r >= c.rows) continue;
+        if (whole) {
+          const int64_t out = (int64_t)(c.row0 + x / n.gqa) * p.H + c.kvh * n.gqa + x % n.gqa;
+          const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
+          __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.o) + out * HD + col;
+#pragma unroll
+          for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<uint32_t*>(dst + d * 8) = pack_bf16(o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
+          if (col == 0) p.lse[out] = row_lse(m[h], l[h]);
+        } else {
+          float* dst = (c.own ? ws.acc_s : ws.acc_p) + (part + r) * HD + col;
+#pragma unroll
+          for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(dst + d * 8) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
+          if (col == 0) (c.own ? ws.ml_s : ws.ml_p)[part + r] = make_float2(m[h], l[h]);
+        }
+      }
+      t += steps;
+      if (t < t_end) next_item<HD>(p, n, L, c);
     }
-    w.k = static_cast<const __nv_bfloat16*>(p.pool.k) + kvh * p.pool.k_head;
-    w.v = static_cast<const __nv_bfloat16*>(p.pool.v) + kvh * p.pool.v_head;
-    w.kvh = kvh;
-    const int steps = (int)min(t_end - t, (int64_t)(n_tiles - tile0));
-    if (tile0 == 0 && threadIdx.x == 0) ws.meta[item] = item_parts(own ? item : item - n.items_s, t, n_tiles, ctas, total);
-
-    // ---- queries: the A operand, straight from memory
-    uint32_t qf[HD / 16][4];
-    const __nv_bfloat16* qrow[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = (lane >> 2) + 8 * h, x = h0 + r;
-      qrow[h] = r < rows ? static_cast<const __nv_bfloat16*>(p.q) + (row0 + x / n.gqa) * p.q_row + (kvh * n.gqa + x % n.gqa) * p.q_head : nullptr;
-    }
-#pragma unroll
-    for (int kk = 0; kk < HD / 16; ++kk)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const __nv_bfloat16* src = qrow[e & 1];
-        qf[kk][e] = src != nullptr ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + (lane & 3) * 2 + (e >> 1) * 8) : 0u;
-      }
-
-    // ---- this warp's keys
-    float o[HD / 8][4] = {};
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    uint8_t* mine = smem + warp * C::kRing;
-    const int key0 = tile0 * kTile + warp * C::kKeys;
-    if (rows <= 8) walk<HD, kTma, true>(p, &map_k, &map_v, box, w, qf, key0, steps, ring, ab, o, m, l);
-    else walk<HD, kTma, false>(p, &map_k, &map_v, box, w, qf, key0, steps, ring, ab, o, m, l);
-
-    // ---- join the four warps: every warp's (m, l, o) into its own ring, then each thread sums its columns
-    float* part = reinterpret_cast<float*>(mine);                      // [16][HD]
-    float2* part_ml = reinterpret_cast<float2*>(mine + kRows * HD * 4);  // [16]
-    static_assert(kRows * HD * 4 + kRows * 8 <= C::kRing, "a warp's part must fit into its ring");
-    __syncwarp();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = (lane >> 2) + 8 * h;
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      if ((lane & 3) == 0) part_ml[r] = make_float2(m[h], l[h]);
-      if (r < rows) {
-#pragma unroll
-        for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(part + r * HD + d * 8 + (lane & 3) * 2) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
-      }
-    }
-    __syncthreads();
-    const bool whole = own && p.G == 0 && steps == n_tiles;
-    const int64_t slot = (own ? item : item - n.items_s) + (int64_t)blockIdx.x;
-    const int slot_rows = own ? n.rows_s : kRows;
-    for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
-      const int r = i / (HD / 4), c = i % (HD / 4) * 4;
-      float mw[kWarps], lw[kWarps], mm = -INFINITY, ll = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int v = 0; v < kWarps; ++v) {
-        const float2 ml = reinterpret_cast<const float2*>(smem + v * C::kRing + kRows * HD * 4)[r];
-        mw[v] = ml.x;
-        lw[v] = ml.y;
-        mm = fmaxf(mm, ml.x);
-      }
-#pragma unroll
-      for (int v = 0; v < kWarps; ++v) {
-        const float a = part_weight(mw[v], lw[v], mm);
-        ll += a * lw[v];
-        const float4 x = *reinterpret_cast<const float4*>(smem + v * C::kRing + (r * HD + c) * 4);
-        acc.x += a * x.x;
-        acc.y += a * x.y;
-        acc.z += a * x.z;
-        acc.w += a * x.w;
-      }
-      const int x = h0 + r;
-      if (whole) {
-        const int64_t out = (int64_t)(row0 + x / n.gqa) * p.H + kvh * n.gqa + x % n.gqa;
-        const float inv = ll == 0.f ? 0.f : 1.f / ll;
-        store4<__nv_bfloat16>(static_cast<__nv_bfloat16*>(p.o) + out * HD + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-        if (c == 0) p.lse[out] = row_lse(mm, ll);
-      } else {
-        float* dst = (own ? ws.acc_s : ws.acc_p) + (slot * slot_rows + r) * HD + c;
-        *reinterpret_cast<float4*>(dst) = acc;
-        if (c == 0) (own ? ws.ml_s : ws.ml_p)[slot * slot_rows + r] = make_float2(mm, ll);
-      }
-    }
-    fence_proxy_async();  // these reads and writes, before the next item's copies
-    __syncthreads();
-    t += steps;
   }
   // The prefix kernel before this one let it start early.  It must have ended when this one ends, for the join waits for this
   // one alone.
@@ -422,23 +446,21 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 // rows with many parts each would leave the machine empty.  A lane reads one part's (m, l) and the warp's common maximum turns
 // them into weights; the sums over o then have no dependent loads.
 template <int HD, int kSplit>
-__global__ void __launch_bounds__(kThreads, 8) paged_attn_join_kernel(const PagedAttnParams p, const Plan n, const Work ws) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 8) paged_attn_join_kernel(const PagedAttnParams p, const Plan n, const Work ws) {
   constexpr int kPer = HD / 32;  // columns of a lane
-  __shared__ float acc_w[kWarps][HD];
-  __shared__ float2 ml_w[kWarps];
+  constexpr int kAtOnce = 8;     // parts in flight
+  __shared__ float acc_w[kJoinWarps][HD];
+  __shared__ float2 ml_w[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int bh = kSplit == 1 ? blockIdx.x * kWarps + warp : blockIdx.x;
+  const int bh = kSplit == 1 ? blockIdx.x * kJoinWarps + warp : blockIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (bh >= p.B * p.H) return;  // kSplit 1 only: no barrier follows
   const int b = bh / p.H, h = bh - b * p.H;
   const int kvh = h / n.gqa, hl = h - kvh * n.gqa;
-  const int len = clamp_len(p.lens[b], p.table_width, p.pool.P, p.status);
-  int2 parts[2] = {make_int2(0, 0), make_int2(0, 0)};
-  if (len > 0) parts[1] = ws.meta[(b * p.Hkv + kvh) * n.RT + hl / kRows];
-  if (p.G == 0 && parts[1].y == 1) return;  // written by the CTA that held the whole item (the same for all warps of the row)
-  int row_p = 0;
+  // The chain of dependent loads is the cost of this kernel: lengths and group, then both items' entries, then the parts.
+  Group gr{0, 0, 0};
+  int g = 0;
   if (p.G > 0) {
-    int g = 0;
     if (p.groups != nullptr) {
       int hi = p.G;
       while (hi - g > 1) {
@@ -446,48 +468,54 @@ __global__ void __launch_bounds__(kThreads, 8) paged_attn_join_kernel(const Page
         if (p.groups[mid] <= b) g = mid; else hi = mid;
       }
     }
-    const Group gr = load_group(p, g);
-    if (gr.len > 0 && b >= gr.r0 && b < gr.r1) {
-      const int x = (b - gr.r0) * n.gqa + hl;
-      parts[0] = ws.meta[first_item(n, p, g, gr.r0) + kvh * row_tiles(gr, n) + x / n.rows_p];
-      row_p = x % n.rows_p;
-      // out of order group rows could leave an item without its entry
-      if (parts[0].x < 0 || parts[0].y < 0 || (int64_t)parts[0].x + parts[0].y > n.items_p + n.ctas_p) parts[0] = make_int2(0, 0);
-      parts[0].x *= n.parts_p;
-      parts[0].y *= n.parts_p;
-    }
+    gr = load_group(p, g);
   }
-  const int total = parts[0].y + parts[1].y;
+  const int len = clamp_len(p.lens[b], p.table_width, p.pool.P, p.status);
+  const bool shared = gr.len > 0 && b >= gr.r0 && b < gr.r1;
+  const int x = shared ? (b - gr.r0) * n.gqa + hl : 0, row_p = x % n.rows_p;
+  int2 pre = make_int2(0, 0), own = make_int2(0, 0);
+  if (shared) pre = ws.meta[first_item(n, p, g, gr.r0) + kvh * row_tiles(gr, n) + x / n.rows_p];
+  if (len > 0) own = ws.meta[(b * p.Hkv + kvh) * n.RT + hl / kRows];
+  if (p.G == 0 && own.y == 1) return;  // written by the worker that held the whole item (the same for all warps of the row)
+  // out of order group rows could leave an item without its entry
+  if (pre.x < 0 || pre.y < 0 || (int64_t)pre.x + pre.y > n.items_p + n.ctas_p) pre = make_int2(0, 0);
+  pre.x *= n.parts_p;
+  pre.y *= n.parts_p;
+  const int total = pre.y + own.y;
   const auto place = [&](int i) {
-    return i < parts[0].y ? (int64_t)(parts[0].x + i) * n.part_rows_p + row_p : (int64_t)(parts[1].x + i - parts[0].y) * n.rows_s + hl % kRows;
+    return i < pre.y ? (int64_t)(pre.x + i) * n.part_rows_p + row_p : (int64_t)(own.x + i - pre.y) * n.rows_s + hl % kRows;
   };
   float m = -INFINITY, l = 0.f, acc[kPer] = {};
-  constexpr int kStep = 32 * kSplit;
-  for (int i0 = (kSplit == 1 ? 0 : warp * 32); i0 < total; i0 += kStep) {
-    const int count = min(32, total - i0), i = i0 + lane;
+  const int first = kSplit == 1 ? 0 : total * warp / kSplit, last = kSplit == 1 ? total : total * (warp + 1) / kSplit;
+  for (int i0 = first; i0 < last; i0 += 32) {
+    const int count = min(32, last - i0), i = i0 + lane;
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (lane < count) ml = (i < parts[0].y ? ws.ml_p : ws.ml_s)[place(i)];
-    const float m_new = fmaxf(m, warp_max(ml.x));
-    const float w = part_weight(ml.x, ml.y, m_new), old = part_weight(m, l, m_new);
-    l = l * old + warp_sum(w * ml.y);
+    if (lane < count) ml = (i < pre.y ? ws.ml_p : ws.ml_s)[place(i)];
+    float w = 0.f;
+    for (int j0 = 0; j0 < count; j0 += kAtOnce) {
+      float part[kAtOnce][kPer];
 #pragma unroll
-    for (int c = 0; c < kPer; ++c) acc[c] *= old;
-    m = m_new;
-    const auto add = [&](int j) {
-      const float wj = __shfl_sync(0xffffffffu, w, j);
-      const float* src = (i0 + j < parts[0].y ? ws.acc_p : ws.acc_s) + place(i0 + j) * HD + lane * kPer;
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int j = min(j0 + k, count - 1);
+        const float* src = (i0 + j < pre.y ? ws.acc_p : ws.acc_s) + place(i0 + j) * HD + lane * kPer;
 #pragma unroll
-      for (int c = 0; c < kPer; ++c) {
-        const float x = src[c];
-        acc[c] += wj != 0.f ? wj * x : 0.f;  // a part without weight may not have been written
+        for (int c = 0; c < kPer; ++c) part[k][c] = src[c];
       }
-    };
-    int j = 0;
-    for (; j + 4 <= count; j += 4) {
+      if (j0 == 0) {  // after the loads of the first parts
+        const float m_new = fmaxf(m, warp_max(ml.x)), old = part_weight(m, l, m_new);
+        w = part_weight(ml.x, ml.y, m_new);
+        l = l * old + warp_sum(w * ml.y);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) add(j + k);
+        for (int c = 0; c < kPer; ++c) acc[c] *= old;
+        m = m_new;
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float wj = j0 + k < count ? __shfl_sync(0xffffffffu, w, j0 + k) : 0.f;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) acc[c] += wj != 0.f ? wj * part[k][c] : 0.f;  // a part without weight may not have been written
+      }
     }
-    for (; j < count; ++j) add(j);
   }
   if constexpr (kSplit > 1) {
 #pragma unroll
@@ -497,11 +525,11 @@ __global__ void __launch_bounds__(kThreads, 8) paged_attn_join_kernel(const Page
     if (warp != 0) return;
     float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-    for (int v = 0; v < kWarps; ++v) mm = fmaxf(mm, ml_w[v].x);
+    for (int v = 0; v < kJoinWarps; ++v) mm = fmaxf(mm, ml_w[v].x);
 #pragma unroll
     for (int c = 0; c < kPer; ++c) acc[c] = 0.f;
 #pragma unroll
-    for (int v = 0; v < kWarps; ++v) {
+    for (int v = 0; v < kJoinWarps; ++v) {
       const float a = part_weight(ml_w[v].x, ml_w[v].y, mm);
       ll += a * ml_w[v].y;
 #pragma unroll
@@ -536,13 +564,16 @@ Plan make_plan(const PagedAttnParams& p) {
   n.part_rows_p = n.rows_p;
   n.items_p = p.G > 0 ? p.Hkv * (int)((int64_t)p.B * n.gqa / n.rows_p + p.G + 1) : 0;
   // one resident wave, but no more CTAs than there can be tiles
-  const int per_sm = p.hd == 128 || p.B + p.G > 2048 ? 2 : 3;
-  const int64_t P = p.pool.P, kTile = p.hd == 128 ? Cfg<128>::kTile : Cfg<64>::kTile;
-  int64_t tiles = (int64_t)n.items_s * ((p.table_width * P + kTile - 1) / kTile), tiles_p = 0;
-  if (n.form == kPrefixSmall) tiles += (int64_t)n.items_p * ((p.ptable_width * P + kTile - 1) / kTile);
+  const int64_t P = p.pool.P, keys = p.hd == 128 ? Cfg<128>::kKeys : Cfg<64>::kKeys;
+  int64_t steps = (int64_t)n.items_s * ((p.table_width * P + keys - 1) / keys), tiles_p = 0;
+  if (n.form == kPrefixSmall) steps += (int64_t)n.items_p * ((p.ptable_width * P + keys - 1) / keys);
   else tiles_p = (int64_t)n.items_p * ((p.ptable_width * P + 63) / 64);
-  n.ctas = (int)(tiles < 148 * per_sm ? (tiles < 1 ? 1 : tiles) : 148 * per_sm);
-  n.ctas_p = n.form == kPrefixSmall ? n.ctas : (int)(tiles_p < 148 ? tiles_p : 148);
+  const int smem = (p.hd == 128 ? smem_bytes<128>(p) : p.hd == 64 ? smem_bytes<64>(p) : smem_bytes<32>(p)) + 2048;
+  const int per_sm = std::max(1, std::min(228 * 1024 / smem, p.hd == 128 ? 4 : 8));
+  const int64_t ctas = (steps + kLeast - 1) / kLeast;  // worker w sits in CTA w % ctas
+  n.ctas = (int)(ctas < 148 * per_sm ? (ctas < 1 ? 1 : ctas) : 148 * per_sm);
+  n.workers = n.ctas * kWarps;
+  n.ctas_p = n.form == kPrefixSmall ? n.workers : (int)(tiles_p < 148 ? tiles_p : 148);
   return n;
 }
 
@@ -583,8 +614,9 @@ int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t
   cfg.numAttrs = 1;
   cfg.dynamicSmemBytes = 0;
   const bool few = p.B * p.H <= 148 * 8;
-  cfg.gridDim = dim3(few ? p.B * p.H : (p.B * p.H + kWarps - 1) / kWarps);
-  return cudaLaunchKernelEx(&cfg, few ? paged_attn_join_kernel<HD, kWarps> : paged_attn_join_kernel<HD, 1>, p, n, ws) == cudaSuccess ? 0 : -3;
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.gridDim = dim3(few ? p.B * p.H : (p.B * p.H + kJoinWarps - 1) / kJoinWarps);
+  return cudaLaunchKernelEx(&cfg, few ? paged_attn_join_kernel<HD, kJoinWarps> : paged_attn_join_kernel<HD, 1>, p, n, ws) == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace
@@ -593,7 +625,7 @@ int64_t paged_attn_workspace(const PagedAttnParams& p) {
   if (p.hd != 32 && p.hd != 64 && p.hd != 128) return -1;
   if (p.B + p.G > kMaxLists) return -1;
   const Plan n = make_plan(p);
-  const int64_t ss = ((int64_t)n.items_s + n.ctas) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas_p) * n.parts_p * n.part_rows_p : 0;
+  const int64_t ss = ((int64_t)n.items_s + n.workers) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas_p) * n.parts_p * n.part_rows_p : 0;
   return round_up(ss * p.hd * 4) + round_up(ss * 8) + round_up(sp * p.hd * 4) + round_up(sp * 8) + round_up(((int64_t)n.items_s + n.items_p) * 8);
 }
 
@@ -601,7 +633,7 @@ int paged_attn(const PagedAttnParams& p, void* workspace, cudaStream_t st) {
   if (p.B == 0) return 0;
   if (p.H < 1 || p.Hkv < 1 || p.H % p.Hkv != 0 || p.H > 65535 || p.B + p.G > kMaxLists) return -10;
   const Plan n = make_plan(p);
-  const int64_t ss = ((int64_t)n.items_s + n.ctas) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas_p) * n.parts_p * n.part_rows_p : 0;
+  const int64_t ss = ((int64_t)n.items_s + n.workers) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas_p) * n.parts_p * n.part_rows_p : 0;
   uint8_t* at = static_cast<uint8_t*>(workspace);
   Work ws;
   ws.acc_s = reinterpret_cast<float*>(at);

@@ -18,15 +18,15 @@ struct Plan {            // sizes that host and device derive alike
   int form;              // PrefixForm
   int rows_p, items_p;   // rows of a prefix item; upper bound on their number
   int parts_p, part_rows_p;  // parts that a CTA leaves of a prefix item, rows of each
-  int ctas;              // of the kernel over own pages (and prefixes in the small form)
-  int ctas_p;            // of the kernel over prefixes
+  int ctas, workers;     // of the kernel over own pages (and prefixes in the small form); its warps
+  int ctas_p;            // workers of the kernel over prefixes: warps, or CTAs in the tcgen05 forms
 };
 
-// Every (item, CTA) pair with work gets the part number item + CTA: both only grow along the row of tiles, so the numbers are
+// Every (item, worker) pair with work gets the part number item + worker: both only grow along the row of tiles, so the numbers are
 // distinct, and consecutive for the parts of one item.
 struct Work {
-  float* acc_s;    // [items_s + ctas, rows_s, HD]
-  float2* ml_s;    // [items_s + ctas, rows_s]
+  float* acc_s;    // [items_s + workers, rows_s, HD]
+  float2* ml_s;    // [items_s + workers, rows_s]
   float* acc_p;    // [(items_p + ctas_p) * parts_p, part_rows_p, HD]
   float2* ml_p;
   int2* meta;      // [items_s + items_p] first part and number of parts of every item that has tiles
@@ -97,7 +97,7 @@ __device__ __forceinline__ int find_list(const int* sum, int n, int t) {
   return lo;
 }
 
-// The part of item [first tile, first tile + n_tiles) of `total` tiles dealt to `ctas` CTAs: first part number and number of parts.
+// The parts of item [first tile, first tile + n_tiles) of `total` tiles dealt to `ctas` workers: first number, and how many.
 __device__ __forceinline__ int2 item_parts(int item, int64_t first_tile, int n_tiles, int64_t ctas, int64_t total) {
   const int a = (int)(((first_tile + 1) * ctas - 1) / total), b = (int)(((first_tile + n_tiles) * ctas - 1) / total);
   return make_int2(item + a, b - a + 1);
