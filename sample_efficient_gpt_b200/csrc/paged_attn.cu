@@ -30,7 +30,8 @@ namespace {
 constexpr int kWarps = 2;               // small CTAs: one or two fit next to a CTA of the prefix kernel
 constexpr int kJoinWarps = 4;
 constexpr int kRows = 16;               // query rows per item
-constexpr int kLeast = 2;               // steps of a worker where there are few
+constexpr int kLeast = 2;               // units of a worker where there are few
+constexpr int kItemCost = 1;            // what an item costs next to its steps, in steps
 constexpr int kThreads = kWarps * 32;
 
 template <int HD> struct Cfg {
@@ -87,78 +88,82 @@ __device__ __forceinline__ int64_t checked_page(const PagedAttnParams& p, const 
   return -1;
 }
 
-// An item, and the step of it that a cursor stands at.
+// An item, and the unit of it that a cursor stands at: kItemCost units for the item itself, then one per step.
 struct Cursor {
   bool own;
-  int list, i;               // sequence or group; item of it
+  int list, i, items;        // sequence or group; item of it; number of its items
   int item;                  // number of the item
   int kvh, h0, rows, row0;   // query rows r = 0 .. rows-1: sequence row0 + (h0 + r) / gqa, head kvh * gqa + (h0 + r) % gqa
-  int step, n_steps;
+  int unit, units;
   KeyWalk w;
 };
 
-struct Lists {  // cumulative steps per item of the sequences, and steps per kv head of the groups
+struct Lists {  // cumulative units per item of the sequences, and units per kv head of the groups
   const int *sum_s, *sum_p;
   int n_groups;
 };
 
 template <int HD>
-__device__ __forceinline__ void set_item(const PagedAttnParams& p, const Plan& n, Cursor& c) {
-  constexpr int kKeys = Cfg<HD>::kKeys;
+__device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + Cfg<HD>::kKeys - 1) / Cfg<HD>::kKeys + kItemCost : 0; }
+
+template <int HD>
+__device__ __forceinline__ void set_list(const PagedAttnParams& p, const Plan& n, Cursor& c) {
   if (c.own) {
-    const int b = c.list;
-    c.kvh = c.i / n.RT;
-    c.h0 = (c.i - c.kvh * n.RT) * kRows;
-    c.item = b * p.Hkv * n.RT + c.i;
-    c.row0 = b;
-    c.rows = min(kRows, n.gqa - c.h0);
-    c.w.len = clamp_len(p.lens[b], p.table_width, p.pool.P, p.status);
-    c.w.pages = p.table + b * p.table_stride;
+    c.row0 = c.list;
+    c.items = p.Hkv * n.RT;
+    c.item = c.list * c.items;
+    c.w.len = clamp_len(p.lens[c.list], p.table_width, p.pool.P, p.status);
+    c.w.pages = p.table + c.list * p.table_stride;
   } else {
     const Group g = load_group(p, c.list);
-    const int rt = row_tiles(g, n);
-    c.kvh = c.i / rt;
-    c.h0 = (c.i - c.kvh * rt) * kRows;
-    c.item = first_item(n, p, c.list, g.r0) + c.i;
     c.row0 = g.r0;
-    c.rows = min(kRows, (g.r1 - g.r0) * n.gqa - c.h0);
+    c.items = p.Hkv * row_tiles(g, n);
+    c.item = first_item(n, p, c.list, g.r0);
     c.w.len = g.len;
     c.w.pages = p.ptable + c.list * p.ptable_stride;
+    c.rows = (g.r1 - g.r0) * n.gqa;
   }
-  c.n_steps = (c.w.len + kKeys - 1) / kKeys;
+  c.units = units_of<HD>(c.w.len);
+}
+// Item i of the cursor's list; `all`: the rows of the list (a sequence's heads of a kv head, a group's rows).
+__device__ __forceinline__ void set_item(const PagedAttnParams& p, const Plan& n, Cursor& c, int i, int all) {
+  const int tiles = (all + kRows - 1) / kRows;
+  c.item += i - c.i;
+  c.i = i;
+  c.kvh = i / tiles;
+  c.h0 = (i - c.kvh * tiles) * kRows;
+  c.rows = min(kRows, all - c.h0);
   c.w.kvh = c.kvh;
   c.w.k = static_cast<const __nv_bfloat16*>(p.pool.k) + c.kvh * p.pool.k_head;
   c.w.v = static_cast<const __nv_bfloat16*>(p.pool.v) + c.kvh * p.pool.v_head;
 }
 
-// The item of step t, and the step's place in it.
+// The item of unit t, and the unit's place in it.
 template <int HD>
-__device__ __forceinline__ Cursor cursor_at(const PagedAttnParams& p, const Plan& n, const Lists& L, int64_t steps_s, int64_t t) {
+__device__ __forceinline__ Cursor cursor_at(const PagedAttnParams& p, const Plan& n, const Lists& L, int64_t units_s, int64_t t, int& all) {
   Cursor c;
-  c.own = t < steps_s;
+  c.own = t < units_s;
   const int per = c.own ? p.Hkv * n.RT : p.Hkv;
-  const int64_t u = c.own ? t : t - steps_s;
+  const int64_t u = c.own ? t : t - units_s;
   const int* sum = c.own ? L.sum_s : L.sum_p;
   c.list = find_list(sum, c.own ? p.B : L.n_groups, (int)(u / per));
-  const int local = (int)(u - (int64_t)sum[c.list] * per);
+  set_list<HD>(p, n, c);
+  all = c.own ? n.gqa : c.rows;
+  const int local = (int)(u - (int64_t)sum[c.list] * per), i = local / c.units;
+  c.unit = local - i * c.units;
   c.i = 0;
-  set_item<HD>(p, n, c);
-  c.i = local / c.n_steps;
-  c.step = local - c.i * c.n_steps;
-  set_item<HD>(p, n, c);
+  set_item(p, n, c, i, all);
   return c;
 }
 
 // To the next item; there is one.
 template <int HD>
-__device__ __forceinline__ void next_item(const PagedAttnParams& p, const Plan& n, const Lists& L, Cursor& c) {
-  const int per = c.own ? p.Hkv * n.RT : p.Hkv, last = c.own ? p.B : L.n_groups;
-  const int* sum = c.own ? L.sum_s : L.sum_p;
-  c.step = 0;
-  // items of the list: its steps (of all items, per kv head or head tile) over those of one item
-  const int items = (int)((int64_t)(sum[c.list + 1] - sum[c.list]) * per / c.n_steps);
-  if (++c.i == items) {
-    c.i = 0;
+__device__ __forceinline__ void next_item(const PagedAttnParams& p, const Plan& n, const Lists& L, Cursor& c, int& all) {
+  c.unit = 0;
+  int i = c.i + 1;
+  if (i == c.items) {
+    const int* sum = c.own ? L.sum_s : L.sum_p;
+    const int last = c.own ? p.B : L.n_groups;
     do ++c.list;
     while (c.list < last && sum[c.list + 1] == sum[c.list]);
     if (c.list == last) {  // from the sequences to the groups
@@ -166,15 +171,34 @@ __device__ __forceinline__ void next_item(const PagedAttnParams& p, const Plan& 
       c.list = 0;
       while (L.sum_p[c.list + 1] == L.sum_p[c.list]) ++c.list;
     }
+    set_list<HD>(p, n, c);
+    all = c.own ? n.gqa : c.rows;
+    i = c.i = 0;
   }
-  set_item<HD>(p, n, c);
+  set_item(p, n, c, i, all);
 }
 
 // What a warp keeps of its ring: steps taken so far.
 struct Ring {
   uint32_t base;  // shared memory of the stages
   uint32_t full;  // mbarriers of the stages (TMA)
+  uint32_t q;     // query rows of the items that the loads have begun: kStages buffers of q_rows rows
+  int q_rows;
 };
+constexpr int kQPad = 16;  // bytes behind a query row, so that the rows of an ldmatrix phase fall on different banks
+
+// Brings the query rows of cursor c into buffer `at` (cp.async; the caller commits).
+template <int HD>
+__device__ __forceinline__ void load_queries(const PagedAttnParams& p, const Plan& n, const Cursor& c, const Ring& ring, int at) {
+  constexpr int kChunks = Cfg<HD>::kChunks;
+  const uint32_t dst = ring.q + at % Cfg<HD>::kStages * ring.q_rows * (HD * 2 + kQPad);
+  for (int i = threadIdx.x & 31; i < ring.q_rows * kChunks; i += 32) {
+    const int r = i / kChunks, ch = i % kChunks, x = c.h0 + r;
+    const bool live = r < c.rows;
+    const int q = live ? x / n.gqa : 0, h = live ? x - q * n.gqa : 0;
+    copy16(dst + r * (HD * 2 + kQPad) + ch * 16, static_cast<const __nv_bfloat16*>(p.q) + (int64_t)(c.row0 + q) * p.q_row + (c.kvh * n.gqa + h) * p.q_head + ch * 8, live);
+  }
+}
 
 template <int HD, bool kTma>
 __device__ __forceinline__ void load_step(const PagedAttnParams& p, const CUtensorMap* map_k, const CUtensorMap* map_v, int box, const KeyWalk& w, int key0,
@@ -330,8 +354,6 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   __shared__ int warp_tot[kWarps];
   __shared__ uint64_t full[kWarps][C::kStages];
   __shared__ int abort_flag;
-  int* sum_s = reinterpret_cast<int*>(smem + kWarps * C::kRing);
-  int* sum_p = sum_s + p.B + 1;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const AbortState ab{&abort_flag, p.status};
@@ -340,58 +362,65 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (int i = 0; i < kWarps * C::kStages; ++i) mbar_init(smem_u32(&full[0][0] + i), 1);
     fence_barrier_init();
   }
-  const Ring ring{smem_u32(smem + warp * C::kRing), smem_u32(full[warp])};
-  Lists L{sum_s, sum_p, n.form == kPrefixSmall ? p.G : 0};
-  scan_tiles<kThreads>(sum_s, p.B, [&](int b) { return (clamp_len(p.lens[b], p.table_width, p.pool.P, p.status) + C::kKeys - 1) / C::kKeys; }, warp_tot);
-  scan_tiles<kThreads>(sum_p, L.n_groups, [&](int g) {
-    const Group w = load_group(p, g);
-    return (w.len + C::kKeys - 1) / C::kKeys * row_tiles(w, n);
-  }, warp_tot);
-  __syncthreads();
-  const int64_t steps_s = (int64_t)sum_s[p.B] * p.Hkv * n.RT, total = steps_s + (int64_t)sum_p[L.n_groups] * p.Hkv;
-  // every worker has at least kLeast steps (one worker may have less), so the parts of an item have consecutive numbers
+  const int q_bytes = C::kStages * n.rows_q * (HD * 2 + kQPad);  // per warp
+  const Ring ring{smem_u32(smem + warp * C::kRing), smem_u32(full[warp]), smem_u32(smem + kWarps * C::kRing + warp * q_bytes), n.rows_q};
+  int* sum_s = reinterpret_cast<int*>(smem + kWarps * (C::kRing + q_bytes));
+  int* sum_p = sum_s + p.B + 1;
+  const Lists L{sum_s, sum_p, n.form == kPrefixSmall ? p.G : 0};
+  scan_tiles<kThreads>(sum_s, p.B, [&](int b) { return units_of<HD>(clamp_len(p.lens[b], p.table_width, p.pool.P, p.status)); }, warp_tot);
+  if (L.n_groups > 0) {
+    scan_tiles<kThreads>(sum_p, L.n_groups, [&](int g) {
+      const Group w = load_group(p, g);
+      return units_of<HD>(w.len) * row_tiles(w, n);
+    }, warp_tot);
+  }
+  const int64_t units_s = (int64_t)sum_s[p.B] * p.Hkv * n.RT, total = units_s + (L.n_groups > 0 ? (int64_t)sum_p[L.n_groups] * p.Hkv : 0);
+  // every worker has at least kLeast units (one worker may have less), so the parts of an item have consecutive numbers
   const int64_t workers = min((int64_t)gridDim.x * kWarps, (total + kLeast - 1) / kLeast);
   const int64_t worker = (int64_t)warp * gridDim.x + blockIdx.x;  // few workers: on SMs of their own
   int64_t t = worker < workers ? total * worker / workers : 0;
   const int64_t t_end = worker < workers ? total * (worker + 1) / workers : 0;
   if (t < t_end) {
-    Cursor ahead = cursor_at<HD>(p, n, L, steps_s, t);  // of the loads
-    Cursor c = ahead;
+    int all, all_ahead;
+    Cursor c = cursor_at<HD>(p, n, L, units_s, t, all);
+    // The loads run ahead: their cursor, the unit that it stands at, items and steps that it has begun.
+    Cursor ahead = c;
+    all_ahead = all;
     int64_t t_ahead = t;
-    int it = 0;  // steps so far: the ring's position
-    bool ok = true;
-    const auto load_next = [&](int at) {
-      if (t_ahead < t_end) {
-        if (ahead.step == ahead.n_steps) next_item<HD>(p, n, L, ahead);
-        load_step<HD, kTma>(p, &map_k, &map_v, box, ahead.w, ahead.step * C::kKeys, ring, at);
-        ++ahead.step;
-        ++t_ahead;
-      } else if (!kTma) {
-        copy_commit();
-      }
-    };
-#pragma unroll
-    for (int s = 0; s < C::kStages - 1; ++s) load_next(s);
-    while (t < t_end && ok) {
-      const int steps = (int)min(t_end - t, (int64_t)(c.n_steps - c.step));
-      if (c.step == 0 && lane == 0) ws.meta[c.item] = item_parts(c.own ? c.item : c.item - n.items_s, t, c.n_steps, workers, total);
-      // ---- queries: the A operand, straight from memory
-      uint32_t qf[HD / 16][4];
-      const __nv_bfloat16* qrow[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = (lane >> 2) + 8 * h, x = c.h0 + r;
-        qrow[h] = r < c.rows ? static_cast<const __nv_bfloat16*>(p.q) + (c.row0 + x / n.gqa) * p.q_row + (c.kvh * n.gqa + x % n.gqa) * p.q_head : nullptr;
-      }
-#pragma unroll
-      for (int kk = 0; kk < HD / 16; ++kk)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const __nv_bfloat16* src = qrow[e & 1];
-          qf[kk][e] = src != nullptr ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + (lane & 3) * 2 + (e >> 1) * 8) : 0u;
+    int items_ahead = 0, it_ahead = 0;
+    load_queries<HD>(p, n, ahead, ring, 0);
+    if (kTma) copy_commit();
+    const auto load_next = [&]() {
+      // over the units that are no steps
+      while (t_ahead < t_end && (ahead.unit < kItemCost || ahead.unit == ahead.units)) {
+        if (ahead.unit == ahead.units) {
+          next_item<HD>(p, n, L, ahead, all_ahead);
+          load_queries<HD>(p, n, ahead, ring, ++items_ahead);
+          if (kTma) copy_commit();
         }
+        const int skip = (int)min(t_end - t_ahead, (int64_t)max(0, kItemCost - ahead.unit));
+        ahead.unit += skip;
+        t_ahead += skip;
+      }
+      if (t_ahead < t_end) {
+        load_step<HD, kTma>(p, &map_k, &map_v, box, ahead.w, (ahead.unit - kItemCost) * C::kKeys, ring, it_ahead++);
+        ++ahead.unit;
+        ++t_ahead;
+      }
+      if (!kTma) copy_commit();
+    };
+    bool ok = true;
+    int it = 0, items = 0;
+#pragma unroll
+    for (int s = 0; s < C::kStages - 1; ++s) load_next();
+    while (t < t_end && ok) {
+      const int units = (int)min(t_end - t, (int64_t)(c.units - c.unit));
+      const int step0 = max(0, c.unit - kItemCost), steps = max(0, c.unit + units - kItemCost) - step0;
+      if (c.unit == 0 && lane == 0) ws.meta[c.item] = item_parts(c.own ? c.item : c.item - n.items_s, t, c.units, workers, total);
       float o[HD / 8][4] = {};
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      uint32_t qf[HD / 16][4];
+      const bool half = c.rows <= 8;
       for (int s = 0; s < steps; ++s, ++it) {
         const int st = it % C::kStages;
         if constexpr (kTma) {
@@ -401,14 +430,29 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           copy_wait<C::kStages - 2>();
           __syncwarp();
         }
-        load_next(it + C::kStages - 1);
-        const int left = c.w.len - (c.step + s) * C::kKeys;
-        if (c.rows <= 8) attend<HD, kTma, true>(p, left, qf, ring, st, o, m, l);
+        if (s == 0) {  // queries: the A operand (rows 8 to 15 only where there are any)
+          if (kTma) {
+            copy_wait<0>();
+            __syncwarp();
+          }
+          const uint32_t src = ring.q + items % C::kStages * ring.q_rows * (HD * 2 + kQPad);
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            // matrices: rows 0-7 and 8-15 of the first eight columns, then of the second
+            const int r = (lane & 7) + (half ? 0 : ((lane >> 3) & 1) * 8);
+            ldsm4(qf[kk], src + r * (HD * 2 + kQPad) + (kk * 2 + (lane >> 4)) * 16);
+            if (half) qf[kk][1] = qf[kk][3] = 0u;
+          }
+          __syncwarp();
+        }
+        load_next();
+        const int left = c.w.len - (step0 + s) * C::kKeys;
+        if (half) attend<HD, kTma, true>(p, left, qf, ring, st, o, m, l);
         else attend<HD, kTma, false>(p, left, qf, ring, st, o, m, l);
         __syncwarp();
       }
       // ---- the row's result, or the part of it
-      const bool whole = c.own && p.G == 0 && steps == c.n_steps;
+      const bool whole = c.own && p.G == 0 && units == c.units;
       const int64_t part = ((c.own ? c.item : c.item - n.items_s) + worker) * (c.own ? n.rows_s : kRows);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -424,15 +468,21 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<uint32_t*>(dst + d * 8) = pack_bf16(o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
           if (col == 0) p.lse[out] = row_lse(m[h], l[h]);
         } else {
-          float* dst = (c.own ? ws.acc_s : ws.acc_p) + (part + r) * HD + col;
+          if (steps > 0) {
+            float* dst = (c.own ? ws.acc_s : ws.acc_p) + (part + r) * HD + col;
 #pragma unroll
-          for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(dst + d * 8) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
+            for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(dst + d * 8) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
+          }
           if (col == 0) (c.own ? ws.ml_s : ws.ml_p)[part + r] = make_float2(m[h], l[h]);
         }
       }
-      t += steps;
-      if (t < t_end) next_item<HD>(p, n, L, c);
+      t += units;
+      if (t < t_end) {
+        next_item<HD>(p, n, L, c, all);
+        ++items;
+      }
     }
+    copy_wait<0>();
   }
   // The prefix kernel before this one let it start early.  It must have ended when this one ends, for the join waits for this
   // one alone.
@@ -546,7 +596,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 8) paged_attn_join_kernel(con
   if (lane == 0) p.lse[at] = row_lse(m, l);
 }
 
-template <int HD> int smem_bytes(const PagedAttnParams& p) { return kWarps * Cfg<HD>::kRing + (p.B + p.G + 2) * (int)sizeof(int); }
+template <int HD> int smem_bytes(const PagedAttnParams& p, const Plan& n) {
+  return kWarps * (Cfg<HD>::kRing + Cfg<HD>::kStages * n.rows_q * (HD * 2 + kQPad)) + (p.B + p.G + 2) * (int)sizeof(int);
+}
 
 // Rows of a kv head per group on average from which the tcgen05 forms are used for the prefixes.
 constexpr int kDenseRows = 32;
@@ -559,16 +611,17 @@ Plan make_plan(const PagedAttnParams& p) {
   n.items_s = p.B * p.Hkv * n.RT;
   const int64_t rows = p.G > 0 ? (int64_t)p.B * n.gqa / p.G : 0;
   n.form = rows >= kDenseRows && paged_prefix_usable(p) ? (p.hd == 64 && rows > 128 ? kPrefixRows : kPrefixKeys) : kPrefixSmall;
+  n.rows_q = n.gqa <= 8 && (p.G == 0 || n.form != kPrefixSmall) ? 8 : kRows;
   n.rows_p = n.form == kPrefixSmall ? kRows : n.form == kPrefixRows ? 256 : 128;
   n.parts_p = n.form == kPrefixKeys ? 2 : 1;
   n.part_rows_p = n.rows_p;
   n.items_p = p.G > 0 ? p.Hkv * (int)((int64_t)p.B * n.gqa / n.rows_p + p.G + 1) : 0;
   // one resident wave, but no more CTAs than there can be tiles
   const int64_t P = p.pool.P, keys = p.hd == 128 ? Cfg<128>::kKeys : Cfg<64>::kKeys;
-  int64_t steps = (int64_t)n.items_s * ((p.table_width * P + keys - 1) / keys), tiles_p = 0;
-  if (n.form == kPrefixSmall) steps += (int64_t)n.items_p * ((p.ptable_width * P + keys - 1) / keys);
+  int64_t steps = (int64_t)n.items_s * ((p.table_width * P + keys - 1) / keys + kItemCost), tiles_p = 0;
+  if (n.form == kPrefixSmall) steps += (int64_t)n.items_p * ((p.ptable_width * P + keys - 1) / keys + kItemCost);
   else tiles_p = (int64_t)n.items_p * ((p.ptable_width * P + 63) / 64);
-  const int smem = (p.hd == 128 ? smem_bytes<128>(p) : p.hd == 64 ? smem_bytes<64>(p) : smem_bytes<32>(p)) + 2048;
+  const int smem = (p.hd == 128 ? smem_bytes<128>(p, n) : p.hd == 64 ? smem_bytes<64>(p, n) : smem_bytes<32>(p, n)) + 2048;
   const int per_sm = std::max(1, std::min(228 * 1024 / smem, p.hd == 128 ? 4 : 8));
   const int64_t ctas = (steps + kLeast - 1) / kLeast;  // worker w sits in CTA w % ctas
   n.ctas = (int)(ctas < 148 * per_sm ? (ctas < 1 ? 1 : ctas) : 148 * per_sm);
@@ -590,7 +643,7 @@ int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
   if (!configured[dev]) {
-    if (cudaFuncSetAttribute(paged_attn_kernel<HD, kTma>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * Cfg<HD>::kRing + (kMaxLists + 2) * 4) != cudaSuccess) return -2;
+    if (cudaFuncSetAttribute(paged_attn_kernel<HD, kTma>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * (Cfg<HD>::kRing + Cfg<HD>::kStages * kRows * (HD * 2 + kQPad)) + (kMaxLists + 2) * 4) != cudaSuccess) return -2;
     configured[dev] = true;
   }
   // The kernels after the first may be brought in while the one before still runs: the walk over own pages needs nothing of the
@@ -609,7 +662,7 @@ int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t
     cfg.numAttrs = 1;
   }
   cfg.gridDim = dim3(n.ctas);
-  cfg.dynamicSmemBytes = smem_bytes<HD>(p);
+  cfg.dynamicSmemBytes = smem_bytes<HD>(p, n);
   if (cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD, kTma>, mk, mv, p, n, ws, box) != cudaSuccess) return -3;
   cfg.numAttrs = 1;
   cfg.dynamicSmemBytes = 0;

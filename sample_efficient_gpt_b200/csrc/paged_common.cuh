@@ -15,6 +15,7 @@ enum PrefixForm { kPrefixSmall = 0, kPrefixRows = 1, kPrefixKeys = 2 };
 struct Plan {            // sizes that host and device derive alike
   int gqa, RT;           // query heads per kv head; 16-row tiles of a sequence's item row
   int rows_s, items_s;   // rows of a part of an own-pages item; number of such items
+  int rows_q;            // query rows that a warp keeps of an item: 8, or 16 where some item has more
   int form;              // PrefixForm
   int rows_p, items_p;   // rows of a prefix item; upper bound on their number
   int parts_p, part_rows_p;  // parts that a CTA leaves of a prefix item, rows of each
@@ -63,29 +64,35 @@ __device__ __forceinline__ int first_item(const Plan& n, const PagedAttnParams& 
   return n.items_s + p.Hkv * (r0 * n.gqa / n.rows_p + g);
 }
 
-// sum[i + 1] = tiles of the first i + 1 lists; all kThreads threads take part, warp_tot has a word per warp
+// sum[i + 1] = tiles of the first i + 1 lists; all kThreads threads take part, warp_tot has a word per warp.  A thread adds up
+// neighbouring lists, whose loads do not wait for one another.
 template <int kThreads, typename F>
 __device__ void scan_tiles(int* sum, int n, F tiles, int* warp_tot) {
-  constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int carry = 0;
-  if (threadIdx.x == 0) sum[0] = 0;
-  for (int base = 0; base < n; base += kThreads) {
-    const int i = base + threadIdx.x;
-    int v = i < n ? tiles(i) : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
-    }
-    if (lane == 31) warp_tot[warp] = v;
-    __syncthreads();
-    int add = carry;
-    for (int w = 0; w < warp; ++w) add += warp_tot[w];
-    if (i < n) sum[i + 1] = v + add;
-    for (int w = 0; w < kWarps; ++w) carry += warp_tot[w];
-    __syncthreads();
+  const int per = (n + kThreads - 1) / kThreads, first = min((int)threadIdx.x * per, n), last = min(first + per, n);
+  int mine = 0;
+#pragma unroll 4
+  for (int i = first; i < last; ++i) {
+    const int v = tiles(i);
+    sum[i + 1] = v;
+    mine += v;
   }
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  if (lane == 31) warp_tot[warp] = upto;
+  if (threadIdx.x == 0) sum[0] = 0;
+  __syncthreads();
+  int at = upto - mine;
+  for (int w = 0; w < warp; ++w) at += warp_tot[w];
+  for (int i = first; i < last; ++i) {
+    at += sum[i + 1];
+    sum[i + 1] = at;
+  }
+  __syncthreads();
 }
 // last i with sum[i] <= t (t < sum[n]); empty lists are passed over
 __device__ __forceinline__ int find_list(const int* sum, int n, int t) {
