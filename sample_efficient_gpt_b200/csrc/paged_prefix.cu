@@ -18,8 +18,9 @@
 // the tensor core at head_dim 64.  A quarter of the exponentials therefore runs as a polynomial on the FMA pipe, and the
 // softmax keeps the maximum off its critical path: the exponentials use the reference of the tiles before, and only when a
 // new score exceeds it by more than 2^8 (rare after the first tile) is the row's sum rescaled and the tile repeated from tensor
-// memory.  Scores pass through the registers 32 columns at a time, the next load in flight, which leaves room on the SM for a
-// CTA of the kernel over own pages.
+// memory.  Scores pass through the registers 32 columns at a time, the next load in flight; P goes back to tensor memory, from
+// where the second product reads it (through shared memory, each warp's fence between its stores and the tensor core's reads
+// cost 290 cycles a tile).  Registers and shared memory leave room on the SM for CTAs of the kernel over own pages.
 #include <cuda.h>
 
 #include <type_traits>
@@ -34,20 +35,29 @@ using namespace sm100;
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kBlock = 128 * 128;  // bytes of 128 rows of 64 bf16: the unit of the query and P tiles
+constexpr int kBlock = 128 * 128;  // bytes of 128 rows of 64 bf16: the unit of the query tiles
 
 template <int HD, bool kSplit> struct Lay {
   static constexpr int kKeys = kSplit ? 64 : 128;              // keys per tile
-  static constexpr int kDepth = !kSplit || HD == 128 ? 2 : 3;  // places of a ring
+  static constexpr int kDepth = 3;                             // places of a ring
   static constexpr int kRings = kSplit ? 2 : 1;                // rings: one for both halves, or one each
   static constexpr int kSlots = kDepth * kRings;
   static constexpr int kTileBlock = kKeys * 128;               // 64 dims of a K or V tile
   static constexpr int kTile = HD / 64 * kTileBlock;
   static constexpr int kQTile = HD / 64 * kBlock;
-  static constexpr int kPTile = kKeys / 64 * kBlock;           // P of one half
-  static constexpr int kK = (kSplit ? 1 : 2) * kQTile, kV = kK + kSlots * kTile, kP = kV + kSlots * kTile, kBars = kP + 2 * kPTile, kSum = kBars + 512;
+  static constexpr int kPCols = 2 * kKeys + 2 * HD;            // tensor memory: first column of P (bf16, two keys a column)
+  static_assert(kPCols + kKeys <= 512, "tensor memory");
+  static constexpr int kK = (kSplit ? 1 : 2) * kQTile, kV = kK + kSlots * kTile, kBars = kV + kSlots * kTile, kSum = kBars + 512;
 };
 
+// 32 lanes x 16 consecutive 32-bit columns
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 constexpr int kPolyPairs = 1;  // of four pairs of exponentials, one takes the polynomial
 
 // 2^x for a pair on the FMA and integer pipes: x = n + f with n the nearest integer (rounding by a large constant), |f| <= 1/2, a
@@ -150,7 +160,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // columns [0, 256): scores of half 0 / 1; from 256 on: outputs of half 0 / 1
+  const uint32_t tmem = *tmem_slot;  // scores of half 0 / 1, outputs of half 0 / 1, P of half 0 / 1
   const int64_t total = (int64_t)sum[p.G] * p.Hkv;
   const int64_t ctas = min((int64_t)gridDim.x, total);
   const int64_t t_begin = blockIdx.x < ctas ? total * blockIdx.x / ctas : 0, t_end = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
@@ -159,21 +169,27 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     // ------------------------------------------------------------------------------------------------ loads
     int used[2] = {0, 0}, tails = 0;  // tiles so far of each ring
     bool ok = true;
+    const bool mine = lane * box < kTileKeys;
     for (int64_t t = t_begin; t < t_end && ok;) {
       const Seg s = find_seg<kTileKeys>(p, n, sum, t, t_end);
+      const auto lookup = [&](int j) {  // the page of this lane's box of tile j, one tile ahead and unchecked
+        const int key = (s.tile0 + j) * kTileKeys + lane * box;
+        return mine && j < s.steps && key < s.len ? s.pages[p.pool.shift >= 0 ? key >> p.pool.shift : key / p.pool.P] : -1;
+      };
+      int found = lookup(0);
       for (int j = 0; j < s.steps && ok; ++j) {
         const int ring = kSplit ? j & 1 : 0, c = ring ? used[1]++ : used[0]++, st = ring * L::kDepth + c % L::kDepth, ph = (c / L::kDepth) & 1;
         const int first = (s.tile0 + j) * kTileKeys, key = first + lane * box;
         int page = p.pool.n_pages, slot = 0;  // a box outside the pool reads as zeros
-        if (lane * box < kTileKeys && key < s.len) {
-          const int i = p.pool.shift >= 0 ? key >> p.pool.shift : key / p.pool.P, found = s.pages[i];
+        if (mine && key < s.len) {
           if ((unsigned)found < (unsigned)p.pool.n_pages) {
             page = found;
-            slot = key - i * p.pool.P;
+            slot = p.pool.shift >= 0 ? key & (p.pool.P - 1) : key % p.pool.P;
           } else {
             atomicCAS(p.status, 0, kStatusAttnPage);
           }
         }
+        found = lookup(j + 1);
         const bool cut = s.len < first + kTileKeys && s.len % box != 0;  // the last box brings slots behind the length
         // K before V: the issuer wants the next scores before it issues the products that free the place of the V tile.
 #pragma unroll
@@ -185,7 +201,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(bar, L::kTile);
           __syncwarp();
-          if (lane * box < kTileKeys) {
+          if (mine) {
 #pragma unroll
             for (int b = 0; b < HD / 64; ++b)
               tma_load_4d(smem_u32(smem) + dst + b * L::kTileBlock + lane * box * 128, kv == 0 ? &map_k : &map_v, bar, b * 64, s.kvh, slot, page);
@@ -213,8 +229,8 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       constexpr uint32_t idesc_s = make_idesc_bf16(128, kTileKeys, false, false);  // Q (K-major) x K (K-major)
       constexpr uint32_t idesc_o = make_idesc_bf16(128, HD, false, true);          // P (K-major) x V (MN-major)
       const uint64_t d_q = make_smem_desc(smem_u32(smem) + (kSplit ? 0 : x * L::kQTile), 16, 1024);
-      const uint64_t d_p = make_smem_desc(smem_u32(smem + L::kP) + x * L::kPTile, 16, 1024);
-      const uint32_t t_s = tmem + x * 128, t_o = tmem + 256 + x * HD;
+      const uint32_t t_p = tmem + L::kPCols + x * (kTileKeys / 2);
+      const uint32_t t_s = tmem + x * kTileKeys, t_o = tmem + 2 * kTileKeys + x * HD;
       int cx = 0, seg = 0;  // tiles of this half, segments
       bool ok = true;
       for (int64_t t = t_begin; t < t_end && ok; ++seg) {
@@ -246,7 +262,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kTileKeys / 16; ++k)
-            umma_bf16(t_o, d_p + (uint64_t)(((k >> 2) * kBlock + (k & 3) * 32) >> 4), d_v + (uint64_t)(k * 128), idesc_o, i > 0 || k > 0);
+            umma_bf16_ts(t_o, t_p + k * 8, d_v + (uint64_t)(k * 128), idesc_o, i > 0 || k > 0);
           umma_commit(smem_u32(&pv_full[x]));
           umma_commit(smem_u32(&v_empty[st]));
         }
@@ -259,8 +275,8 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     // ------------------------------------------------------------------------------------------------ softmax of half x
     const int x = (warp >> 2) - 1, sub = warp & 3, r = sub * 32 + lane;  // r: row of the half's tile == TMEM lane
     const uint32_t lane_addr = (uint32_t)(sub * 32) << 16;
-    const uint32_t t_s = tmem + x * 128 + lane_addr, t_o = tmem + 256 + x * HD + lane_addr;
-    uint8_t* sP = smem + L::kP + x * L::kPTile + r * 128;
+    const uint32_t t_s = tmem + x * kTileKeys + lane_addr, t_o = tmem + 2 * kTileKeys + x * HD + lane_addr;
+    const uint32_t t_p = tmem + L::kPCols + x * (kTileKeys / 2) + lane_addr;
     const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
     int cx = 0, seg = 0;
     bool ok = true;
@@ -378,6 +394,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&s_empty[x]));
               }
+              uint32_t pk[16];
 #pragma unroll
               for (int q4 = 0; q4 < 4; ++q4) {
                 float e[8];
@@ -393,9 +410,11 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                   }
                   l2[k & 1] = add2(l2[k & 1], pack2(e[2 * k], e[2 * k + 1]));
                 }
-                const int c16 = c * 4 + q4;  // bf16 operand tile: 16-byte chunk c16 of row r at c16 ^ (r & 7) inside its 64-column block
-                *reinterpret_cast<bf16x8*>(sP + (c16 >> 3) * kBlock + (((c16 & 7) ^ (r & 7)) << 4)) = pack8(e);
+                const bf16x8 b8 = pack8(e);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) pk[q4 * 4 + k] = *reinterpret_cast<const uint32_t*>(&b8.v[k]);
               }
+              tmem_st_32x16(t_p + c * 16, pk);
             }
             if (redo) continue;
             float a0, a1, a2, a3;
@@ -408,8 +427,8 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         };
         ok = left < kTileKeys ? one_tile(std::true_type{}) : one_tile(std::false_type{});
         if (!ok) break;
+        tmem_st_wait();
         tc_fence_before();
-        fence_proxy_async();  // the P tile is visible to the tensor core
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&p_full[x]));
       }
