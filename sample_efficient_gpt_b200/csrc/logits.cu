@@ -5,10 +5,12 @@
 //
 // Bound by bytes: one read and one write of the logits.  A CTA takes a range of neighbouring entries of a row, 16 bytes a
 // thread and access, with their loads in flight while it counts the part of the row's history that falls into its range in
-// shared memory (integer atomics: the order does not matter).  Every CTA of a row reads the whole history, out of L2; eight
+// shared memory (integer atomics: the order does not matter).  Every CTA of a row reads the whole history, out of L2; four
 // loads a thread are in flight, otherwise their latency bounds the kernel.  Bit 31 of a count says that the prompt has the
 // token, bit 30 that a bias waits for it, bit 29 that more than one does: entries with a bias are left to the threads that hold
 // the biases, so that no second array is needed and the call may work in place.
+#include <type_traits>
+
 #include "common.cuh"
 #include "paged.h"
 
@@ -20,14 +22,14 @@ constexpr uint32_t kPrompt = 1u << 31, kBiased = 1u << 30, kTwice = 1u << 29, kC
 constexpr int kThreads = 512;
 constexpr int kEntries = 16;                  // entries per thread
 constexpr int kRange = kThreads * kEntries;   // entries per CTA
-constexpr int kBatch = 8;                     // history loads of a thread in flight
+constexpr int kBatch = 4;                     // history loads of a thread in flight
 
 struct RowScale {
-  float rep, pres, freq;
+  float rep, inv, pres, freq;  // inv = 1 / rep: x * inv is within one and a half roundings of x / rep, at a twentieth of its instructions
 };
 
 __device__ __forceinline__ float penalise(float x, uint32_t seen, const RowScale& s) {
-  if ((seen & (kPrompt | kCount)) != 0) x = x > 0.f ? x / s.rep : x * s.rep;
+  if ((seen & (kPrompt | kCount)) != 0) x *= x > 0.f ? s.inv : s.rep;
   const uint32_t n = seen & kCount;
   if (n != 0) x = x - s.freq * (float)n - s.pres;
   return x;
@@ -59,7 +61,7 @@ __device__ __forceinline__ void count_history(const Tok* tokens, int len, int pr
     for (int j = 0; j < kBatch; ++j) tok[j] = i0 + j * kThreads < len ? tokens[i0 + j * kThreads] : (Tok)-1;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      if (tok[j] < (Tok)lo || tok[j] - (Tok)lo >= (Tok)n) continue;
+      if ((std::make_unsigned_t<Tok>)(tok[j] - (Tok)lo) >= (std::make_unsigned_t<Tok>)n) continue;
       uint32_t* at = &seen[(int)tok[j] - base];
       if (i0 + j * kThreads < prompt) atomicOr(at, kPrompt);
       else atomicAdd(at, 1u);
@@ -68,7 +70,7 @@ __device__ __forceinline__ void count_history(const Tok* tokens, int len, int pr
 }
 
 template <typename T, int VEC, bool kCounts>
-__global__ void __launch_bounds__(kThreads) process_logits_kernel(const LogitsParams p) {
+__global__ void __launch_bounds__(kThreads, 3) process_logits_kernel(const LogitsParams p) {
   constexpr int kVecs = kEntries / VEC;
   extern __shared__ uint4 seen4[];  // [kRange + VEC] counts
   uint32_t* seen = reinterpret_cast<uint32_t*>(seen4);
@@ -81,6 +83,27 @@ __global__ void __launch_bounds__(kThreads) process_logits_kernel(const LogitsPa
   const int first = head + blockIdx.x * kRange, base = first - VEC;
   const int lo = blockIdx.x == 0 ? 0 : first, hi = min(p.V, first + kRange);
   if (lo >= hi) return;
+  // What does not depend on anything is asked for first: the row's scalars, its logits, the thread's bias.
+  int mask_row = -1, len = 0, prompt = 0;
+  if (p.mask != nullptr) mask_row = p.mask_rows[b];
+  RowScale s{1.f, 1.f, 0.f, 0.f};
+  const int* ids = p.bias_ids + (int64_t)b * p.K;
+  const float* bias = p.bias + (int64_t)b * p.K;
+  int my_id = -1;
+  float my_bias = 0.f, my_x = 0.f;
+  if (kCounts) {
+    if (p.tokens != nullptr) {
+      len = p.token_lens[b];
+      if (p.prompt_lens != nullptr) prompt = p.prompt_lens[b];
+    }
+    if (p.repetition != nullptr) s.rep = p.repetition[b];
+    if (p.presence != nullptr) s.pres = p.presence[b];
+    if (p.frequency != nullptr) s.freq = p.frequency[b];
+    if (tid < p.K) {
+      my_id = ids[tid];
+      my_bias = bias[tid];
+    }
+  }
   Pack<T, VEC> in[kVecs];
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
@@ -88,32 +111,21 @@ __global__ void __launch_bounds__(kThreads) process_logits_kernel(const LogitsPa
     if (v + VEC <= hi) in[i] = *reinterpret_cast<const Pack<T, VEC>*>(x + v);
   }
   const int* words = nullptr;
-  if (p.mask != nullptr) {
-    const int r = p.mask_rows[b];
-    if (r >= p.n_masks && tid == 0) atomicCAS(p.status, 0, kStatusLogitsMask);
-    if (r >= 0 && r < p.n_masks) words = p.mask + r * p.mask_row;
-  }
-  RowScale s{1.f, 0.f, 0.f};
-  const int* ids = p.bias_ids + (int64_t)b * p.K;
+  if (mask_row >= p.n_masks && tid == 0 && p.mask != nullptr) atomicCAS(p.status, 0, kStatusLogitsMask);
+  if (mask_row >= 0 && mask_row < p.n_masks) words = p.mask + mask_row * p.mask_row;
   if (kCounts) {
     for (int i = tid; i < (kRange + VEC + 3) / 4; i += kThreads) seen4[i] = make_uint4(0, 0, 0, 0);
-    int len = 0, prompt = 0;
-    if (p.tokens != nullptr) {
-      len = p.token_lens[b];
-      if (p.prompt_lens != nullptr) prompt = p.prompt_lens[b];
-      if (len < 0 || len > p.tokens_width) {
-        if (tid == 0) atomicCAS(p.status, 0, kStatusLogitsLength);
-        len = len < 0 ? 0 : p.tokens_width;
-      }
+    if (len < 0 || len > p.tokens_width) {
+      if (tid == 0) atomicCAS(p.status, 0, kStatusLogitsLength);
+      len = len < 0 ? 0 : p.tokens_width;
     }
-    if (p.repetition != nullptr) s.rep = p.repetition[b];
-    if (p.presence != nullptr) s.pres = p.presence[b];
-    if (p.frequency != nullptr) s.freq = p.frequency[b];
+    s.inv = 1.f / s.rep;
+    if (my_id >= lo && my_id < hi) my_x = to_f<T>(x[my_id]);
     __syncthreads();
     if (p.tokens64) count_history(static_cast<const int64_t*>(p.tokens) + b * p.tokens_row, len, prompt, lo, hi - lo, base, seen);
     else count_history(static_cast<const int*>(p.tokens) + b * p.tokens_row, len, prompt, lo, hi - lo, base, seen);
     for (int i = tid; i < p.K; i += kThreads) {
-      const int v = ids[i];
+      const int v = i == tid ? my_id : ids[i];
       if (v >= lo && v < hi && (atomicOr(&seen[v - base], kBiased) & kBiased) != 0) atomicOr(&seen[v - base], kTwice);
     }
     __syncthreads();
@@ -173,12 +185,11 @@ __global__ void __launch_bounds__(kThreads) process_logits_kernel(const LogitsPa
     }
   }
   if (kCounts && p.K > 0) {
-    const float* bias = p.bias + (int64_t)b * p.K;
     for (int i = tid; i < p.K; i += kThreads) {
-      const int v = ids[i];
+      const int v = i == tid ? my_id : ids[i];
       if (v < lo || v >= hi) continue;
       const uint32_t c = seen[v - base];
-      float r = penalise(to_f<T>(x[v]), c, s) + bias[i];
+      float r = penalise(i == tid ? my_x : to_f<T>(x[v]), c, s) + (i == tid ? my_bias : bias[i]);
       if (c & kTwice) {  // the first entry's thread adds them all
         bool mine = true;
 #pragma unroll 8

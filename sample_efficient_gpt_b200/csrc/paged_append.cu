@@ -21,7 +21,7 @@ using namespace sm100;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr float kQkEps = 1e-6f;
 constexpr float kMixEps = 1e-8f;
 
@@ -72,12 +72,9 @@ __device__ __forceinline__ TokenPlace find_place(const PagedAppendParams& p, int
 
 // An item's 16 elements -> the finished query, key or value elements.  u1, u2: the first block's values (or nullptr).
 template <int HD>
-__device__ __forceinline__ void finish(const PagedAppendParams& p, int slot, const float* cos, const float* sin, const bf16x8* u1, const bf16x8* u2, float c,
+__device__ __forceinline__ void finish(const PagedAppendParams& p, int slot, const float* cs, const float* sn, const bf16x8* u1, const bf16x8* u2, float c,
                                        float a1, float a2, float qg, float* x1, float* x2) {
   if (slot < p.H + p.Hkv) {
-    float cs[8], sn[8];
-    load8<float>(cos, cs);
-    load8<float>(sin, sn);
     float ss = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -169,25 +166,29 @@ __global__ void __launch_bounds__(kThreads) paged_append_few_kernel(const PagedA
       unpack8(x[0], x1);
       unpack8(x[1], x2);
       const int64_t rot = (int64_t)w.pos * HALF + sub * 8;
-      finish<HD>(p, slot, p.cos + rot, p.sin + rot, p.v1 != nullptr ? &u[0] : nullptr, &u[1], c, a1, a2, qg, x1, x2);
+      float cs[8], sn[8];
+      load8<float>(p.cos + rot, cs);
+      load8<float>(p.sin + rot, sn);
+      finish<HD>(p, slot, cs, sn, p.v1 != nullptr ? &u[0] : nullptr, &u[1], c, a1, a2, qg, x1, x2);
     }
     store_item<HD>(p, t, w, slot, sub, x1, x2);
   }
 }
 
 // ---------------------------------------------------------------------------------------------- a ring of token groups
-constexpr int kRing = 3;
-constexpr int kMaxTokens = 16;      // tokens of a group
+constexpr int kRing = 4;              // stages at most
+constexpr int kMaxTokens = 16;        // tokens of a group at most
 constexpr int kSmemCta = 110 * 1024;  // two CTAs share an SM
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-// A stage: for each token its projection row, its v1 row, its cos and sin rows (token_bytes in all).
+// A stage: for each token its projection row, its v1 row, its cos and sin rows (token_bytes in all).  tokens: 1, 2, 4, 8 or 16;
+// eight warps share them, each walks over the heads of one token (or of a part of it) with the rotation in registers.
 template <int HD>
-__global__ void __launch_bounds__(kThreads + 32) paged_append_ring_kernel(const PagedAppendParams p, int tokens, int token_bytes) {
-  constexpr int HALF = HD / 2, LPH = HD / 16;
+__global__ void __launch_bounds__(kThreads + 32) paged_append_ring_kernel(const PagedAppendParams p, int tokens, int ring, int token_bytes) {
+  constexpr int HALF = HD / 2, LPH = HD / 16, kHeads = 32 / LPH;  // heads that a warp covers at once
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ TokenPlace place[kRing][kMaxTokens];
   __shared__ uint64_t full[kRing], empty[kRing];
@@ -198,22 +199,22 @@ __global__ void __launch_bounds__(kThreads + 32) paged_append_ring_kernel(const 
   const AbortState ab{&abort_flag, p.status};
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int i = 0; i < kRing; ++i) {
+    for (int i = 0; i < ring; ++i) {
       mbar_init(smem_u32(&full[i]), 1);
-      mbar_init(smem_u32(&empty[i]), kThreads / 32);
+      mbar_init(smem_u32(&empty[i]), kWarps);
     }
     fence_barrier_init();
   }
   __syncthreads();
-  if (warp == kThreads / 32) {
+  if (warp == kWarps) {
     // a lane per token: finds its place and fetches its rows
-    int i = 0;
-    for (int g = blockIdx.x; g < n_groups; g += gridDim.x, ++i) {
-      const int st = i % kRing, t = g * tokens + lane;
+    int st = 0, ph = 0;
+    for (int g = blockIdx.x; g < n_groups; g += gridDim.x) {
+      const int t = g * tokens + lane;
       const bool live = lane < tokens && t < p.T;
       TokenPlace w{-1, 0, 0};
       if (live) w = find_place(p, t);
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[st]), ((i / kRing) & 1) ^ 1, ab, 81))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[st]), ph ^ 1, ab, 81))) break;
       if (live) place[st][lane] = w;
       const int n = __popc(__ballot_sync(0xffffffffu, live && w.page >= 0));
       __syncwarp();  // the places of all lanes are written before lane 0 arrives
@@ -227,29 +228,40 @@ __global__ void __launch_bounds__(kThreads + 32) paged_append_ring_kernel(const 
         bulk_load(dst + row_bytes + v1_bytes, p.cos + (int64_t)w.pos * HALF, HD * 2, bar);
         bulk_load(dst + row_bytes + v1_bytes + HD * 2, p.sin + (int64_t)w.pos * HALF, HD * 2, bar);
       }
+      if (++st == ring) st = 0, ph ^= 1;
     }
   } else {
     const float a1 = *p.alpha1, a2 = *p.alpha2, qg = *p.qgain, c = *p.vscale * rsqrtf(a1 * a1 + a2 * a2 + kMixEps);
-    int i = 0;
-    for (int g = blockIdx.x; g < n_groups; g += gridDim.x, ++i) {
-      const int st = i % kRing, t0 = g * tokens, n_items = min(tokens, p.T - t0) * nslots * LPH;
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full[st]), (i / kRing) & 1, ab, 82))) break;
-      for (int item = threadIdx.x; item < n_items; item += kThreads) {  // the LPH lanes of a head stay together
-        const int sub = item % LPH, rest = item / LPH, tok = rest / nslots, slot = rest - tok * nslots;
+    const int sub = lane % LPH, head = lane / LPH;
+    const int share = tokens < kWarps ? kWarps / tokens : 1;  // warps per token
+    int st = 0, ph = 0;
+    for (int g = blockIdx.x; g < n_groups; g += gridDim.x) {
+      const int t0 = g * tokens;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full[st]), ph, ab, 82))) break;
+      for (int tok = warp / share; tok < tokens && t0 + tok < p.T; tok += kWarps / share) {
         const TokenPlace w = place[st][tok];
-        float x1[8] = {}, x2[8] = {};
+        const uint8_t* src = smem + (st * tokens + tok) * token_bytes;
+        const float* rot = reinterpret_cast<const float*>(src + row_bytes + v1_bytes) + sub * 8;
+        float cs[8], sn[8];
         if (w.page >= 0) {
-          const uint8_t* src = smem + (st * tokens + tok) * token_bytes;
-          unpack8(*reinterpret_cast<const bf16x8*>(src + (slot * HD + sub * 8) * 2), x1);
-          unpack8(*reinterpret_cast<const bf16x8*>(src + (slot * HD + HALF + sub * 8) * 2), x2);
-          const bf16x8* u = reinterpret_cast<const bf16x8*>(src + row_bytes + ((slot - nrot) * HD + sub * 8) * 2);
-          const float* cos = reinterpret_cast<const float*>(src + row_bytes + v1_bytes) + sub * 8;
-          finish<HD>(p, slot, cos, cos + HALF, v1_bytes != 0 ? u : nullptr, u + HALF / 8, c, a1, a2, qg, x1, x2);
+          load8<float>(rot, cs);
+          load8<float>(rot + HALF, sn);
         }
-        store_item<HD>(p, t0 + tok, w, slot, sub, x1, x2);
+#pragma unroll 2
+        for (int slot = warp % share * kHeads + head; slot < nslots; slot += share * kHeads) {  // the LPH lanes of a head stay together
+          float x1[8] = {}, x2[8] = {};
+          if (w.page >= 0) {
+            unpack8(*reinterpret_cast<const bf16x8*>(src + (slot * HD + sub * 8) * 2), x1);
+            unpack8(*reinterpret_cast<const bf16x8*>(src + (slot * HD + HALF + sub * 8) * 2), x2);
+            const bf16x8* u = reinterpret_cast<const bf16x8*>(src + row_bytes + ((slot - nrot) * HD + sub * 8) * 2);
+            finish<HD>(p, slot, cs, sn, v1_bytes != 0 ? u : nullptr, u + HALF / 8, c, a1, a2, qg, x1, x2);
+          }
+          store_item<HD>(p, t0 + tok, w, slot, sub, x1, x2);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&empty[st]));
+      if (++st == ring) st = 0, ph ^= 1;
     }
   }
   if (*static_cast<volatile int*>(&abort_flag) != 0) {
@@ -261,11 +273,13 @@ template <int HD>
 int launch(const PagedAppendParams& p, cudaStream_t st) {
   const int nslots = p.H + 2 * p.Hkv, per_token = nslots * (HD / 16);
   const int token_bytes = nslots * HD * 2 + (p.v1 != nullptr ? p.Hkv * HD * 2 : 0) + HD * 4;
-  int tokens = kSmemCta / kRing / token_bytes;
+  int tokens = kMaxTokens;
+  while (tokens > 0 && 2 * tokens * token_bytes > kSmemCta) tokens /= 2;
   if ((int64_t)p.T * per_token <= 148 * 2 * kThreads || tokens == 0) {
     paged_append_few_kernel<HD><<<p.T, kThreads, 0, st>>>(p);
   } else {
-    if (tokens > kMaxTokens) tokens = kMaxTokens;
+    int ring = kSmemCta / (tokens * token_bytes);
+    if (ring > kRing) ring = kRing;
     static bool configured[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
@@ -274,7 +288,7 @@ int launch(const PagedAppendParams& p, cudaStream_t st) {
       configured[dev] = true;
     }
     const int groups = (p.T + tokens - 1) / tokens;
-    paged_append_ring_kernel<HD><<<groups < 148 * 2 ? groups : 148 * 2, kThreads + 32, kRing * tokens * token_bytes, st>>>(p, tokens, token_bytes);
+    paged_append_ring_kernel<HD><<<groups < 148 * 2 ? groups : 148 * 2, kThreads + 32, ring * tokens * token_bytes, st>>>(p, tokens, ring, token_bytes);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
