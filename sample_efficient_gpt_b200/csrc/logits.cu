@@ -11,8 +11,7 @@
 // the biases, so that no second array is needed and the call may work in place.
 #include <type_traits>
 
-#include "common.cuh"
-#include "paged.h"
+#include "paged_common.cuh"
 
 namespace seg {
 
@@ -43,9 +42,9 @@ template <> struct Pack<float, 4> {
   __device__ void set(const float* f) { v = make_float4(f[0], f[1], f[2], f[3]); }
 };
 template <> struct Pack<__nv_bfloat16, 8> {
-  bf16x8 v;
-  __device__ void get(float* f) const { unpack8(v, f); }
-  __device__ void set(const float* f) { v = pack8(f); }
+  uint4 v;
+  __device__ void get(float* f) const { unpack8(load16(&v), f); }
+  __device__ void set(const float* f) { store16(&v, pack8(f)); }
 };
 template <typename T> struct Pack<T, 1> {
   T v;

@@ -11,8 +11,7 @@
 // loads (length -> page -> rotation).  Many: that chain, longer by the search for the token's sequence, would stand in front
 // of every CTA's work, so a producer warp runs it ahead and brings each group of tokens - projection rows, first values,
 // rotation rows - into a ring in shared memory with bulk copies, from which eight warps compute and store.
-#include "common.cuh"
-#include "paged.h"
+#include "paged_common.cuh"
 #include "sm100.cuh"
 
 namespace seg {
@@ -72,7 +71,7 @@ __device__ __forceinline__ TokenPlace find_place(const PagedAppendParams& p, int
 
 // An item's 16 elements -> the finished query, key or value elements.  u1, u2: the first block's values (or nullptr).
 template <int HD>
-__device__ __forceinline__ void finish(const PagedAppendParams& p, int slot, const float* cs, const float* sn, const bf16x8* u1, const bf16x8* u2, float c,
+__device__ __forceinline__ void finish(const PagedAppendParams& p, int slot, const float* cs, const float* sn, const void* u1, const void* u2, float c,
                                        float a1, float a2, float qg, float* x1, float* x2) {
   if (slot < p.H + p.Hkv) {
     float ss = 0.f;
@@ -95,8 +94,8 @@ __device__ __forceinline__ void finish(const PagedAppendParams& p, int slot, con
   } else {
     float w1[8], w2[8];
     if (u1 != nullptr) {
-      unpack8(*u1, w1);
-      unpack8(*u2, w2);
+      unpack8(load16(u1), w1);
+      unpack8(load16(u2), w2);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -113,8 +112,8 @@ __device__ __forceinline__ void store_item(const PagedAppendParams& p, int64_t t
   const bf16x8 y1 = pack8(x1), y2 = pack8(x2);
   if (slot < p.H) {
     __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.q) + (t * p.H + slot) * HD + sub * 8;
-    *reinterpret_cast<bf16x8*>(dst) = y1;
-    *reinterpret_cast<bf16x8*>(dst + HALF) = y2;
+    store16(dst, y1);
+    store16(dst + HALF, y2);
     return;
   }
   const bool is_k = slot < p.H + p.Hkv;
@@ -122,14 +121,14 @@ __device__ __forceinline__ void store_item(const PagedAppendParams& p, int64_t t
   if (w.page >= 0) {
     __nv_bfloat16* dst = is_k ? static_cast<__nv_bfloat16*>(p.pool.k) + w.page * p.pool.k_page + w.slot * p.pool.k_slot + h * p.pool.k_head
                               : static_cast<__nv_bfloat16*>(p.pool.v) + w.page * p.pool.v_page + w.slot * p.pool.v_slot + h * p.pool.v_head;
-    *reinterpret_cast<bf16x8*>(dst + sub * 8) = y1;
-    *reinterpret_cast<bf16x8*>(dst + HALF + sub * 8) = y2;
+    store16(dst + sub * 8, y1);
+    store16(dst + HALF + sub * 8, y2);
   }
   void* out = is_k ? p.k_out : p.v_out;
   if (out != nullptr) {
     __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(out) + (t * p.Hkv + h) * HD + sub * 8;
-    *reinterpret_cast<bf16x8*>(dst) = y1;
-    *reinterpret_cast<bf16x8*>(dst + HALF) = y2;
+    store16(dst, y1);
+    store16(dst + HALF, y2);
   }
 }
 
@@ -146,12 +145,12 @@ __global__ void __launch_bounds__(kThreads) paged_append_few_kernel(const PagedA
     const bool live = item < n_items;
     bf16x8 x[2], u[2];
     if (live) {  // on their way before anything is known about where the token goes
-      x[0] = *reinterpret_cast<const bf16x8*>(row + slot * HD + sub * 8);
-      x[1] = *reinterpret_cast<const bf16x8*>(row + slot * HD + HALF + sub * 8);
+      x[0] = load16(row + slot * HD + sub * 8);
+      x[1] = load16(row + slot * HD + HALF + sub * 8);
       if (slot >= nrot && p.v1 != nullptr) {
         const __nv_bfloat16* v1 = static_cast<const __nv_bfloat16*>(p.v1) + (t * p.Hkv + (slot - nrot)) * HD + sub * 8;
-        u[0] = *reinterpret_cast<const bf16x8*>(v1);
-        u[1] = *reinterpret_cast<const bf16x8*>(v1 + HALF);
+        u[0] = load16(v1);
+        u[1] = load16(v1 + HALF);
       }
     }
     const float a1 = *p.alpha1, a2 = *p.alpha2, qg = *p.qgain, c = *p.vscale * rsqrtf(a1 * a1 + a2 * a2 + kMixEps);
@@ -251,10 +250,10 @@ __global__ void __launch_bounds__(kThreads + 32) paged_append_ring_kernel(const 
         for (int slot = warp % share * kHeads + head; slot < nslots; slot += share * kHeads) {  // the LPH lanes of a head stay together
           float x1[8] = {}, x2[8] = {};
           if (w.page >= 0) {
-            unpack8(*reinterpret_cast<const bf16x8*>(src + (slot * HD + sub * 8) * 2), x1);
-            unpack8(*reinterpret_cast<const bf16x8*>(src + (slot * HD + HALF + sub * 8) * 2), x2);
-            const bf16x8* u = reinterpret_cast<const bf16x8*>(src + row_bytes + ((slot - nrot) * HD + sub * 8) * 2);
-            finish<HD>(p, slot, cs, sn, v1_bytes != 0 ? u : nullptr, u + HALF / 8, c, a1, a2, qg, x1, x2);
+            unpack8(load16(src + (slot * HD + sub * 8) * 2), x1);
+            unpack8(load16(src + (slot * HD + HALF + sub * 8) * 2), x2);
+            const uint8_t* u = src + row_bytes + ((slot - nrot) * HD + sub * 8) * 2;
+            finish<HD>(p, slot, cs, sn, v1_bytes != 0 ? u : nullptr, u + HD, c, a1, a2, qg, x1, x2);
           }
           store_item<HD>(p, t0 + tok, w, slot, sub, x1, x2);
         }

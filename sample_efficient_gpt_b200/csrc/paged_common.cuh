@@ -1,4 +1,4 @@
-// What the kernels of the paged attention share: the plan of a call, the checked reads of lengths and group borders, and the
+// What the paged kernels share: 16-byte accesses; of the attention the plan of a call, the checked reads of lengths and group borders, and the
 // dealing of key tiles to CTAs.
 #pragma once
 #include <cuda.h>
@@ -7,6 +7,25 @@
 #include "paged.h"
 
 namespace seg {
+
+// Eight bf16 in one 16-byte access.  (The compiler splits the copy of a structure of bf16 pairs into 4-byte accesses.)
+__device__ __forceinline__ bf16x8 load16(const void* p) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  bf16x8 r;
+  r.v[0] = *reinterpret_cast<const __nv_bfloat162*>(&v.x);
+  r.v[1] = *reinterpret_cast<const __nv_bfloat162*>(&v.y);
+  r.v[2] = *reinterpret_cast<const __nv_bfloat162*>(&v.z);
+  r.v[3] = *reinterpret_cast<const __nv_bfloat162*>(&v.w);
+  return r;
+}
+__device__ __forceinline__ void store16(void* p, const bf16x8& r) {
+  uint4 v;
+  v.x = *reinterpret_cast<const uint32_t*>(&r.v[0]);
+  v.y = *reinterpret_cast<const uint32_t*>(&r.v[1]);
+  v.z = *reinterpret_cast<const uint32_t*>(&r.v[2]);
+  v.w = *reinterpret_cast<const uint32_t*>(&r.v[3]);
+  *reinterpret_cast<uint4*>(p) = v;
+}
 
 // Which kernel walks over the prefixes: 16 rows at a time next to the sequences' own pages (paged_attn.cu), or one of the two
 // tcgen05 forms (paged_prefix.cu): 256 rows of one group per CTA, or 128 rows with the keys dealt to the two halves of a CTA.
