@@ -1,6 +1,7 @@
 // Python bindings of the paged serving kernels (paged_append.cu, paged_attn.cu, logits.cu).  Everything that can be known on
 // the host is checked here; lengths, page numbers and group borders live on the device and are checked by the kernels.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -17,6 +18,11 @@ using torch::Tensor;
 using OptTensor = std::optional<Tensor>;
 
 cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+// Straight from the allocator: the small calls are bound by the host.
+Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const c10::Device& dev) {
+  return at::detail::empty_cuda(sizes, type, dev, std::nullopt);
+}
 
 void check_on(const Tensor& t, const c10::Device& dev, const char* name) {
   TORCH_CHECK(t.device() == dev, name, " must be on ", dev, ", got ", t.device());
@@ -128,10 +134,10 @@ std::tuple<Tensor, OptTensor, OptTensor> paged_append(const Tensor& qkv, const O
   p.T = (int)T; p.B = (int)B; p.H = (int)H; p.Hkv = (int)Hkv; p.hd = (int)hd;
   p.rope_rows = (int)cos.size(0);
   p.qknorm = qknorm;
-  Tensor q = torch::empty({T, H, hd}, qkv.options());
+  Tensor q = new_tensor({T, H, hd}, at::kBFloat16, dev);
   OptTensor k, v;
-  if (want_k) k = torch::empty({T, Hkv, hd}, qkv.options());
-  if (want_v) v = torch::empty({T, Hkv, hd}, qkv.options());
+  if (want_k) k = new_tensor({T, Hkv, hd}, at::kBFloat16, dev);
+  if (want_v) v = new_tensor({T, Hkv, hd}, at::kBFloat16, dev);
   p.q = q.data_ptr();
   p.k_out = want_k ? k->data_ptr() : nullptr;
   p.v_out = want_v ? v->data_ptr() : nullptr;
@@ -191,13 +197,13 @@ std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor& k_page
   const int64_t longest = std::max<int64_t>(p.table_width, p.ptable_width) * p.pool.P;
   TORCH_CHECK(longest < (int64_t)1 << 30, "page tables may hold at most 2^30 tokens per sequence");
   TORCH_CHECK((longest / 64 + 1) * (B + G) * H < (int64_t)1 << 31, "batch x heads x page-table width is too large for one call");
-  Tensor o = torch::empty({B, H, hd}, q.options());
-  Tensor lse = torch::empty({B, H}, q.options().dtype(at::kFloat));
+  Tensor o = new_tensor({B, H, hd}, at::kBFloat16, dev);
+  Tensor lse = new_tensor({B, H}, at::kFloat, dev);
   p.o = o.data_ptr();
   p.lse = lse.data_ptr<float>();
   const int64_t bytes = seg::paged_attn_workspace(p);
   TORCH_CHECK(bytes >= 0, "at most 8192 sequences and groups in one call, got ", B + G);
-  Tensor ws = torch::empty({bytes}, q.options().dtype(at::kByte));
+  Tensor ws = new_tensor({bytes}, at::kByte, dev);
   const int rc = seg::paged_attn(p, ws.data_ptr(), cur_stream());
   TORCH_CHECK(rc == 0, "paged_attention failed with code ", rc);
   return {o, lse};
@@ -281,7 +287,7 @@ Tensor process_logits(const Tensor& logits, const OptTensor& tokens, const OptTe
       TORCH_CHECK(hi(y) <= lo(logits) || hi(logits) <= lo(y), "out must be the logits themselves or memory of its own");
     }
   } else {
-    y = torch::empty({B, V}, logits.options());
+    y = new_tensor({B, V}, logits.scalar_type(), dev);
   }
   p.x = logits.data_ptr();
   p.x_row = logits.stride(0);

@@ -129,6 +129,7 @@ def parse_args(argv=None):
     p.add_argument("-x", "--max-problems", type=int, default=None)
     p.add_argument("--log-file", type=Path, default=None)
     p.add_argument("--device-type", type=str, default="", choices=["", "cuda", "cpu"], help="empty => autodetect")
+    p.add_argument("--paged", action="store_true", help="decode over a paged cache: prompts of any lengths in one batch, samples share their prompt")
     return p.parse_args(argv)
 
 
@@ -146,7 +147,7 @@ def main(argv=None):
     device = torch.device("cuda", local) if cuda else torch.device("cpu")
     if cuda:
         torch.cuda.set_device(device)
-    engine = load_engine(args.checkpoint, device, args.dtype, max_model_len=2048)
+    engine = load_engine(args.checkpoint, device, args.dtype, max_model_len=2048, paged=args.paged)
 
     log_file = args.log_file
     if log_file is not None:

@@ -4,11 +4,17 @@ evals/chat_web.py:89-110).
 
 * ``StaticKVCache``: keys/values in buffers allocated once for ``max_len`` positions and written in place - a decode
   step appends one column instead of re-concatenating the whole cache.
-* ``SamplingParams``: n, max_tokens, temperature, top_k, top_p, stop_token_ids (the subset of vLLM's the evaluations use).
+* ``SamplingParams``: n, max_tokens, temperature, top_k, top_p, stop_token_ids (the subset of vLLM's the evaluations use), and
+  penalties, biases and constraints on the tokens.
 * ``GraphDecoder``: the one-token decode step of a dense model as a CUDA graph over static buffers (token, position,
   per-layer K/V caches of ``max_len`` positions, a position mask): the ~12 small kernels per layer of a decode step are
   launch-bound, a graph replay issues them in one call.  The prompt is prefilled eagerly into the same buffers.
 * ``EngineDecoder``: the same step on the training engine's fused kernels and bf16 weight shadows (default on a GPU).
+* ``PagedDecoder`` (``ChatEngine(paged=True)``): prompts of any lengths in one batch over a paged cache; the ``n`` continuations
+  of a prompt share its pages, so a prompt is prefilled, stored and read once.  Keys and values are appended by
+  ``ops.qkv_post_paged`` and read by ``ops.paged_attention``; the one-token step is a CUDA graph.
+* ``LogitsProcessor``: the repetition / presence / frequency penalties, ``logit_bias``, ``allowed_token_ids`` and ``choices`` of
+  ``SamplingParams`` through ``ops.process_logits``.
 * ``ChatEngine``: renders conversations (tokenizer chat template, else the ``<|user_start|>...`` special-token format,
   else a plain-text fallback), runs prompts of equal length as one batch (the model has no padding mask), samples on the
   device, and checks for "all rows finished" every few steps so the decode loop does not synchronise per token.
@@ -269,6 +275,199 @@ class EngineDecoder:
         return self.logits
 
 
+class PagedDecoder:
+    """Prefill and one-token steps over a paged cache, dense blocks with per-head (or no) gating.
+
+    ``start(prompts, n, budget)`` prefills the prompts (any lengths, each once) and gives the first logits of ``len(prompts) * n``
+    rows; ``step(tokens)`` feeds one token per row.  With ``n`` > 1 a prompt's pages are a prefix that its rows share, and each row has
+    pages of its own for ``budget`` tokens; with one row per prompt both lie in the row's pages.  Buffers (and the graph) are kept
+    between calls and replaced when a call needs more rows or pages.  On a GPU bf16; on the CPU the statements of each op, fp32."""
+
+    PREFILL_TOKENS = 32768  # tokens that one prefill pass takes at most (a longer prompt goes by itself)
+
+    def __init__(self, model, device, engine=None, page_size: int = 64):
+        from sample_efficient_gpt_b200.training.engine import FusedEngine
+
+        at = model.blocks[0].attn
+        if any(b.is_moe for b in model.blocks) or at.gating not in (False, "per-head"):
+            raise ValueError("paged decode supports dense blocks with per-head (or no) gating")
+        self.model, self.device, self.P = model, torch.device(device), page_size
+        self.lp = torch.bfloat16 if self.device.type == "cuda" else torch.float32
+        self.eng = engine if engine is not None else FusedEngine(model, self.lp)
+        self.H, self.Hkv, self.hd = at.n_heads, at.n_kv_heads, at.head_dim
+        self.scales = [float(b.ln1.position_scale) for b in model.blocks]
+        self.final_scale = float(model.final_norm.position_scale)
+        self.pages, self.shape = 0, None
+        self.graph: torch.cuda.CUDAGraph | None = None
+        self.logits: Tensor | None = None
+
+    # ---- buffers
+    def _reserve(self, pages: int, rows: int, width: int, groups: int, prefix_width: int):
+        i32 = lambda *n: torch.zeros(*n, dtype=torch.int32, device=self.device)  # noqa: E731
+        if pages > self.pages:
+            pages = max(pages, self.pages * 3 // 2)
+            # by head, so that a page's tokens of one head lie next to each other
+            mk = lambda: torch.zeros(pages, self.Hkv, self.P, self.hd, dtype=self.lp, device=self.device).transpose(1, 2)  # noqa: E731
+            self.graph = None
+            self.kp = self.vp = None  # before the new pools take their place
+            self.kp, self.vp = [mk() for _ in self.model.blocks], [mk() for _ in self.model.blocks]
+            self.pages = pages
+        old = self.shape
+        if old is None or old[0] != rows or old[2] != groups or width > old[1] or prefix_width > old[3]:
+            if old is not None:
+                width, prefix_width = max(width, old[1]), max(prefix_width, old[3])
+            self.graph = None
+            self.shape = (rows, width, groups, prefix_width)
+            self.token, self.lens, self.pos_base, self.table = torch.zeros(rows, dtype=torch.long, device=self.device), i32(rows), i32(rows), i32(rows, width)
+            self.prefix_table = i32(groups, max(1, prefix_width)) if groups else None
+            self.prefix_lens, self.group_rows = (i32(groups), i32(groups + 1)) if groups else (None, None)
+
+    def _tables(self, prompts: list[list[int]], n: int, budget: int):
+        """Hands out pages and fills the tables; returns the table that the prompts are written through."""
+        P, need = self.P, lambda t: -(-t // self.P)
+        rows, groups = len(prompts) * n, len(prompts) if n > 1 else 0
+        lens = [len(x) for x in prompts]
+        own = [need(budget)] * rows if groups else [need(t + budget) for t in lens]
+        shared = [need(t) for t in lens] if groups else []
+        self._reserve(sum(own) + sum(shared), rows, max(own), groups, max(shared, default=0))
+        at = 0
+
+        def fill(table: Tensor, counts: list[int]):
+            nonlocal at
+            host = torch.full(table.shape, -1, dtype=torch.int32)
+            for i, c in enumerate(counts):
+                host[i, :c] = torch.arange(at, at + c, dtype=torch.int32)
+                at += c
+            table.copy_(host)
+
+        fill(self.table, own)
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+        if groups:
+            fill(self.prefix_table, shared)
+            self.prefix_lens.copy_(i32(lens))
+            self.group_rows.copy_(i32([g * n for g in range(groups + 1)]))
+            self.lens.zero_()
+            self.pos_base.copy_(i32([t for t in lens for _ in range(n)]))
+            return self.prefix_table
+        self.lens.copy_(i32(lens))
+        self.pos_base.zero_()
+        return self.table
+
+    # ---- model
+    def _block(self, i: int, res, delta, v1, attend):
+        """One block; ``attend(i, qkv, v1, qgain)`` -> (o [T, H, hd], v1)."""
+        from sample_efficient_gpt_b200 import ops
+
+        eng, blk = self.eng, self.model.blocks[i]
+        at, scale, T = blk.attn, self.scales[i], res.size(0)
+        x, n1, _, _ = ops.add_rmsnorm_fwd(res, delta, blk.ln1.gain, scale, blk.ln1.eps, self.lp, False)
+        if i in eng.qkvz_w:
+            n_qkv = at.qkv.linear.weight.size(0)
+            qkvz = ops.matmul_nt(n1, eng.qkvz_w[i])
+            qkv, z = qkvz[:, :n_qkv], qkvz[:, n_qkv : n_qkv + self.H].contiguous()
+        else:
+            qkv = ops.matmul_nt(n1, eng._w(at.qkv.linear.weight))
+            z = ops.matmul_nt(n1, eng._w(at.attn_gate.linear.weight)) if at.gating else None
+        o, v1 = attend(i, qkv, v1, at.sdpa_qknorm.gain if at.qknorm else eng._ones)
+        g = ops.gate_fwd(o, z) if at.gating else o.reshape(T, self.H * self.hd)
+        a = ops.matmul_nt(g, eng._w(at.out.linear.weight))
+        y, n2, _, _ = ops.add_rmsnorm_fwd(x, a, blk.ln2.gain, scale, blk.ln2.eps, self.lp, False)
+        _, f = ops.up_swiglu(n2, eng._w(blk.ffn.up.linear.weight))
+        return y, ops.matmul_nt(f, eng._w(blk.ffn.down.linear.weight)), v1
+
+    def _append(self, i: int, qkv, v1, qgain, table, lens, cu, pos_base, want_k: bool, want_v: bool):
+        from sample_efficient_gpt_b200 import ops
+
+        at = self.model.blocks[i].attn
+        return ops.qkv_post_paged(qkv, v1, at.rope.cos, at.rope.sin, qgain, at.alpha1, at.alpha2, at.scale, self.H, self.Hkv, self.hd, at.qknorm,
+                                  self.kp[i], self.vp[i], table, lens, cu, pos_base, want_k=want_k, want_v=want_v)
+
+    def _final(self, res, delta) -> Tensor:
+        from sample_efficient_gpt_b200 import ops
+
+        fn = self.model.final_norm
+        _, hf, _, _ = ops.add_rmsnorm_fwd(res, delta, fn.gain, self.final_scale, fn.eps, self.lp, False)
+        logits = ops.matmul_nt(hf, self.eng._w(self.model.lm_head.linear.weight)).float()
+        return logits * self.model.output_mult if self.model.output_mult != 1.0 else logits
+
+    def _prefill(self, prompts: list[list[int]], table: Tensor) -> Tensor:
+        from sample_efficient_gpt_b200 import ops
+
+        starts = [0]
+        for x in prompts:
+            starts.append(starts[-1] + len(x))
+        ids = torch.tensor([t for x in prompts for t in x], dtype=torch.long, device=self.device)
+        cu = torch.tensor(starts, dtype=torch.int32, device=self.device)
+        none = torch.zeros(len(prompts), dtype=torch.int32, device=self.device)
+
+        def attend(i, qkv, v1, qgain):
+            q, k, v = self._append(i, qkv, v1, qgain, table, none, cu, None, True, True)
+            o = torch.empty_like(q)
+            for a, b in zip(starts, starts[1:]):  # causal over each prompt's own tokens, from the finished keys and values
+                o[a:b] = ops.attention_fwd(q[None, a:b], k[None, a:b], v[None, a:b], True, 0, for_backward=False)[0][0]
+            return o, v if v1 is None else v1
+
+        res, delta, v1 = self.model.embedding.weight.detach()[ids].float(), None, None
+        for i in range(self.model.n_layers):
+            res, delta, v1 = self._block(i, res, delta, v1, attend)
+        last = cu[1:].long() - 1
+        return self._final(res[last], delta[last])
+
+    def _step(self) -> Tensor:
+        from sample_efficient_gpt_b200 import ops
+
+        lens = self.lens + 1  # with the token of this step
+
+        def attend(i, qkv, v1, qgain):
+            q, _, v = self._append(i, qkv, v1, qgain, self.table, self.lens, None, self.pos_base, False, v1 is None)
+            o, _ = ops.paged_attention(q, self.kp[i], self.vp[i], self.table, lens, self.prefix_table, self.prefix_lens, self.group_rows)
+            return o, v if v1 is None else v1
+
+        res, delta, v1 = self.model.embedding.weight.detach()[self.token].float(), None, None
+        for i in range(self.model.n_layers):
+            res, delta, v1 = self._block(i, res, delta, v1, attend)
+        return self._final(res, delta)
+
+    @torch.inference_mode()
+    def start(self, prompts: list[list[int]], n: int, budget: int) -> Tensor:
+        """Logits [len(prompts) * n, V] after the prompts; the rows of a prompt lie next to each other."""
+        if not prompts or not all(prompts) or n < 1 or budget < 1:
+            raise ValueError("start() needs prompts of at least one token, n >= 1 and budget >= 1")
+        longest = max(map(len, prompts)) + budget
+        if longest > self.model.blocks[0].attn.rope.cos.size(0):
+            raise ValueError(f"{longest} positions do not fit the model's rotation table")
+        table, out, a = self._tables(prompts, n, budget), [], 0
+        while a < len(prompts):
+            b, tokens = a + 1, len(prompts[a])
+            while b < len(prompts) and tokens + len(prompts[b]) <= self.PREFILL_TOKENS:
+                tokens += len(prompts[b])
+                b += 1
+            out.append(self._prefill(prompts[a:b], table[a:b]))
+            a = b
+        return torch.cat(out).repeat_interleave(n, dim=0)
+
+    @torch.inference_mode()
+    def step(self, tokens: Tensor, active: Tensor | None = None) -> Tensor:
+        """Feed one token per row; logits [R, V] (a static buffer).  Rows that are not ``active`` stay where they are."""
+        self.token.copy_(tokens.view(-1))
+        if self.device.type != "cuda":
+            self.logits = self._step()
+        else:
+            if self.graph is None:
+                side = torch.cuda.Stream(device=self.device)
+                side.wait_stream(torch.cuda.current_stream(self.device))
+                with torch.cuda.stream(side):
+                    for _ in range(2):
+                        self._step()
+                torch.cuda.current_stream(self.device).wait_stream(side)
+                self.graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(self.graph):
+                    self.logits = self._step()
+            self.graph.replay()
+        self.lens.add_(1 if active is None else active.to(torch.int32))
+        return self.logits
+
+
 @dataclass
 class SamplingParams:
     n: int = 1
@@ -278,6 +477,97 @@ class SamplingParams:
     top_p: float = 1.0
     stop_token_ids: list[int] = field(default_factory=list)
     seed: int | None = None
+    repetition_penalty: float = 1.0  # on tokens of the prompt and the answer: > 1 makes them less likely
+    presence_penalty: float = 0.0  # on tokens of the answer, once
+    frequency_penalty: float = 0.0  # on tokens of the answer, per occurrence
+    logit_bias: dict[int, float] | None = None
+    allowed_token_ids: list[int] | None = None  # no other token is sampled (stop tokens neither, unless they are listed)
+    choices: list[list[int]] | None = None  # the answer is one of these token sequences, none of which begins another
+
+    @property
+    def penalised(self) -> bool:
+        return self.repetition_penalty != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0
+
+
+class LogitsProcessor:
+    """What ``SamplingParams`` asks to be done to a batch's logits before sampling, and the state that it needs."""
+
+    def __init__(self, p: SamplingParams, rows: list[list[int]], budget: int, vocab: int, device):
+        self.p, self.device = p, device
+        R, i32 = len(rows), lambda v: torch.tensor(v, dtype=torch.int32, device=device)
+        full = lambda v: torch.full((R,), float(v), device=device)  # noqa: E731
+        self.args: dict = {}
+        if p.penalised:
+            if not p.repetition_penalty > 0.0 or not all(abs(v) < float("inf") for v in (p.repetition_penalty, p.presence_penalty, p.frequency_penalty)):
+                raise ValueError("repetition_penalty must be positive, and all penalties finite")
+            lens = [len(x) for x in rows]
+            history = torch.full((R, max(lens) + budget), -1, dtype=torch.int32)
+            for r, x in enumerate(rows):
+                history[r, : len(x)] = torch.tensor(x, dtype=torch.int32)
+            self.args.update(tokens=history.to(device), prompt_lens=i32(lens), token_lens=i32(lens), repetition=full(p.repetition_penalty),
+                             presence=full(p.presence_penalty), frequency=full(p.frequency_penalty))
+        if p.logit_bias:
+            if any(not 0 <= t < vocab or not abs(v) < float("inf") for t, v in p.logit_bias.items()):
+                raise ValueError(f"logit_bias takes finite values for tokens in [0, {vocab})")
+            self.args.update(bias_ids=i32(list(p.logit_bias)).expand(R, -1).contiguous(),
+                             bias_values=torch.tensor(list(p.logit_bias.values()), dtype=torch.float32, device=device).expand(R, -1).contiguous())
+        self.state: Tensor | None = None
+        if p.allowed_token_ids is not None or p.choices is not None:
+            if p.allowed_token_ids is not None and p.choices is not None:
+                raise ValueError("allowed_token_ids and choices exclude each other")
+            nodes = [dict.fromkeys(p.allowed_token_ids)] if p.allowed_token_ids is not None else self._trie(p.choices)
+            if not nodes[0] or any(not 0 <= t < vocab for node in nodes for t in node):
+                raise ValueError(f"the answer must be allowed at least one token, all in [0, {vocab})")
+            bits = torch.zeros(len(nodes), (vocab + 31) // 32 * 32, dtype=torch.bool)
+            for i, node in enumerate(nodes):
+                bits[i, list(node)] = True
+            words = (bits.view(len(nodes), -1, 32).long() << torch.arange(32)).sum(-1)
+            self.args.update(mask=torch.where(words >= 2**31, words - 2**32, words).to(torch.int32).to(device), mask_rows=i32([0] * R))
+            if p.choices is not None:
+                # the next node of every node and child token; node len(nodes): the answer is complete (all tokens allowed, none used)
+                wide = max(len(node) for node in nodes)
+                self.children = torch.tensor([list(node) + [-1] * (wide - len(node)) for node in nodes] + [[-1] * wide], device=device)
+                self.next = torch.tensor([list(node.values()) + [0] * (wide - len(node)) for node in nodes] + [[len(nodes)] * wide], device=device)
+                self.end, self.state = len(nodes), torch.zeros(R, dtype=torch.long, device=device)
+
+    @staticmethod
+    def _trie(choices: list[list[int]]) -> list[dict[int, int]]:
+        """Nodes as {token: next node}; the node behind a choice's last token is len(nodes)."""
+        nodes: list[dict[int, int | None]] = [{}]
+        for choice in choices:
+            at = 0
+            for k, t in enumerate(choice):
+                last = k == len(choice) - 1
+                if t in nodes[at] and (last or nodes[at][t] is None):
+                    if last and nodes[at][t] is None:
+                        break  # the same choice again
+                    raise ValueError("no choice may begin another one")
+                if t not in nodes[at]:
+                    nodes[at][t] = None if last else len(nodes)
+                    if not last:
+                        nodes.append({})
+                if not last:
+                    at = nodes[at][t]
+        if not all(choices):
+            raise ValueError("a choice has at least one token")
+        return [{t: len(nodes) if nxt is None else nxt for t, nxt in node.items()} for node in nodes]
+
+    def __call__(self, logits: Tensor) -> Tensor:
+        from sample_efficient_gpt_b200 import ops
+
+        return ops.process_logits(logits, **self.args) if self.args else logits
+
+    def push(self, tokens: Tensor) -> Tensor | None:
+        """Take the sampled tokens [R] into account; rows whose choice is complete (or None)."""
+        if self.p.penalised:
+            self.args["tokens"].scatter_(1, self.args["token_lens"].long()[:, None].clamp(max=self.args["tokens"].size(1) - 1), tokens[:, None].to(torch.int32))
+            self.args["token_lens"] = (self.args["token_lens"] + 1).clamp(max=self.args["tokens"].size(1))
+        if self.state is None:
+            return None
+        hit = self.children[self.state] == tokens[:, None]
+        self.state = torch.where(hit, self.next[self.state], 0).sum(-1).where(self.state != self.end, self.state)
+        self.args["mask_rows"] = torch.where(self.state == self.end, -1, self.state).to(torch.int32)
+        return self.state == self.end
 
 
 def sample_next(logits: Tensor, p: SamplingParams, gen: torch.Generator | None = None) -> Tensor:
@@ -309,7 +599,8 @@ def _message_text(content) -> str:
 class ChatEngine:
     def __init__(self, model, tokenizer, device="cpu", max_model_len: int = 2048, chat_template: str | None = None,
                  dtype: torch.dtype | None = None, sync_every: int = 16, cuda_graphs: bool | None = None, cast_weights: bool = False,
-                 fused_decode: bool | None = None):
+                 fused_decode: bool | None = None, paged: bool = False):
+        """``paged``: decode over a paged cache (``PagedDecoder``), prompts of any lengths in one batch."""
         self.model, self.tokenizer, self.device = model.to(device).eval(), tokenizer, torch.device(device)
         self.max_model_len, self.chat_template, self.sync_every = max_model_len, chat_template, sync_every
         self.autocast = (torch.autocast("cuda", dtype=dtype or torch.bfloat16) if self.device.type == "cuda" else nullcontext())
@@ -329,6 +620,11 @@ class ChatEngine:
         can_fuse = (self.cuda_graphs and (dtype or torch.bfloat16) == torch.bfloat16 and _ops.ext() is not None
                     and self.model.blocks[0].attn.head_dim % 16 == 0)
         self.fused_decode = can_fuse if fused_decode is None else (fused_decode and can_fuse)
+        if paged and not dense:
+            raise ValueError("paged decode supports dense blocks with per-head (or no) gating")
+        if paged and self.device.type == "cuda" and (dtype or torch.bfloat16) != torch.bfloat16:
+            raise ValueError("paged decode runs in bfloat16 on a GPU")
+        self.paged = PagedDecoder(self.model, self.device) if paged else None
 
     # ---- prompt rendering -------------------------------------------------------------------------------------------
     def render(self, messages: list[dict]) -> list[int]:
@@ -365,6 +661,8 @@ class ChatEngine:
         stop = torch.tensor(sorted(set(p.stop_token_ids)), device=self.device, dtype=torch.long)
         out = torch.zeros(B, budget, dtype=torch.long, device=self.device)
         done = torch.zeros(B, dtype=torch.bool, device=self.device)
+        rows = prompt.tolist() if p.penalised else [[]] * B  # a copy from the device only where it is needed
+        process = LogitsProcessor(p, rows, budget, self.model.vocab_size, self.device)
         step_in, steps = prompt, 0
         decoder = None
         if self.cuda_graphs:
@@ -383,10 +681,13 @@ class ChatEngine:
                     last = decoder.prefill(prompt) if t == 0 else decoder.step(step_in)
                 else:
                     last = self.model(step_in, kv_cache=caches)[0][:, -1, :]
-                nxt = sample_next(last, p, gen)
+                nxt = sample_next(process(last), p, gen)
                 if stop.numel():
                     done = done | torch.isin(nxt, stop)
                 out[:, t] = torch.where(done, torch.full_like(nxt, -1), nxt)
+                complete = process.push(nxt)
+                if complete is not None:
+                    done = done | complete
                 step_in, steps = nxt[:, None], t + 1
                 if on_token is not None:
                     if bool(done[0]):
@@ -397,11 +698,63 @@ class ChatEngine:
         rows = out[:, :steps].cpu().tolist()
         return [row[: row.index(-1)] if -1 in row else row for row in rows]
 
+    MAX_PAGED_ROWS = 256
+
+    @torch.inference_mode()
+    def _decode_paged(self, prompts: list[list[int]], p: SamplingParams, gen=None) -> list[list[list[int]]]:
+        """Prompts of any lengths, ``p.n`` rows each -> new token ids per prompt and row (stop token excluded)."""
+        room = [min(p.max_tokens, self.max_model_len - len(x)) for x in prompts]
+        live = [i for i, r in enumerate(room) if r > 0]
+        results: list[list[list[int]]] = [[[] for _ in range(p.n)] for _ in prompts]
+        if not live:
+            return results
+        budget, R = max(room[i] for i in live), len(live) * p.n
+        rows = [prompts[i] for i in live for _ in range(p.n)]
+        limit = torch.tensor([room[i] for i in live for _ in range(p.n)], device=self.device)
+        stop = torch.tensor(sorted(set(p.stop_token_ids)), device=self.device, dtype=torch.long)
+        out = torch.full((R, budget), -1, dtype=torch.long, device=self.device)
+        done = torch.zeros(R, dtype=torch.bool, device=self.device)
+        process = LogitsProcessor(p, rows, budget, self.model.vocab_size, self.device)
+        logits, steps = self.paged.start([prompts[i] for i in live], p.n, budget), 0
+        for t in range(budget):
+            if t > 0:
+                logits = self.paged.step(nxt, ~done)
+            nxt = sample_next(process(logits), p, gen)
+            if stop.numel():
+                done = done | torch.isin(nxt, stop)
+            out[:, t] = torch.where(done, torch.full_like(nxt, -1), nxt)
+            complete = process.push(nxt)
+            done = done | (limit <= t + 1)
+            if complete is not None:
+                done = done | complete
+            steps = t + 1
+            if (t + 1) % self.sync_every == 0 and bool(done.all()):
+                break
+        tokens = out[:, :steps].cpu().tolist()
+        if self.device.type == "cuda":
+            from sample_efficient_gpt_b200.ops import gemm
+
+            code = gemm.status(self.device.index)
+            if code != 0:
+                raise RuntimeError(f"a kernel reported status {code} during generation")
+        for j, i in enumerate(live):
+            for k in range(p.n):
+                row = tokens[j * p.n + k]
+                results[i][k] = row[: row.index(-1)] if -1 in row else row
+        return results
+
     def generate_ids(self, prompts: list[list[int]], p: SamplingParams) -> list[list[list[int]]]:
         """For each prompt, ``p.n`` continuations (token ids)."""
         gen = None
         if p.seed is not None:
             gen = torch.Generator(device=self.device).manual_seed(p.seed)
+        if self.paged is not None:
+            for i, ids in enumerate(prompts):
+                prompts[i] = ids[-(self.max_model_len - 1):]
+            at_once, rows = max(1, self.MAX_PAGED_ROWS // p.n), []
+            for a in range(0, len(prompts), at_once):
+                rows += self._decode_paged(prompts[a : a + at_once], p, gen)
+            return rows
         results: list[list[list[int]] | None] = [None] * len(prompts)
         by_len: dict[int, list[int]] = {}
         for i, ids in enumerate(prompts):
@@ -458,8 +811,9 @@ def load_chat_template(tokenizer_dir) -> str | None:
     return f.read_text() if f.is_file() else None
 
 
-def load_engine(checkpoint: str, device="cuda", dtype: str = "bfloat16", max_model_len: int = 2048) -> ChatEngine:
-    """``checkpoint`` is a converted HF directory (config.json + weights + tokenizer) or a native ``.pt`` file."""
+def load_engine(checkpoint: str, device="cuda", dtype: str = "bfloat16", max_model_len: int = 2048, paged: bool = False) -> ChatEngine:
+    """``checkpoint`` is a converted HF directory (config.json + weights + tokenizer) or a native ``.pt`` file.  ``paged``: see
+    ``ChatEngine``."""
     path = Path(checkpoint)
     if path.is_dir():
         from transformers import AutoTokenizer
@@ -475,4 +829,4 @@ def load_engine(checkpoint: str, device="cuda", dtype: str = "bfloat16", max_mod
         tr = Trainer(load_from=str(path), load_components="infer", **{"trainer.device": str(device)})
         model, tokenizer, template = tr.model, tr.tokenizer, None
     torch_dtype = {"float32": torch.float32, "bfloat16": torch.bfloat16, "auto": None}[dtype]
-    return ChatEngine(model, tokenizer, device, max_model_len, template, torch_dtype, cast_weights=True)
+    return ChatEngine(model, tokenizer, device, max_model_len, template, torch_dtype, cast_weights=True, paged=paged)

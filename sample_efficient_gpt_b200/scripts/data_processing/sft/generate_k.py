@@ -62,6 +62,7 @@ def main(argv=None):
     p.add_argument("--max-new-tokens", type=int, default=384)
     p.add_argument("--temperature", type=float, default=0.7)
     p.add_argument("--top-k", type=int, default=30)
+    p.add_argument("--paged", action="store_true", help="decode over a paged cache: the k samples share their prompt's pages")
     a = p.parse_args(argv)
     from sample_efficient_gpt_b200.evals.generation import load_engine
 
@@ -72,7 +73,7 @@ def main(argv=None):
     if a.limit > 0:
         rows = rows[: a.limit]
     rows = [rows[i] for i in contiguous_shard(len(rows), rank, world)]
-    engine = load_engine(a.model_dir, device_for(rank))
+    engine = load_engine(a.model_dir, device_for(rank), paged=a.paged)
     write_rows(a.output_dir / f"{Path(a.prefix).stem}_rank{rank}.jsonl", generate_rows(rows, engine, a.k, a.max_new_tokens, a.temperature, a.top_k))
 
 
