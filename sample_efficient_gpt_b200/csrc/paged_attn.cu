@@ -35,8 +35,8 @@ constexpr int kItemCost = 1;            // what an item costs next to its steps,
 constexpr int kThreads = kWarps * 32;
 
 template <int HD> struct Cfg {
-  static constexpr int kKeys = HD == 128 ? 16 : 32;        // keys per warp and step
-  static constexpr int kStages = HD == 128 ? 3 : HD == 64 ? 2 : 4;
+  static constexpr int kKeys = 32;                         // keys per warp and step
+  static constexpr int kStages = HD == 32 ? 4 : 2;
   static constexpr int kChunks = HD / 8;                   // 16-byte chunks of a row
   static constexpr int kMat = kKeys * HD * 2;              // K or V of one step
   static constexpr int kStageBytes = 2 * kMat;

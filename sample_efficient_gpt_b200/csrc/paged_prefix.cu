@@ -10,8 +10,8 @@
 // memory).  The key tiles (128 keys; 64 in the kKeys form, which is bound by the latency of its loads and wants more of them in
 // flight) of all items in one row are dealt to one CTA per SM in equal, contiguous ranges.
 //
-// Roles of a CTA (384 threads): warp 0 loads, every lane one box of a page (1 to 16 boxes of 8 to 128 keys a tile) into rings
-// of K and V tiles; keys behind the length come as zeros or are masked, their values are set to zero before the products see
+// Roles of a CTA (384 threads): warps 0 and 3 load K and V, every lane one box of a page (1 to 16 boxes of 8 to 128 keys a
+// tile) into rings of tiles; keys behind the length come as zeros or are masked, their values are set to zero before the products see
 // them; warps 1 and 2 issue the products of half 0 / 1; warps 4-7 and 8-11 are the softmax of half 0 / 1, a row per thread.
 //
 // Bound: one exp2 per score, 16 a cycle and SM on the special-function unit: 2048 cycles for 256 x 128 scores against 1024 of
@@ -165,8 +165,11 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   const int64_t ctas = min((int64_t)gridDim.x, total);
   const int64_t t_begin = blockIdx.x < ctas ? total * blockIdx.x / ctas : 0, t_end = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------------------------------------ loads
+  if (warp == 0 || warp == 3) {
+    // ------------------------------------------------------------------------------------------------ loads: K (warp 0), V (warp 3)
+    const bool is_v = warp == 3;
+    uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
+    const CUtensorMap* map = is_v ? &map_v : &map_k;
     int used[2] = {0, 0}, tails = 0;  // tiles so far of each ring
     bool ok = true;
     const bool mine = lane * box < kTileKeys;
@@ -190,23 +193,17 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
         }
         found = lookup(j + 1);
-        const bool cut = s.len < first + kTileKeys && s.len % box != 0;  // the last box brings slots behind the length
-        // K before V: the issuer wants the next scores before it issues the products that free the place of the V tile.
+        const bool mend = is_v && s.len < first + kTileKeys && s.len % box != 0;  // the last box brings slots behind the length
+        const uint32_t dst = (is_v ? L::kV : L::kK) + st * L::kTile, bar = smem_u32(mend ? tail : &full[st]);
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[st]), ph ^ 1, ab, 61 + is_v));
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(bar, L::kTile);
+        __syncwarp();
+        if (mine) {
 #pragma unroll
-        for (int kv = 0; kv < 2 && ok; ++kv) {
-          uint64_t* tile_full = kv == 0 ? &k_full[st] : &v_full[st];
-          const bool mend = kv == 1 && cut;
-          const uint32_t dst = (kv == 0 ? L::kK : L::kV) + st * L::kTile, bar = smem_u32(mend ? tail : tile_full);
-          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(kv == 0 ? &k_empty[st] : &v_empty[st]), ph ^ 1, ab, 61 + kv));
-          if (!ok) break;
-          if (lane == 0) mbar_expect_tx(bar, L::kTile);
-          __syncwarp();
-          if (mine) {
-#pragma unroll
-            for (int b = 0; b < HD / 64; ++b)
-              tma_load_4d(smem_u32(smem) + dst + b * L::kTileBlock + lane * box * 128, kv == 0 ? &map_k : &map_v, bar, b * 64, s.kvh, slot, page);
-          }
-          if (!mend) continue;
+          for (int b = 0; b < HD / 64; ++b) tma_load_4d(smem_u32(smem) + dst + b * L::kTileBlock + lane * box * 128, map, bar, b * 64, s.kvh, slot, page);
+        }
+        if (mend) {
           // values behind the length: zeros, so that no weight of zero meets what lies there
           ok = __all_sync(0xffffffffu, mbar_wait(bar, tails & 1, ab, 63));
           if (!ok) break;
@@ -217,7 +214,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(tile_full));
+          if (lane == 0) mbar_arrive(smem_u32(&full[st]));
         }
       }
       t += s.steps;
