@@ -485,8 +485,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     copy_wait<0>();
   }
   // The prefix kernel before this one let it start early.  It must have ended when this one ends, for the join waits for this
-  // one alone.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // one alone: the last CTA waits for it, and the others make room for those that do not fit beside it yet.
+  if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (*static_cast<volatile int*>(&abort_flag) != 0) {
     for (int i = 0; i < 2000; ++i) __nanosleep(100);  // copies in flight land before the CTA's memory is given away
   }
@@ -644,6 +644,7 @@ int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
   if (!configured[dev]) {
     if (cudaFuncSetAttribute(paged_attn_kernel<HD, kTma>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * (Cfg<HD>::kRing + Cfg<HD>::kStages * kRows * (HD * 2 + kQPad)) + (kMaxLists + 2) * 4) != cudaSuccess) return -2;
+    if (cudaFuncSetAttribute(paged_attn_kernel<HD, kTma>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess) return -2;
     configured[dev] = true;
   }
   // The kernels after the first may be brought in while the one before still runs: the walk over own pages needs nothing of the

@@ -482,6 +482,8 @@ int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
   if (!configured[dev]) {
     if (cudaFuncSetAttribute(paged_prefix_kernel<HD, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return -2;
+    // all of the SM's memory as shared memory: with the least that this kernel needs, no CTA of the next one would fit beside it
+    if (cudaFuncSetAttribute(paged_prefix_kernel<HD, kSplit>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess) return -2;
     configured[dev] = true;
   }
   paged_prefix_kernel<HD, kSplit><<<n.ctas_p, kThreads, L::kSum + (p.G + 1) * 4, st>>>(mk, mv, p, n, ws, box);
