@@ -162,7 +162,13 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;  // scores of half 0 / 1, outputs of half 0 / 1, P of half 0 / 1
   const int64_t total = (int64_t)sum[p.G] * p.Hkv;
-  const int64_t ctas = min((int64_t)gridDim.x, total);
+  // One prefix: a number of CTAs that gives each a part of one item only, where that leaves at most a sixteenth of them idle (a
+  // second part costs a CTA about 5 us: queries, first maximum, outputs).
+  int64_t ctas = min((int64_t)gridDim.x, total);
+  if (p.G == 1 && total > 0) {
+    const int64_t items = (int64_t)p.Hkv * row_tiles(load_group(p, 0), n), even = ctas / items * items;
+    if (even * 16 >= ctas * 15) ctas = even;
+  }
   const int64_t t_begin = blockIdx.x < ctas ? total * blockIdx.x / ctas : 0, t_end = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
 
   if (warp == 0 || warp == 3) {
@@ -357,13 +363,6 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               tmem_ld_wait_regs(v[c & 1]);
               if (c + 1 < kChunks) tmem_ld_32x32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
               scaled(tail_tile, v[c & 1], c, neg2, y, mx);
-              if (c == 0 && i > 0 && pass == 0) {  // P V of the tile before has read the P tile
-                if (!wait(&pv_full[x], (at - 1) & 1, 71)) {
-                  tmem_ld_wait();
-                  return false;
-                }
-                tc_fence_after();
-              }
               if (c == kChunks - 1) {
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 const bool low = top > 8.f || (m == -INFINITY && top > -INFINITY);
@@ -410,6 +409,13 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 const bf16x8 b8 = pack8(e);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) pk[q4 * 4 + k] = *reinterpret_cast<const uint32_t*>(&b8.v[k]);
+              }
+              if (c == 0 && i > 0 && pass == 0) {  // P V of the tile before has read the P tile
+                if (!wait(&pv_full[x], (at - 1) & 1, 71)) {
+                  tmem_ld_wait();
+                  return false;
+                }
+                tc_fence_after();
               }
               tmem_st_32x16(t_p + c * 16, pk);
             }
