@@ -35,8 +35,13 @@ PairWorkspace& pair_workspace(DeviceState& st, const c10::Device& dev, cudaStrea
   return it->second;
 }
 
-DeviceState& device_state(const c10::Device& dev) {
+std::map<int, DeviceState>& device_states() {
   static std::map<int, DeviceState> states;
+  return states;
+}
+
+DeviceState& device_state(const c10::Device& dev) {
+  auto& states = device_states();
   auto it = states.find(dev.index());
   if (it == states.end()) {
     DeviceState st;
@@ -52,6 +57,7 @@ DeviceState& device_state(const c10::Device& dev) {
 // The per-device status word of the GEMM / attention kernels, for other binding files whose kernels report into it
 // (index checks of the debug build).
 int* package_status_ptr(const c10::Device& dev) { return device_state(dev).status.data_ptr<int>(); }
+bool package_status_ready(const c10::Device& dev) { return device_states().count(dev.index()) != 0; }
 
 namespace {
 

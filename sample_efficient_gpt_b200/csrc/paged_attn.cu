@@ -5,7 +5,7 @@
 //
 // Work items: (sequence, kv head, 16 of its query heads) over the sequence's own pages, and (group, kv head, 16 of the group's
 // rows x query heads) over the group's prefix, which is therefore read once per 16 rows and not once per sequence (groups
-// with many rows have a kernel of their own, paged_prefix.cu).  Items are cut into steps of 32 keys (16 at head_dim 128); the
+// with many rows have a kernel of their own, paged_prefix.cu).  Items are cut into steps of 32 keys; the
 // steps of all items in one row are dealt to the warps of one resident wave in equal, contiguous ranges, so that ragged lengths
 // and single long sequences fill the machine alike.  A range that does not hold an item alone leaves (m, l, unnormalised o) in
 // fp32, and a second kernel joins the parts of every row in a fixed order (no atomics: the result does not depend on timing).
@@ -366,14 +366,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const Ring ring{smem_u32(smem + warp * C::kRing), smem_u32(full[warp]), smem_u32(smem + kWarps * C::kRing + warp * q_bytes), n.rows_q};
   int* sum_s = reinterpret_cast<int*>(smem + kWarps * (C::kRing + q_bytes));
   int* sum_p = sum_s + p.B + 1;
-  const Lists L{sum_s, sum_p, n.form == kPrefixSmall ? p.G : 0};
   scan_tiles<kThreads>(sum_s, p.B, [&](int b) { return units_of<HD>(clamp_len(p.lens[b], p.table_width, p.pool.P, p.status)); }, warp_tot);
-  if (L.n_groups > 0) {
-    scan_tiles<kThreads>(sum_p, L.n_groups, [&](int g) {
-      const Group w = load_group(p, g);
-      return units_of<HD>(w.len) * row_tiles(w, n);
-    }, warp_tot);
-  }
+  Lists L{sum_s, sum_p, n.form == kPrefixSmall ? p.G : 0};
+  if (L.n_groups > 0 && !scan_groups<kThreads>(sum_p, p, n, ws, [](int len) { return units_of<HD>(len); }, warp_tot)) L.n_groups = 0;
   const int64_t units_s = (int64_t)sum_s[p.B] * p.Hkv * n.RT, total = units_s + (L.n_groups > 0 ? (int64_t)sum_p[L.n_groups] * p.Hkv : 0);
   // every worker has at least kLeast units (one worker may have less), so the parts of an item have consecutive numbers
   const int64_t workers = min((int64_t)gridDim.x * kWarps, (total + kLeast - 1) / kLeast);
@@ -519,6 +514,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 8) paged_attn_join_kernel(con
       }
     }
     gr = load_group(p, g);
+    if (p.groups != nullptr && ws.meta[n.items_s + n.items_p].x != 0) gr.len = 0;  // borders out of order: no prefixes
   }
   const int len = clamp_len(p.lens[b], p.table_width, p.pool.P, p.status);
   const bool shared = gr.len > 0 && b >= gr.r0 && b < gr.r1;
@@ -527,8 +523,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 8) paged_attn_join_kernel(con
   if (shared) pre = ws.meta[first_item(n, p, g, gr.r0) + kvh * row_tiles(gr, n) + x / n.rows_p];
   if (len > 0) own = ws.meta[(b * p.Hkv + kvh) * n.RT + hl / kRows];
   if (p.G == 0 && own.y == 1) return;  // written by the worker that held the whole item (the same for all warps of the row)
-  // out of order group rows could leave an item without its entry
-  if (pre.x < 0 || pre.y < 0 || (int64_t)pre.x + pre.y > n.items_p + n.ctas_p) pre = make_int2(0, 0);
+  // a wait that gave up leaves items without their entries
+  if (pre.x < 0 || pre.y < 0 || (int64_t)pre.x + pre.y > (int64_t)n.items_p + n.ctas_p) pre = make_int2(0, 0);
+  if (own.x < 0 || own.y < 0 || (int64_t)own.x + own.y > (int64_t)n.items_s + n.workers) own = make_int2(0, 0);
   pre.x *= n.parts_p;
   pre.y *= n.parts_p;
   const int total = pre.y + own.y;
@@ -680,7 +677,7 @@ int64_t paged_attn_workspace(const PagedAttnParams& p) {
   if (p.B + p.G > kMaxLists) return -1;
   const Plan n = make_plan(p);
   const int64_t ss = ((int64_t)n.items_s + n.workers) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas_p) * n.parts_p * n.part_rows_p : 0;
-  return round_up(ss * p.hd * 4) + round_up(ss * 8) + round_up(sp * p.hd * 4) + round_up(sp * 8) + round_up(((int64_t)n.items_s + n.items_p) * 8);
+  return round_up(ss * p.hd * 4) + round_up(ss * 8) + round_up(sp * p.hd * 4) + round_up(sp * 8) + round_up(((int64_t)n.items_s + n.items_p + 1) * 8);
 }
 
 int paged_attn(const PagedAttnParams& p, void* workspace, cudaStream_t st) {

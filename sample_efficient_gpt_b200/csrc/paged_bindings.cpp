@@ -11,6 +11,7 @@
 #include "paged.h"
 
 int* package_status_ptr(const c10::Device& dev);  // gemm_bindings.cpp
+bool package_status_ready(const c10::Device& dev);
 
 namespace {
 
@@ -22,6 +23,17 @@ cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 // Straight from the allocator: the small calls are bound by the host.
 Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const c10::Device& dev) {
   return at::detail::empty_cuda(sizes, type, dev, std::nullopt);
+}
+
+// The status word.  Made by the package's first call on a device; inside a capture it would be the graph's memory, and every
+// replay would clear it.
+int* status_word(const c10::Device& dev) {
+  if (!package_status_ready(dev)) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    TORCH_CHECK(cudaStreamIsCapturing(cur_stream(), &capture) == cudaSuccess && capture == cudaStreamCaptureStatusNone,
+                "the first call on a device cannot be captured into a graph: run the step once before");
+  }
+  return package_status_ptr(dev);
 }
 
 void check_on(const Tensor& t, const c10::Device& dev, const char* name) {
@@ -114,6 +126,7 @@ std::tuple<Tensor, OptTensor, OptTensor> paged_append(const Tensor& qkv, const O
     check_contig(*v1, at::kBFloat16, T * Hkv * hd, dev, "v1");
     check_rows16(*v1, dev, "v1");
   }
+  TORCH_CHECK(table.size(1) * k_pages.size(1) < (int64_t)1 << 30, "page tables may hold at most 2^30 tokens per sequence");
   c10::cuda::CUDAGuard guard(dev);
   p.qkv = qkv.data_ptr();
   p.qkv_stride = qkv.stride(0);
@@ -130,7 +143,7 @@ std::tuple<Tensor, OptTensor, OptTensor> paged_append(const Tensor& qkv, const O
   p.lens = lens.data_ptr<int>();
   p.cu = cu.has_value() ? cu->data_ptr<int>() : nullptr;
   p.pos_base = pos_base.has_value() ? pos_base->data_ptr<int>() : nullptr;
-  p.status = package_status_ptr(dev);
+  p.status = status_word(dev);
   p.T = (int)T; p.B = (int)B; p.H = (int)H; p.Hkv = (int)Hkv; p.hd = (int)hd;
   p.rope_rows = (int)cos.size(0);
   p.qknorm = qknorm;
@@ -192,11 +205,11 @@ std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor& k_page
   p.groups = groups.has_value() ? groups->data_ptr<int>() : nullptr;
   p.B = (int)B; p.H = (int)H; p.Hkv = (int)Hkv; p.hd = (int)hd; p.G = (int)G;
   p.scale_log2 = (float)(sc * 1.4426950408889634);
-  p.status = package_status_ptr(dev);
+  p.status = status_word(dev);
   // positions and tile numbers are 32-bit inside the kernels
   const int64_t longest = std::max<int64_t>(p.table_width, p.ptable_width) * p.pool.P;
   TORCH_CHECK(longest < (int64_t)1 << 30, "page tables may hold at most 2^30 tokens per sequence");
-  TORCH_CHECK((longest / 64 + 1) * (B + G) * H < (int64_t)1 << 31, "batch x heads x page-table width is too large for one call");
+  TORCH_CHECK((longest / 32 + 2) * (B + G) * H < (int64_t)1 << 31, "batch x heads x page-table width is too large for one call");
   Tensor o = new_tensor({B, H, hd}, at::kBFloat16, dev);
   Tensor lse = new_tensor({B, H}, at::kFloat, dev);
   p.o = o.data_ptr();
@@ -293,7 +306,7 @@ Tensor process_logits(const Tensor& logits, const OptTensor& tokens, const OptTe
   p.x_row = logits.stride(0);
   p.y = y.data_ptr();
   p.y_row = y.stride(0);
-  p.status = package_status_ptr(dev);
+  p.status = status_word(dev);
   const int rc = seg::process_logits(p, cur_stream());
   TORCH_CHECK(rc == 0, "process_logits failed with code ", rc);
   return y;

@@ -49,7 +49,8 @@ struct Work {
   float2* ml_s;    // [items_s + workers, rows_s]
   float* acc_p;    // [(items_p + ctas_p) * parts_p, part_rows_p, HD]
   float2* ml_p;
-  int2* meta;      // [items_s + items_p] first part and number of parts of every item that has tiles
+  int2* meta;      // [items_s + items_p + 1] first part and number of parts of every item that has tiles; x of the last: group_rows
+                   // are out of order (written where there are any)
 };
 
 __device__ __forceinline__ float exp2_(float x) {
@@ -65,12 +66,14 @@ __device__ __forceinline__ int clamp_len(int n, int width, int P, int* status) {
 }
 struct Group {
   int r0, r1, len;
+  bool bad;  // borders out of order
 };
 __device__ __forceinline__ Group load_group(const PagedAttnParams& p, int g) {
   Group w;
   w.r0 = p.groups != nullptr ? p.groups[g] : 0;
   w.r1 = p.groups != nullptr ? p.groups[g + 1] : p.B;
-  if (w.r0 < 0 || w.r1 < w.r0 || w.r1 > p.B) {
+  w.bad = w.r0 < 0 || w.r1 < w.r0 || w.r1 > p.B;
+  if (w.bad) {
     atomicCAS(p.status, 0, kStatusAttnGroups);
     w.r0 = w.r1 = 0;
   }
@@ -112,6 +115,21 @@ __device__ void scan_tiles(int* sum, int n, F tiles, int* warp_tot) {
     sum[i + 1] = at;
   }
   __syncthreads();
+}
+// sum of the groups' tiles (`tiles` of a group's length, for each of its row tiles); false: borders out of order somewhere, and no
+// prefix counts - groups that overlap could hold more rows than the call, beyond every bound that the host has checked.
+template <int kThreads, typename F>
+__device__ bool scan_groups(int* sum, const PagedAttnParams& p, const Plan& n, const Work& ws, F tiles, int* warp_tot) {
+  bool bad = false;
+  scan_tiles<kThreads>(sum, p.G, [&](int g) {
+    const Group w = load_group(p, g);
+    bad |= w.bad;
+    return tiles(w.len) * row_tiles(w, n);
+  }, warp_tot);
+  if (p.groups == nullptr) return true;
+  bad = __syncthreads_or(bad) != 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) ws.meta[n.items_s + n.items_p] = make_int2(bad, 0);
+  return !bad;
 }
 // last i with sum[i] <= t (t < sum[n]); empty lists are passed over
 __device__ __forceinline__ int find_list(const int* sum, int n, int t) {

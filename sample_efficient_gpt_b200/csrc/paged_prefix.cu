@@ -153,15 +153,12 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
-  scan_tiles<kThreads>(sum, p.G, [&](int g) {
-    const Group w = load_group(p, g);
-    return (w.len + kTileKeys - 1) / kTileKeys * row_tiles(w, n);
-  }, warp_tot);
+  const bool in_order = scan_groups<kThreads>(sum, p, n, ws, [](int len) { return (len + kTileKeys - 1) / kTileKeys; }, warp_tot);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;  // scores of half 0 / 1, outputs of half 0 / 1, P of half 0 / 1
-  const int64_t total = (int64_t)sum[p.G] * p.Hkv;
+  const int64_t total = in_order ? (int64_t)sum[p.G] * p.Hkv : 0;
   // One prefix: a number of CTAs that gives each a part of one item only, where that leaves at most a sixteenth of them idle (a
   // second part costs a CTA about 5 us: queries, first maximum, outputs).
   int64_t ctas = min((int64_t)gridDim.x, total);

@@ -167,7 +167,7 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, prefix_table=None
     table entries behind the last page needed are never read.
 
     Lengths, pages and borders are read on the device only: a length beyond its table is cut to the table, a page outside the
-    pool reads as zeros, and groups out of order count as empty; each sets the status word (``ops.gemm.status()``: 53, 54, 55).
+    pool reads as zeros, and with borders out of order no row has a prefix; each sets the status word (``ops.gemm.status()``: 53, 54, 55).
     CUDA: bf16, head_dim 32, 64 or 128, at most 8192 sequences and groups; capturable into a graph."""
     if _use_cuda(q, "paged_attention"):
         _count(2)

@@ -2,6 +2,9 @@
 
 import functools
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -297,6 +300,27 @@ def test_attention_reports_what_does_not_fit():
     assert take_status() == 55
 
 
+@pytest.mark.parametrize("H,rows", [(4, [0, 40, 0, 40, 40]), (4, [0, 40, 40, 40, 30]), (32, [0, 40, 0, 40]), (128, [3, 40, 0, 40])])
+def test_groups_out_of_order_leave_no_prefix(H, rows):
+    """Overlapping groups would hold more rows than the call has; with them no row has a prefix."""
+    lens = [(7 * i) % 50 for i in range(40)]
+    c = cache_case(lens, H, 2, 64, 16, prefix_lens=[200] * (len(rows) - 1), seed=14)
+    o, lse = run_attention(c, rows)
+    assert take_status() == 55
+    check_attention(o, lse, attention_oracle(c["q"], c["ks"], c["vs"], [-1] * 40), 64)
+
+
+def test_overlapping_groups_of_a_long_prefix():
+    """Their tiles together would pass 32 bits: nothing of them is walked over."""
+    c = cache_case([5] * 2048, 1, 1, 64, 16, prefix_lens=[16], seed=15)
+    d = to_dev(c)
+    wide = d["prefix_table"][:, :1].expand(2048, 2**14).contiguous()
+    rows = i32([0, 2048] * 1024 + [0])
+    o, lse = ops.paged_attention(d["q"], d["k_pages"], d["v_pages"], d["page_table"], d["seq_lens"], wide, i32([2**18] * 2048), rows)
+    assert take_status() == 55
+    check_attention(o, lse, attention_oracle(c["q"], c["ks"], c["vs"], [-1] * 2048), 64)
+
+
 # ------------------------------------------------------------------------------------------------------------------ logits
 def logits_case(B, V, L, K, M, dtype, seed=0, tok=torch.int32):
     g = torch.Generator().manual_seed(seed)
@@ -405,6 +429,12 @@ def test_refusals():
                       ((a["prefix_table"], a["prefix_lens"], i32([0, 1, 2])), "group_rows")]:
         with pytest.raises(RuntimeError, match=text):
             call(*pre)
+    with pytest.raises(RuntimeError, match="2\\^30"):
+        call(page_table=torch.zeros(2, 2**26, dtype=torch.int32, device=DEV))
+    with pytest.raises(RuntimeError, match="2\\^30"):
+        good(page_table=torch.zeros(2, 2**26, dtype=torch.int32, device=DEV))
+    with pytest.raises(RuntimeError, match="too large"):  # 128 heads x 2^29 tokens in steps of 32
+        ops.paged_attention(torch.zeros(1, 128, 64, device=DEV, dtype=BF16), a["k_pages"], a["v_pages"], torch.zeros(1, 2**25, dtype=torch.int32, device=DEV), i32([0]))
     with pytest.raises(RuntimeError, match="finite"):
         ops.paged_attention(a["q"], a["k_pages"], a["v_pages"], a["page_table"], a["seq_lens"], scale=float("nan"))
     x = torch.zeros(2, 64, device=DEV)
@@ -415,6 +445,33 @@ def test_refusals():
                        (dict(out=x[:1].expand(2, 64)), "overlap")]:
         with pytest.raises(RuntimeError, match=text):
             ops.process_logits(**{"logits": x, **args})
+
+
+def test_first_call_of_a_process_is_not_captured():
+    """It would put the status word into the graph's memory."""
+    code = """if True:
+        import torch
+        from sample_efficient_gpt_b200 import ops
+        x = torch.zeros(2, 64, device="cuda")
+        g = torch.cuda.CUDAGraph()
+        try:
+            with torch.cuda.graph(g):
+                ops.process_logits(x)
+        except RuntimeError as e:
+            assert "cannot be captured" in str(e), e
+        else:
+            raise SystemExit("captured")
+        ops.process_logits(x)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ops.process_logits(x)
+        x.fill_(3.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert (y == 3).all()
+    """
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600, cwd=Path(__file__).resolve().parents[1])
+    assert r.returncode == 0, r.stdout + r.stderr
 
 
 def test_empty_batches():
