@@ -322,12 +322,12 @@ class PagedDecoder:
             self.prefix_table = i32(groups, max(1, prefix_width)) if groups else None
             self.prefix_lens, self.group_rows = (i32(groups), i32(groups + 1)) if groups else (None, None)
 
-    def _tables(self, prompts: list[list[int]], n: int, budget: int):
+    def _tables(self, prompts: list[list[int]], n: int, budget: list[int]):
         """Hands out pages and fills the tables; returns the table that the prompts are written through."""
         P, need = self.P, lambda t: -(-t // self.P)
         rows, groups = len(prompts) * n, len(prompts) if n > 1 else 0
         lens = [len(x) for x in prompts]
-        own = [need(budget)] * rows if groups else [need(t + budget) for t in lens]
+        own = [need(b) for b in budget for _ in range(n)] if groups else [need(t + b) for t, b in zip(lens, budget)]
         shared = [need(t) for t in lens] if groups else []
         self._reserve(sum(own) + sum(shared), rows, max(own), groups, max(shared, default=0))
         at = 0
@@ -429,11 +429,13 @@ class PagedDecoder:
         return self._final(res, delta)
 
     @torch.inference_mode()
-    def start(self, prompts: list[list[int]], n: int, budget: int) -> Tensor:
-        """Logits [len(prompts) * n, V] after the prompts; the rows of a prompt lie next to each other."""
-        if not prompts or not all(prompts) or n < 1 or budget < 1:
+    def start(self, prompts: list[list[int]], n: int, budget: int | list[int]) -> Tensor:
+        """Logits [len(prompts) * n, V] after the prompts; the rows of a prompt lie next to each other.  ``budget``: tokens that
+        rows may take, one number or one for each prompt; a row that has taken them must not be active any more."""
+        budget = [budget] * len(prompts) if isinstance(budget, int) else list(budget)
+        if not prompts or not all(prompts) or n < 1 or len(budget) != len(prompts) or min(budget) < 1:
             raise ValueError("start() needs prompts of at least one token, n >= 1 and budget >= 1")
-        longest = max(map(len, prompts)) + budget
+        longest = max(len(x) + b for x, b in zip(prompts, budget))
         if longest > self.model.blocks[0].attn.rope.cos.size(0):
             raise ValueError(f"{longest} positions do not fit the model's rotation table")
         table, out, a = self._tables(prompts, n, budget), [], 0
@@ -715,7 +717,7 @@ class ChatEngine:
         out = torch.full((R, budget), -1, dtype=torch.long, device=self.device)
         done = torch.zeros(R, dtype=torch.bool, device=self.device)
         process = LogitsProcessor(p, rows, budget, self.model.vocab_size, self.device)
-        logits, steps = self.paged.start([prompts[i] for i in live], p.n, budget), 0
+        logits, steps = self.paged.start([prompts[i] for i in live], p.n, [room[i] for i in live]), 0
         for t in range(budget):
             if t > 0:
                 logits = self.paged.step(nxt, ~done)

@@ -51,6 +51,18 @@ def test_paged_greedy_is_the_plain_decode(kw):
     assert paged.generate_ids([list(PROMPTS[1])], p) == [a[1]]
 
 
+def test_a_long_prompt_beside_a_short_one():
+    """Each row stops where its own prompt leaves no room, up to the last position of the rotation table."""
+    m = model(max_seq_len=40)
+    prompts = [[5] * 37, [7, 8, 9]]
+    for n in (1, 2):
+        p = SamplingParams(n=n, max_tokens=100, temperature=0.0)
+        a = ChatEngine(m, Tok(), "cpu", max_model_len=40).generate_ids([list(x) for x in prompts], p)
+        engine = ChatEngine(m, Tok(), "cpu", max_model_len=40, paged=True)
+        engine.paged.P = 4
+        assert engine.generate_ids([list(x) for x in prompts], p) == a and [len(r[0]) for r in a] == [3, 37]
+
+
 def test_paged_step_logits_match_the_full_forward():
     m = model()
     dec = PagedDecoder(m, "cpu", page_size=3)
