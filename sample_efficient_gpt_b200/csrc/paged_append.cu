@@ -274,7 +274,9 @@ int launch(const PagedAppendParams& p, cudaStream_t st) {
   const int token_bytes = nslots * HD * 2 + (p.v1 != nullptr ? p.Hkv * HD * 2 : 0) + HD * 4;
   int tokens = kMaxTokens;
   while (tokens > 0 && 2 * tokens * token_bytes > kSmemCta) tokens /= 2;
-  if ((int64_t)p.T * per_token <= 148 * 2 * kThreads || tokens == 0) {
+  // Up to four CTAs' items per SM.  A CTA per token against the ring, us: 18 + 12 heads of 64 3.2 / 6.1 for 256 tokens, 5.6 / 6.4 for
+  // 1024, 9.1 / 7.5 for 2048, 140.9 / 59.5 for 32768; 32 + 16 heads of 128 5.6 / 5.9 for 256, 6.3 / 6.5 for 512, 9.9 / 9.1 for 1024.
+  if ((int64_t)p.T * per_token <= 148 * 4 * kThreads || tokens == 0) {
     paged_append_few_kernel<HD><<<p.T, kThreads, 0, st>>>(p);
   } else {
     int ring = kSmemCta / (tokens * token_bytes);

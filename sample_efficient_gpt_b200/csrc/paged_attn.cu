@@ -30,8 +30,9 @@ namespace {
 constexpr int kWarps = 2;               // small CTAs: one or two fit next to a CTA of the prefix kernel
 constexpr int kJoinWarps = 4;
 constexpr int kRows = 16;               // query rows per item
-constexpr int kLeast = 2;               // units of a worker where there are few
-constexpr int kItemCost = 1;            // what an item costs next to its steps, in steps
+// What an item costs next to its steps (queries, first maximum, outputs), in steps.  64 ragged sequences of up to 8192 tokens:
+// 79.6 us at 0, 73.2 at 1, 72.9 at 2; 1000 sequences of up to 64: 40.3, 37.0, 37.0.
+constexpr int kItemCost = 1;
 constexpr int kThreads = kWarps * 32;
 
 template <int HD> struct Cfg {
@@ -370,8 +371,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   Lists L{sum_s, sum_p, n.form == kPrefixSmall ? p.G : 0};
   if (L.n_groups > 0 && !scan_groups<kThreads>(sum_p, p, n, ws, [](int len) { return units_of<HD>(len); }, warp_tot)) L.n_groups = 0;
   const int64_t units_s = (int64_t)sum_s[p.B] * p.Hkv * n.RT, total = units_s + (L.n_groups > 0 ? (int64_t)sum_p[L.n_groups] * p.Hkv : 0);
-  // every worker has at least kLeast units (one worker may have less), so the parts of an item have consecutive numbers
-  const int64_t workers = min((int64_t)gridDim.x * kWarps, (total + kLeast - 1) / kLeast);
+  // every worker has a unit, so the parts of an item have consecutive numbers.  (At least two or four for each: 700 tokens of one
+  // sequence take 9.1 and 11.4 us instead of 7.9.)
+  const int64_t workers = min((int64_t)gridDim.x * kWarps, total);
   const int64_t worker = (int64_t)warp * gridDim.x + blockIdx.x;  // few workers: on SMs of their own
   int64_t t = worker < workers ? total * worker / workers : 0;
   const int64_t t_end = worker < workers ? total * (worker + 1) / workers : 0;
@@ -597,8 +599,24 @@ template <int HD> int smem_bytes(const PagedAttnParams& p, const Plan& n) {
   return kWarps * (Cfg<HD>::kRing + Cfg<HD>::kStages * n.rows_q * (HD * 2 + kQPad)) + (p.B + p.G + 2) * (int)sizeof(int);
 }
 
-// Rows of a kv head per group on average from which the tcgen05 forms are used for the prefixes.
-constexpr int kDenseRows = 32;
+// The tcgen05 forms walk over the prefixes where the small form would read them more than once (more than 16 rows of a kv head
+// in the average group) and would read this many elements of keys in all (tiles of 16 rows x kv heads x tokens that the tables
+// hold x dims).  They start about 10 us later, for their tensor memory, deeper pipeline and larger join, and then pass 128 or 256
+// rows at a time.  Small form against them, us, by millions of elements, prefix alone:
+//   6: 21.8 / 29.7 (128 rows x 12 heads, 1024 tokens)   12: 20.9 / 20.4 (126 x 6, 4096)   16: 25.2 / 27.4 (32 x 8, hd 128, 8000)
+//   18: 28.6 / 30.7 (768 x 6, 1024)   24: 32.5 / 32.0 (128 x 12, 4096)   31: 41.7 / 31.7 (128 x 8, hd 128, 4001)
+//   60: 48.4 / 29.2 (66 x 6, 32768)
+constexpr int64_t kDenseElements = 20 << 20;
+
+PrefixForm prefix_form(const PagedAttnParams& p) {
+  const int64_t gqa = p.H / p.Hkv, rows = p.G > 0 ? p.B * gqa / p.G : 0;  // of an average group
+  if (rows <= kRows || !paged_prefix_usable(p)) return kPrefixSmall;
+  const int64_t tiles = (rows + kRows - 1) / kRows * p.G;
+  if ((double)tiles * p.Hkv * p.hd * p.ptable_width * p.pool.P < kDenseElements) return kPrefixSmall;
+  // 32768 tokens, 6 kv heads, 256 rows at a time against 128: 35.1 / 39.2 us for 129 rows, 43.3 / 45.1 for 255, 54.6 / 54.5 for
+  // 384, 74.3 / 87.1 for 768; up to 128 rows the second half of a CTA has work in the latter form alone: 34.8 / 30.5.
+  return p.hd == 64 && rows > 128 ? kPrefixRows : kPrefixKeys;
+}
 
 Plan make_plan(const PagedAttnParams& p) {
   Plan n;
@@ -606,8 +624,7 @@ Plan make_plan(const PagedAttnParams& p) {
   n.RT = (n.gqa + kRows - 1) / kRows;
   n.rows_s = n.gqa < kRows ? n.gqa : kRows;
   n.items_s = p.B * p.Hkv * n.RT;
-  const int64_t rows = p.G > 0 ? (int64_t)p.B * n.gqa / p.G : 0;
-  n.form = rows >= kDenseRows && paged_prefix_usable(p) ? (p.hd == 64 && rows > 128 ? kPrefixRows : kPrefixKeys) : kPrefixSmall;
+  n.form = prefix_form(p);
   n.rows_q = n.gqa <= 8 && (p.G == 0 || n.form != kPrefixSmall) ? 8 : kRows;
   n.rows_p = n.form == kPrefixSmall ? kRows : n.form == kPrefixRows ? 256 : 128;
   n.parts_p = n.form == kPrefixKeys ? 2 : 1;
@@ -620,8 +637,7 @@ Plan make_plan(const PagedAttnParams& p) {
   else tiles_p = (int64_t)n.items_p * ((p.ptable_width * P + 63) / 64);
   const int smem = (p.hd == 128 ? smem_bytes<128>(p, n) : p.hd == 64 ? smem_bytes<64>(p, n) : smem_bytes<32>(p, n)) + 2048;
   const int per_sm = std::max(1, std::min(228 * 1024 / smem, p.hd == 128 ? 4 : 8));
-  const int64_t ctas = (steps + kLeast - 1) / kLeast;  // worker w sits in CTA w % ctas
-  n.ctas = (int)(ctas < 148 * per_sm ? (ctas < 1 ? 1 : ctas) : 148 * per_sm);
+  n.ctas = (int)(steps < 148 * per_sm ? (steps < 1 ? 1 : steps) : 148 * per_sm);  // worker w sits in CTA w % ctas
   n.workers = n.ctas * kWarps;
   n.ctas_p = n.form == kPrefixSmall ? n.workers : (int)(tiles_p < 148 ? tiles_p : 148);
   return n;
@@ -664,6 +680,8 @@ int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t
   if (cudaLaunchKernelEx(&cfg, paged_attn_kernel<HD, kTma>, mk, mv, p, n, ws, box) != cudaSuccess) return -3;
   cfg.numAttrs = 1;
   cfg.dynamicSmemBytes = 0;
+  // Four warps a row against one, us: 9.1 / 9.8 for 18 rows, 13.2 / 15.5 for 96, 51.8 / 57.0 and 73.1 / 72.3 for 1152; 20.6 / 18.5
+  // for 2304, 120.4 / 112.2 for 4608.
   const bool few = p.B * p.H <= 148 * 8;
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.gridDim = dim3(few ? p.B * p.H : (p.B * p.H + kJoinWarps - 1) / kJoinWarps);
@@ -696,7 +714,8 @@ int paged_attn(const PagedAttnParams& p, void* workspace, cudaStream_t st) {
   ws.ml_p = reinterpret_cast<float2*>(at);
   at += round_up(sp * 8);
   ws.meta = reinterpret_cast<int2*>(at);
-  const bool tma = pool_box(p.pool.P, 8) == 8;  // whole 8-row groups of the swizzle pattern
+  // Whole 8-row groups of the swizzle pattern.  64 ragged sequences of up to 8192 tokens: 73 us, with cp.async 112.
+  const bool tma = pool_box(p.pool.P, 8) == 8;
   switch (p.hd) {
     case 32: return tma ? launch<32, true>(p, n, ws, st) : launch<32, false>(p, n, ws, st);
     case 64: return tma ? launch<64, true>(p, n, ws, st) : launch<64, false>(p, n, ws, st);

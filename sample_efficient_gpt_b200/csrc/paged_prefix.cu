@@ -160,7 +160,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   const uint32_t tmem = *tmem_slot;  // scores of half 0 / 1, outputs of half 0 / 1, P of half 0 / 1
   const int64_t total = in_order ? (int64_t)sum[p.G] * p.Hkv : 0;
   // One prefix: a number of CTAs that gives each a part of one item only, where that leaves at most a sixteenth of them idle (a
-  // second part costs a CTA about 5 us: queries, first maximum, outputs).
+  // second part costs a CTA about 5 us: queries, first maximum, outputs; 256 sequences on 32768 tokens: 74 us, otherwise 78).
   int64_t ctas = min((int64_t)gridDim.x, total);
   if (p.G == 1 && total > 0) {
     const int64_t items = (int64_t)p.Hkv * row_tiles(load_group(p, 0), n), even = ctas / items * items;

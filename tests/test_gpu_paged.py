@@ -152,9 +152,23 @@ def dev_pool(t):
     return out.copy_(t)
 
 
+ROOM = [1]
+
+
+@pytest.fixture(params=[1, 2**19])
+def prefix_room(request):
+    """Tokens that the prefix tables have room for at least: the kernel that walks over a prefix is chosen by it."""
+    ROOM[0] = request.param
+    yield
+    ROOM[0] = 1
+
+
 def run_attention(c, rows=None, **kw):
     kp, vp = dev_pool(c["k_pages"]), dev_pool(c["v_pages"])
     d = to_dev(c)
+    if d["prefix_table"] is not None:
+        more = ROOM[0] // kp.size(1) - d["prefix_table"].size(1)
+        d["prefix_table"] = torch.nn.functional.pad(d["prefix_table"], (0, max(0, more)), value=-1)
     pre = (d["prefix_table"], d["prefix_lens"], None if rows is None else i32(rows)) if rows is not None or d["prefix_table"] is not None else (None,) * 3
     return ops.paged_attention(d["q"], kp, vp, d["page_table"], d["seq_lens"], *pre, **kw)
 
@@ -168,6 +182,7 @@ def test_attention_lengths(H, Hkv, hd, P, layout):
     check_attention(o, lse, attention_oracle(c["q"], c["ks"], c["vs"]), hd)
 
 
+@pytest.mark.usefixtures("prefix_room")
 @pytest.mark.parametrize("H,Hkv,hd", [(18, 6, 64), (4, 4, 32), (32, 8, 128), (40, 2, 64)])
 @pytest.mark.parametrize("P,layout", [(16, "head"), (24, "token"), (64, "token"), (256, "head")])
 def test_attention_shared_prefix(H, Hkv, hd, P, layout):
@@ -179,6 +194,7 @@ def test_attention_shared_prefix(H, Hkv, hd, P, layout):
     check_attention(o, lse, attention_oracle(c["q"], c["ks"], c["vs"], group), hd)
 
 
+@pytest.mark.usefixtures("prefix_room")
 @pytest.mark.parametrize("B,plen,H,Hkv,hd,P", [(1, 5000, 18, 6, 64, 16), (7, 129, 12, 12, 64, 16), (64, 1000, 18, 6, 64, 64), (100, 2100, 24, 2, 64, 32), (70, 513, 32, 8, 128, 128),
                                                (33, 700, 16, 4, 64, 40), (20, 900, 18, 6, 64, 16), (11, 127, 18, 6, 64, 8), (45, 128, 18, 6, 64, 128),
                                                (40, 300, 18, 6, 64, 12)])
@@ -190,6 +206,7 @@ def test_attention_one_prefix_for_all(B, plen, H, Hkv, hd, P):
 
 
 # rows of a kv head per group: few (16 at a time), tens (128, the keys in two halves), hundreds (256)
+@pytest.mark.usefixtures("prefix_room")
 @pytest.mark.parametrize("H,Hkv,hd,P,layout", [(18, 6, 64, 16, "token"), (24, 2, 64, 24, "head"), (32, 8, 128, 32, "head"), (64, 2, 128, 8, "token"), (40, 1, 64, 256, "token")])
 def test_attention_large_groups(H, Hkv, hd, P, layout):
     sizes, plens = [40, 0, 1, 44], [1500, 64, 129, 700]
@@ -201,6 +218,7 @@ def test_attention_large_groups(H, Hkv, hd, P, layout):
     check_attention(o, lse, attention_oracle(c["q"], c["ks"], c["vs"], group), hd)
 
 
+@pytest.mark.usefixtures("prefix_room")
 @pytest.mark.parametrize("B,H,Hkv,hd", [(4, 6, 2, 64), (30, 6, 2, 64), (90, 6, 2, 64), (30, 8, 2, 128)])
 @pytest.mark.parametrize("scale", [0.125, -0.4, 0.0])
 def test_attention_maximum_that_grows(B, H, Hkv, hd, scale):
@@ -216,6 +234,7 @@ def test_attention_maximum_that_grows(B, H, Hkv, hd, scale):
     check_attention(o, lse, attention_oracle(c["q"], c["ks"], c["vs"], [0] * B, scale=scale), hd)
 
 
+@pytest.mark.usefixtures("prefix_room")
 @pytest.mark.parametrize("B", [4, 30, 90])
 def test_attention_prefix_special_values(B):
     """A key that no query can prefer (-inf scores), a query of NaN, a page that does not exist - in every form."""
@@ -241,6 +260,7 @@ def test_attention_prefix_special_values(B):
     assert take_status() == 54
 
 
+@pytest.mark.usefixtures("prefix_room")
 def test_attention_is_the_same_every_time():
     for lens in ([5, 900, 0, 2000, 1], list(range(40)), list(range(120))):
         c = cache_case(lens, 18, 6, 64, 16, "token", [2900], seed=3)
@@ -300,6 +320,7 @@ def test_attention_reports_what_does_not_fit():
     assert take_status() == 55
 
 
+@pytest.mark.usefixtures("prefix_room")
 @pytest.mark.parametrize("H,rows", [(4, [0, 40, 0, 40, 40]), (4, [0, 40, 40, 40, 30]), (32, [0, 40, 0, 40]), (128, [3, 40, 0, 40])])
 def test_groups_out_of_order_leave_no_prefix(H, rows):
     """Overlapping groups would hold more rows than the call has; with them no row has a prefix."""
