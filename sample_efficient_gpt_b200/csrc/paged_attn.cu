@@ -68,11 +68,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 // made l NaN: then the row becomes NaN, as the formula says.
 __device__ __forceinline__ float part_weight(float m, float l, float mm) { return m == -INFINITY ? l : exp2_(m - mm); }
 __device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f; }
-// Byte offset of 16-byte chunk c of row r in a step's K or V: blocks of 64 dims (hd 32: 32), chunks of neighbouring rows permuted
-// (the pattern that TMA writes) so that the eight rows of an ldmatrix phase fall on different banks.
+// Byte offset of 16-byte chunk c of row r in a step's K or V: eight rows at a time, of them blocks of 64 dims (hd 32: 32), chunks of
+// neighbouring rows permuted (the pattern that TMA writes) so that the eight rows of an ldmatrix phase fall on different banks.
 template <int HD> __device__ __forceinline__ uint32_t swz(int r, int c) {
   if (HD == 32) return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
-  return (c >> 3) * (Cfg<HD>::kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+  return (r >> 3) * (HD * 16) + (c >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
 // Addresses of one walk's keys: a list of pages and the kv head inside them.
@@ -209,13 +209,12 @@ __device__ __forceinline__ void load_step(const PagedAttnParams& p, const CUtens
   const int st = it % C::kStages;
   const uint32_t stage = ring.base + st * C::kStageBytes;
   if constexpr (kTma) {
-    // a lane per box: K or V, block of dims, tokens
-    constexpr int kBlocks = HD / 64 > 0 ? HD / 64 : 1;
+    // a lane per box: K or V, tokens
     const uint32_t bar = ring.full + st * 8;
     if (lane == 0) mbar_expect_tx(bar, C::kStageBytes);
     __syncwarp();
-    if (lane < 2 * kBlocks * (C::kKeys / box)) {
-      const int kv = lane & 1, blk = (lane >> 1) % kBlocks, b = (lane >> 1) / kBlocks, key = key0 + b * box;
+    if (lane < 2 * (C::kKeys / box)) {
+      const int kv = lane & 1, b = lane >> 1, key = key0 + b * box;
       int page = p.pool.n_pages, slot = 0;  // outside the pool: zeros
       if (key < w.len) {
         const int j = p.pool.shift >= 0 ? key >> p.pool.shift : key / p.pool.P;
@@ -225,7 +224,7 @@ __device__ __forceinline__ void load_step(const PagedAttnParams& p, const CUtens
           slot = key - j * p.pool.P;
         }
       }
-      tma_load_4d(stage + kv * C::kMat + blk * (C::kKeys * 128) + b * box * (HD < 64 ? 64 : 128), kv ? map_v : map_k, bar, blk * 64, w.kvh, slot, page);
+      load_box(stage + kv * C::kMat + b * box * HD * 2, kv ? map_v : map_k, bar, slot, w.kvh, page);
     }
   } else {
     constexpr int kRowsPer = 32 / C::kChunks;  // rows that the warp covers at once
@@ -500,11 +499,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 8) paged_attn_join_kernel(con
   __shared__ float2 ml_w[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bh = kSplit == 1 ? blockIdx.x * kJoinWarps + warp : blockIdx.x;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (bh >= p.B * p.H) return;  // kSplit 1 only: no barrier follows
   const int b = bh / p.H, h = bh - b * p.H;
   const int kvh = h / n.gqa, hl = h - kvh * n.gqa;
-  // The chain of dependent loads is the cost of this kernel: lengths and group, then both items' entries, then the parts.
+  // The chain of dependent loads is the cost of this kernel: lengths and group (the call's inputs: before the wait), then both
+  // items' entries, then the parts.
   Group gr{0, 0, 0};
   int g = 0;
   if (p.G > 0) {
@@ -516,9 +515,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 8) paged_attn_join_kernel(con
       }
     }
     gr = load_group(p, g);
-    if (p.groups != nullptr && ws.meta[n.items_s + n.items_p].x != 0) gr.len = 0;  // borders out of order: no prefixes
   }
   const int len = clamp_len(p.lens[b], p.table_width, p.pool.P, p.status);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.groups != nullptr && ws.meta[n.items_s + n.items_p].x != 0) gr.len = 0;  // borders out of order: no prefixes
   const bool shared = gr.len > 0 && b >= gr.r0 && b < gr.r1;
   const int x = shared ? (b - gr.r0) * n.gqa + hl : 0, row_p = x % n.rows_p;
   int2 pre = make_int2(0, 0), own = make_int2(0, 0);
@@ -647,7 +647,7 @@ int64_t round_up(int64_t n) { return (n + 255) / 256 * 256; }
 
 template <int HD, bool kTma>
 int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t st) {
-  const int box = pool_box(p.pool.P, Cfg<HD>::kKeys);
+  const int box = pool_box(p.pool.P, HD == 128 ? 8 : Cfg<HD>::kKeys);
   CUtensorMap mk = {}, mv = {};
   if (kTma && (make_pool_map(&mk, p.pool.k, p, p.pool.k_page, p.pool.k_slot, p.pool.k_head, box) != 0 ||
                make_pool_map(&mv, p.pool.v, p, p.pool.v_page, p.pool.v_slot, p.pool.v_head, box) != 0))

@@ -42,8 +42,8 @@ template <int HD, bool kSplit> struct Lay {
   static constexpr int kDepth = 3;                             // places of a ring
   static constexpr int kRings = kSplit ? 2 : 1;                // rings: one for both halves, or one each
   static constexpr int kSlots = kDepth * kRings;
-  static constexpr int kTileBlock = kKeys * 128;               // 64 dims of a K or V tile
-  static constexpr int kTile = HD / 64 * kTileBlock;
+  static constexpr int kGroup = HD / 64 * 1024;                // bytes of 8 keys: blocks of 64 dims behind each other
+  static constexpr int kTile = kKeys / 8 * kGroup;
   static constexpr int kQTile = HD / 64 * kBlock;
   static constexpr int kPCols = 2 * kKeys + 2 * HD;            // tensor memory: first column of P (bf16, two keys a column)
   static_assert(kPCols + kKeys <= 512, "tensor memory");
@@ -202,18 +202,15 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (!ok) break;
         if (lane == 0) mbar_expect_tx(bar, L::kTile);
         __syncwarp();
-        if (mine) {
-#pragma unroll
-          for (int b = 0; b < HD / 64; ++b) tma_load_4d(smem_u32(smem) + dst + b * L::kTileBlock + lane * box * 128, map, bar, b * 64, s.kvh, slot, page);
-        }
+        if (mine) load_box(smem_u32(smem) + dst + lane * box * (HD * 2), map, bar, slot, s.kvh, page);
         if (mend) {
           // values behind the length: zeros, so that no weight of zero meets what lies there
           ok = __all_sync(0xffffffffu, mbar_wait(bar, tails & 1, ab, 63));
           if (!ok) break;
           ++tails;
-          for (int i = (s.len - first) * 8 + lane; i < kTileKeys * 8; i += 32) {
+          for (int i = (s.len - first) * 8 + lane; i < kTileKeys * 8; i += 32) {  // key i / 8, 16 bytes of each block
 #pragma unroll
-            for (int b = 0; b < HD / 64; ++b) *reinterpret_cast<uint4*>(smem + dst + b * L::kTileBlock + i * 16) = make_uint4(0, 0, 0, 0);
+            for (int b = 0; b < HD / 64; ++b) *reinterpret_cast<uint4*>(smem + dst + (i >> 6) * L::kGroup + b * 1024 + (i & 63) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async();
           __syncwarp();
@@ -242,11 +239,11 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           const int at = cx + i, st = (kSplit ? x * L::kDepth : 0) + at % L::kDepth, ph = (at / L::kDepth) & 1;
           if (!mbar_wait(smem_u32(&k_full[st]), ph, ab, 65)) return false;
           if (at > 0 && !mbar_wait(smem_u32(&s_empty[x]), (at - 1) & 1, ab, 66)) return false;
-          const uint64_t d_k = make_smem_desc(smem_u32(smem + L::kK + st * L::kTile), 16, 1024);
+          const uint64_t d_k = make_smem_desc(smem_u32(smem + L::kK + st * L::kTile), 16, L::kGroup);
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k) {
-            const uint64_t oq = (uint64_t)(((k >> 2) * kBlock + (k & 3) * 32) >> 4), ok_ = (uint64_t)(((k >> 2) * L::kTileBlock + (k & 3) * 32) >> 4);
+            const uint64_t oq = (uint64_t)(((k >> 2) * kBlock + (k & 3) * 32) >> 4), ok_ = (uint64_t)(((k >> 2) * 1024 + (k & 3) * 32) >> 4);
             umma_bf16(t_s, d_q + oq, d_k + ok_, idesc_s, k > 0);
           }
           umma_commit(smem_u32(&s_full[x]));
@@ -258,11 +255,11 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           if (i + 1 < mine && !scores(i + 1)) { ok = false; break; }
           const int at = cx + i, st = (kSplit ? x * L::kDepth : 0) + at % L::kDepth, ph = (at / L::kDepth) & 1;
           if (!mbar_wait(smem_u32(&v_full[st]), ph, ab, 67) || !mbar_wait(smem_u32(&p_full[x]), at & 1, ab, 68)) { ok = false; break; }
-          const uint64_t d_v = make_smem_desc(smem_u32(smem + L::kV + st * L::kTile), L::kTileBlock, 1024);
+          const uint64_t d_v = make_smem_desc(smem_u32(smem + L::kV + st * L::kTile), 1024, L::kGroup);
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kTileKeys / 16; ++k)
-            umma_bf16_ts(t_o, t_p + k * 8, d_v + (uint64_t)(k * 128), idesc_o, i > 0 || k > 0);
+            umma_bf16_ts(t_o, t_p + k * 8, d_v + (uint64_t)(2 * k * (L::kGroup >> 4)), idesc_o, i > 0 || k > 0);
           umma_commit(smem_u32(&pv_full[x]));
           umma_commit(smem_u32(&v_empty[st]));
         }
@@ -475,7 +472,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 template <int HD, bool kSplit>
 int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t st) {
   using L = Lay<HD, kSplit>;
-  const int box = pool_box(p.pool.P, L::kKeys);
+  const int box = pool_box(p.pool.P, HD == 128 ? 8 : L::kKeys);
   CUtensorMap mk, mv;
   if (make_pool_map(&mk, p.pool.k, p, p.pool.k_page, p.pool.k_slot, p.pool.k_head, box) != 0 ||
       make_pool_map(&mv, p.pool.v, p, p.pool.v_page, p.pool.v_slot, p.pool.v_head, box) != 0)
