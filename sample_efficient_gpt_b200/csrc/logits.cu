@@ -9,6 +9,8 @@
 // loads a thread are in flight, otherwise their latency bounds the kernel.  Bit 31 of a count says that the prompt has the
 // token, bit 30 that a bias waits for it, bit 29 that more than one does: entries with a bias are left to the threads that hold
 // the biases, so that no second array is needed and the call may work in place.
+// Measured: 512 rows of 100003 fp32, 8192 tokens each, 111 us (418 MB, 3.8 TB/s): 73 as a copy, 88 with biases alone; the
+// counting and the penalties 14, the mask 13.  64 rows of 49152 bf16: 11 us, one row 4.9: one chain of loads after the other.
 #include <type_traits>
 
 #include "paged_common.cuh"
