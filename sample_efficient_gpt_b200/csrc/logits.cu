@@ -21,8 +21,6 @@ namespace {
 
 constexpr uint32_t kPrompt = 1u << 31, kBiased = 1u << 30, kTwice = 1u << 29, kCount = kTwice - 1;
 constexpr int kThreads = 512;
-constexpr int kEntries = 16;                  // entries per thread
-constexpr int kRange = kThreads * kEntries;   // entries per CTA
 constexpr int kBatch = 4;                     // history loads of a thread in flight
 
 struct RowScale {
@@ -70,9 +68,10 @@ __device__ __forceinline__ void count_history(const Tok* tokens, int len, int pr
   }
 }
 
-template <typename T, int VEC, bool kCounts>
-__global__ void __launch_bounds__(kThreads, 3) process_logits_kernel(const LogitsParams p) {
-  constexpr int kVecs = kEntries / VEC;
+// kEntries: entries of a thread, 16 or 32.
+template <typename T, int VEC, bool kCounts, int kEntries>
+__global__ void __launch_bounds__(kThreads, kEntries == 32 ? 2 : 3) process_logits_kernel(const LogitsParams p) {
+  constexpr int kVecs = kEntries / VEC, kRange = kThreads * kEntries;
   extern __shared__ uint4 seen4[];  // [kRange + VEC] counts
   uint32_t* seen = reinterpret_cast<uint32_t*>(seen4);
   const int b = blockIdx.y, tid = threadIdx.x;
@@ -205,11 +204,24 @@ __global__ void __launch_bounds__(kThreads, 3) process_logits_kernel(const Logit
   }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, int kEntries>
 int launch(const LogitsParams& p, cudaStream_t st) {
+  constexpr int kRange = kThreads * kEntries, kSmem = (kRange + VEC + 3) / 4 * 16;
   const dim3 grid((p.V + kRange - 1) / kRange, p.B);
-  if (p.tokens != nullptr || p.K > 0) process_logits_kernel<T, VEC, true><<<grid, kThreads, (kRange + VEC + 3) / 4 * 16, st>>>(p);
-  else process_logits_kernel<T, VEC, false><<<grid, kThreads, 0, st>>>(p);
+  if (p.tokens != nullptr || p.K > 0) {
+    if (kSmem > 48 * 1024) {
+      static bool configured[64] = {};
+      int dev = 0;
+      if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
+      if (!configured[dev]) {
+        if (cudaFuncSetAttribute(process_logits_kernel<T, VEC, true, kEntries>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return -2;
+        configured[dev] = true;
+      }
+    }
+    process_logits_kernel<T, VEC, true, kEntries><<<grid, kThreads, kSmem, st>>>(p);
+  } else {
+    process_logits_kernel<T, VEC, false, kEntries><<<grid, kThreads, 0, st>>>(p);
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
@@ -222,8 +234,13 @@ int process_logits(const LogitsParams& p, cudaStream_t st) {
   // 16-byte accesses need every row of the output at the input's distance from a 16-byte boundary.  64 rows of 49152 bf16: 11.1 us,
   // one entry at a time 15.0; 512 rows of 100003 fp32: 111 and 146.
   const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.y)) & 15) == 0 && (p.B == 1 || ((p.x_row - p.y_row) * size & 15) == 0);
-  if (p.bf16) return aligned ? launch<__nv_bfloat16, 8>(p, st) : launch<__nv_bfloat16, 1>(p, st);
-  return aligned ? launch<float, 4>(p, st) : launch<float, 1>(p, st);
+  if (!p.bf16) return aligned ? launch<float, 4, 16>(p, st) : launch<float, 1, 16>(p, st);
+  if (!aligned) return launch<__nv_bfloat16, 1, 16>(p, st);
+  // bf16, more CTAs than run at once: twice the entries (as many bytes in flight as fp32 has), so that fewer CTAs read a row's history.  16
+  // against 32 entries a thread, rows of 49152, us: 11.2 / 14.4 for 72 rows (432 CTAs), 14.3 / 13.7 for 96 (576), 52.9 / 48.3 for 512; 512 rows
+  // of 100003: 96.4 / 84.2.  For fp32 111.9 / 110.2, and one row 5.1 / 6.5.
+  const bool many = (int64_t)((p.V + kThreads * 16 - 1) / (kThreads * 16)) * p.B > 148 * 3;
+  return many ? launch<__nv_bfloat16, 8, 32>(p, st) : launch<__nv_bfloat16, 8, 16>(p, st);
 }
 
 }  // namespace seg

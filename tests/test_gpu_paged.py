@@ -370,7 +370,8 @@ def check_logits(y, c):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, BF16])
-@pytest.mark.parametrize("B,V,L,K,M", [(1, 1, 1, 1, 1), (3, 33, 40, 5, 2), (2, 8192, 300, 64, 1), (5, 8193, 1, 7, 3), (2, 20011, 2048, 300, 4)])
+@pytest.mark.parametrize("B,V,L,K,M", [(1, 1, 1, 1, 1), (3, 33, 40, 5, 2), (2, 8192, 300, 64, 1), (5, 8193, 1, 7, 3), (2, 20011, 2048, 300, 4),
+                                        (500, 33, 40, 5, 2), (160, 20011, 200, 300, 4), (230, 16385, 64, 9, 3)])
 def test_logits(B, V, L, K, M, dtype):
     c = logits_case(B, V, L, K, M, dtype, seed=V)
     if K > 4:
