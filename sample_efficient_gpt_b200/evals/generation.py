@@ -310,6 +310,7 @@ class PagedDecoder:
             mk = lambda: torch.zeros(pages, self.Hkv, self.P, self.hd, dtype=self.lp, device=self.device).transpose(1, 2)  # noqa: E731
             self.graph = None
             self.kp = self.vp = None  # before the new pools take their place
+            self.pages = 0  # should they not fit
             self.kp, self.vp = [mk() for _ in self.model.blocks], [mk() for _ in self.model.blocks]
             self.pages = pages
         old = self.shape
@@ -455,17 +456,18 @@ class PagedDecoder:
         if self.device.type != "cuda":
             self.logits = self._step()
         else:
-            if self.graph is None:
-                side = torch.cuda.Stream(device=self.device)
-                side.wait_stream(torch.cuda.current_stream(self.device))
-                with torch.cuda.stream(side):
-                    for _ in range(2):
-                        self._step()
-                torch.cuda.current_stream(self.device).wait_stream(side)
-                self.graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(self.graph):
-                    self.logits = self._step()
-            self.graph.replay()
+            with torch.cuda.device(self.device):  # a capture records the current device's streams
+                if self.graph is None:
+                    side = torch.cuda.Stream()
+                    side.wait_stream(torch.cuda.current_stream())
+                    with torch.cuda.stream(side):
+                        for _ in range(2):
+                            self._step()
+                    torch.cuda.current_stream().wait_stream(side)
+                    self.graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(self.graph):
+                        self.logits = self._step()
+                self.graph.replay()
         self.lens.add_(1 if active is None else active.to(torch.int32))
         return self.logits
 

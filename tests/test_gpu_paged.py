@@ -182,6 +182,21 @@ def test_attention_lengths(H, Hkv, hd, P, layout):
     check_attention(o, lse, attention_oracle(c["q"], c["ks"], c["vs"]), hd)
 
 
+@pytest.mark.parametrize("B,H,Hkv,hd,P,most", [(200, 18, 6, 64, 16, 90), (1500, 4, 4, 32, 8, 9), (120, 32, 8, 128, 24, 300), (30, 40, 1, 64, 12, 2000), (70, 17, 1, 64, 16, 700),
+                                               (1300, 1, 1, 64, 16, 40), (1200, 1, 1, 128, 1, 2)])
+def test_attention_many_rows_without_prefix(B, H, Hkv, hd, P, most):
+    """Rows whose sequences are empty, whole in a worker's range, or cut between two or many."""
+    lens = [(37 * b * b) % most if b % 7 else 0 for b in range(B)]
+    lens[B // 2] = 5 * most
+    c = cache_case(lens, H, Hkv, hd, P, "head", seed=B)
+    want = attention_oracle(c["q"], c["ks"], c["vs"])
+    torch.full((B * H * hd * 4,), float("nan"), device=DEV)  # what the allocator hands out next is not zero
+    o, lse = run_attention(c)
+    check_attention(o, lse, want, hd)
+    again = run_attention(c)
+    assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
+
+
 @pytest.mark.usefixtures("prefix_room")
 @pytest.mark.parametrize("H,Hkv,hd", [(18, 6, 64), (4, 4, 32), (32, 8, 128), (40, 2, 64)])
 @pytest.mark.parametrize("P,layout", [(16, "head"), (24, "token"), (64, "token"), (256, "head")])

@@ -63,6 +63,24 @@ def test_a_long_prompt_beside_a_short_one():
         assert engine.generate_ids([list(x) for x in prompts], p) == a and [len(r[0]) for r in a] == [3, 37]
 
 
+def test_decoder_survives_pools_that_do_not_fit(monkeypatch):
+    m = model()
+    dec = PagedDecoder(m, "cpu", page_size=4)
+    want = dec.start(PROMPTS[:2], 1, 3).clone()
+    make = torch.zeros
+
+    def limited(*size, **kw):
+        if len(size) == 4:
+            raise torch.OutOfMemoryError("no room")
+        return make(*size, **kw)
+
+    monkeypatch.setattr(torch, "zeros", limited)
+    with pytest.raises(torch.OutOfMemoryError):
+        dec.start(PROMPTS, 3, 9)
+    monkeypatch.undo()
+    assert torch.equal(dec.start(PROMPTS[:2], 1, 3), want)
+
+
 def test_paged_step_logits_match_the_full_forward():
     m = model()
     dec = PagedDecoder(m, "cpu", page_size=3)
