@@ -62,6 +62,11 @@ __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, ui
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_first(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {  // d = a b
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -259,15 +264,20 @@ __device__ __forceinline__ void attend(const PagedAttnParams& p, int left, const
   const int lane = threadIdx.x & 31;
   {
     const uint32_t sk = ring.base + st * C::kStageBytes, sv = sk + C::kMat;
-    float sc[kN][4] = {};
+    float sc[kN][4];
 #pragma unroll
     for (int kk = 0; kk < HD / 16; ++kk) {
 #pragma unroll
       for (int n = 0; n < kN; n += 2) {
         uint32_t b[4];
         ldsm4(b, sk + swz<HD>(n * 8 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
-        mma(sc[n], qf[kk], b[0], b[1]);
-        mma(sc[n + 1], qf[kk], b[2], b[3]);
+        if (kk == 0) {
+          mma_first(sc[n], qf[kk], b[0], b[1]);
+          mma_first(sc[n + 1], qf[kk], b[2], b[3]);
+        } else {
+          mma(sc[n], qf[kk], b[0], b[1]);
+          mma(sc[n + 1], qf[kk], b[2], b[3]);
+        }
       }
     }
     // relative to the reference; scaled before the mask and the maximum, for the scale may be zero or negative
@@ -293,7 +303,7 @@ __device__ __forceinline__ void attend(const PagedAttnParams& p, int left, const
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int e = 0; e < kE; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], sc[n][e]);
+      for (int e = 0; e < kE; e += 2) mx[e >> 1] = max3(mx[e >> 1], sc[n][e], sc[n][e + 1]);
     bool low = mx[0] > 8.f || (m[0] == -INFINITY && mx[0] > -INFINITY);
     if (!kHalf) low = low || mx[1] > 8.f || (m[1] == -INFINITY && mx[1] > -INFINITY);
     if (__any_sync(0xffffffffu, low)) {  // move the references to the maxima (always in an item's first step, rarely after it)
@@ -376,31 +386,31 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   // sequence take 9.1 and 11.4 us instead of 7.9.)
   const int64_t workers = min((int64_t)gridDim.x * kWarps, total);
   const int64_t worker = (int64_t)warp * gridDim.x + blockIdx.x;  // few workers: on SMs of their own
-  int64_t t = worker < workers ? total * worker / workers : 0;
-  const int64_t t_end = worker < workers ? total * (worker + 1) / workers : 0;
-  if (t < t_end) {
+  const int64_t t0 = worker < workers ? total * worker / workers : 0;
+  const int share = worker < workers ? (int)(total * (worker + 1) / workers - t0) : 0;  // all units of a call fit into 31 bits
+  int t = 0;  // units of the share behind this worker
+  if (t < share) {
     int all, all_ahead;
-    Cursor c = cursor_at<HD>(p, n, L, units_s, t, all);
+    Cursor c = cursor_at<HD>(p, n, L, units_s, t0, all);
     // The loads run ahead: their cursor, the unit that it stands at, items and steps that it has begun.
     Cursor ahead = c;
     all_ahead = all;
-    int64_t t_ahead = t;
-    int items_ahead = 0, it_ahead = 0;
+    int t_ahead = 0, items_ahead = 0, it_ahead = 0;
     load_queries<HD>(p, n, ahead, ring, 0);
     if (kTma) copy_commit();
     const auto load_next = [&]() {
       // over the units that are no steps
-      while (t_ahead < t_end && (ahead.unit < kItemCost || ahead.unit == ahead.units)) {
+      while (t_ahead < share && (ahead.unit < kItemCost || ahead.unit == ahead.units)) {
         if (ahead.unit == ahead.units) {
           next_item<HD>(p, n, L, ahead, all_ahead);
           load_queries<HD>(p, n, ahead, ring, ++items_ahead);
           if (kTma) copy_commit();
         }
-        const int skip = (int)min(t_end - t_ahead, (int64_t)max(0, kItemCost - ahead.unit));
+        const int skip = min(share - t_ahead, max(0, kItemCost - ahead.unit));
         ahead.unit += skip;
         t_ahead += skip;
       }
-      if (t_ahead < t_end) {
+      if (t_ahead < share) {
         load_step<HD, kTma>(p, &map_k, &map_v, box, ahead.w, (ahead.unit - kItemCost) * C::kKeys, ring, it_ahead++);
         ++ahead.unit;
         ++t_ahead;
@@ -411,10 +421,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     int it = 0, items = 0;
 #pragma unroll
     for (int s = 0; s < C::kStages - 1; ++s) load_next();
-    while (t < t_end && ok) {
-      const int units = (int)min(t_end - t, (int64_t)(c.units - c.unit));
+    while (t < share && ok) {
+      const int units = min(share - t, c.units - c.unit);
       const int step0 = max(0, c.unit - kItemCost), steps = max(0, c.unit + units - kItemCost) - step0;
-      if (c.unit == 0 && lane == 0) ws.meta[c.item] = item_parts(c.own ? c.item : c.item - n.items_s, t, c.units, workers, total);
+      if (c.unit == 0 && lane == 0) ws.meta[c.item] = item_parts(c.own ? c.item : c.item - n.items_s, t0 + t, c.units, workers, total);
       float o[HD / 8][4] = {};
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
       uint32_t qf[HD / 16][4];
@@ -475,7 +485,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         }
       }
       t += units;
-      if (t < t_end) {
+      if (t < share) {
         next_item<HD>(p, n, L, c, all);
         ++items;
       }
