@@ -625,6 +625,8 @@ PrefixForm prefix_form(const PagedAttnParams& p) {
   if (rows <= kRows || !paged_prefix_usable(p)) return kPrefixSmall;
   const int64_t tiles = (rows + kRows - 1) / kRows * p.G;
   if ((double)tiles * p.Hkv * p.hd * p.ptable_width * p.pool.P < kDenseElements) return kPrefixSmall;
+  // their parts have room for 256 rows of every group and kv head: with many groups of few rows the small form's take less
+  if ((double)p.Hkv * (p.B * gqa / 128 + p.G + 1) * 256 * p.hd * 4 > 1 << 30) return kPrefixSmall;
   // 32768 tokens, 6 kv heads, 256 rows at a time against 128: 35.1 / 39.2 us for 129 rows, 43.3 / 45.1 for 255, 54.6 / 54.5 for
   // 384, 74.3 / 87.1 for 768; up to 128 rows the second half of a CTA has work in the latter form alone: 34.8 / 30.5.
   return p.hd == 64 && rows > 128 ? kPrefixRows : kPrefixKeys;

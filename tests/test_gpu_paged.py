@@ -234,6 +234,19 @@ def test_attention_large_groups(H, Hkv, hd, P, layout):
 
 
 @pytest.mark.usefixtures("prefix_room")
+@pytest.mark.parametrize("H,Hkv,hd", [(16, 1, 64), (20, 1, 128)])
+def test_attention_many_groups(H, Hkv, hd):
+    sizes = [(5 * g) % 4 for g in range(900)]
+    rows = [0]
+    for n in sizes:
+        rows.append(rows[-1] + n)
+    plens = [(11 * g) % 40 for g in range(900)]
+    c = cache_case([b % 3 for b in range(rows[-1])], H, Hkv, hd, 16, "token", plens, seed=hd)
+    o, lse = run_attention(c, rows)
+    check_attention(o, lse, attention_oracle(c["q"], c["ks"], c["vs"], [g for g, n in enumerate(sizes) for _ in range(n)]), hd)
+
+
+@pytest.mark.usefixtures("prefix_room")
 @pytest.mark.parametrize("B,H,Hkv,hd", [(4, 6, 2, 64), (30, 6, 2, 64), (90, 6, 2, 64), (30, 8, 2, 128)])
 @pytest.mark.parametrize("scale", [0.125, -0.4, 0.0])
 def test_attention_maximum_that_grows(B, H, Hkv, hd, scale):
@@ -386,7 +399,7 @@ def check_logits(y, c):
 
 @pytest.mark.parametrize("dtype", [torch.float32, BF16])
 @pytest.mark.parametrize("B,V,L,K,M", [(1, 1, 1, 1, 1), (3, 33, 40, 5, 2), (2, 8192, 300, 64, 1), (5, 8193, 1, 7, 3), (2, 20011, 2048, 300, 4),
-                                        (500, 33, 40, 5, 2), (160, 20011, 200, 300, 4), (230, 16385, 64, 9, 3)])
+                                        (500, 33, 40, 5, 2), (150, 17003, 100, 12, 3)])
 def test_logits(B, V, L, K, M, dtype):
     c = logits_case(B, V, L, K, M, dtype, seed=V)
     if K > 4:
@@ -594,3 +607,31 @@ def test_side_stream_and_graphs():
     graphs[0].replay()
     now = _decode(c, 18, 6, 64, rows)
     assert torch.equal(outs[0][0], now[0])
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on the GPU: each has its own workspace, and neither waits for the other."""
+    cases = [cache_case([(13 * b) % 70 for b in range(n)], 18, 6, 64, 16, prefix_lens=[p], seed=n) for n, p in ((60, 3000), (90, 2000))]
+    dev = [to_dev(c) for c in cases]
+    room = [torch.nn.functional.pad(d["prefix_table"], (0, 2**15 - d["prefix_table"].size(1)), value=-1) for d in dev]
+    x = torch.randn(64, 5000, device=DEV)
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(6):
+        for d, table, stream in zip(dev, room, streams):
+            with torch.cuda.stream(stream):
+                got.append(ops.paged_attention(d["q"], d["k_pages"], d["v_pages"], d["page_table"], d["seq_lens"], table, d["prefix_lens"]))
+                ops.process_logits(x)
+    torch.cuda.synchronize()
+    for i, (o, lse) in enumerate(got):
+        check_attention(o, lse, attention_oracle(cases[i % 2]["q"], cases[i % 2]["ks"], cases[i % 2]["vs"], [0] * len(cases[i % 2]["q"])), 64)
+        assert torch.equal(o, got[i % 2][0]) and torch.equal(lse, got[i % 2][1])
+
+
+def test_logits_empty_lists():
+    x = torch.randn(3, 70, device=DEV)
+    empty = torch.zeros(3, 0, dtype=torch.int32, device=DEV)
+    y = ops.process_logits(x, tokens=empty, token_lens=i32([0, 0, 0]), repetition=torch.full((3,), 2.0, device=DEV), bias_ids=empty, bias_values=empty.float(),
+                           mask=torch.zeros(0, 3, dtype=torch.int32, device=DEV), mask_rows=i32([-1, -1, -1]))
+    assert torch.equal(x, y)
