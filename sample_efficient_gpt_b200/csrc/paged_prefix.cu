@@ -65,8 +65,8 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r)
 
 // 2^x for a pair on the FMA and integer pipes: x = n + f with n the nearest integer (rounding by a large constant), |f| <= 1/2, a
 // polynomial of degree 4 for 2^f (minimax of the relative error, 2.6e-6; a weight is rounded to bf16 anyway), n added to the
-// exponent.  x <= 100; below -126 the result is 2^-126 instead of 0.  One pair of four takes it: none 79.3 us, one 77.2, two 85.2
-// (768 rows on 32768 tokens, 6 kv heads).
+// exponent.  x <= 100; below -126 the result is 2^-126 instead of 0, and so it is for NaN, which the caller keeps in the row's maximum.
+// One pair of four takes it: none 79.3 us, one 77.2, two 85.2 (768 rows on 32768 tokens, 6 kv heads).
 __device__ __forceinline__ void exp2_pair(uint64_t x, float& p0, float& p1) {
   float x0, x1;
   unpack2(x, x0, x1);
@@ -318,7 +318,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         ok = wait(&s_full[x], at & 1, 69);
         if (!ok) break;
         tc_fence_after();
-        // The scores of chunk c relative to the reference, and the row's running maximum of them.
+        // The scores of chunk c relative to the reference, and the row's running maximum of them, NaN where one of them is.
         auto scaled = [&](auto tail_tile, const uint32_t* w, int c, uint64_t neg2, uint64_t* y, float* mx) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -330,7 +330,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               if (c * 32 + 2 * e + 1 >= left) b = -INFINITY;
               y[e] = pack2(a, b);
             }
-            mx[e & 3] = max3(mx[e & 3], a, b);
+            mx[e & 3] = max3_nan(mx[e & 3], a, b);
           }
         };
         constexpr int kChunks = kTileKeys / 32;
@@ -346,7 +346,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               if (c + 1 < kChunks) tmem_ld_32x32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
               scaled(tail_tile, v[c & 1], c, 0ull, y, mx);
             }
-            m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            m = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
           }
           // A second pass where the reference was too low; a third is for scores so large that their own rounding exceeds 8.
           for (int pass = 0;; ++pass) {
@@ -362,7 +362,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               if (c + 1 < kChunks) tmem_ld_32x32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
               scaled(tail_tile, v[c & 1], c, neg2, y, mx);
               if (c == kChunks - 1) {
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
                 const bool low = top > 8.f || (m == -INFINITY && top > -INFINITY);
                 redo = pass < 2 && __any_sync(0xffffffffu, low);
                 if (redo) {
@@ -383,6 +383,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                   m = m_new;
                   break;
                 }
+                if (top != top) l = top;  // a score of NaN makes the row NaN; its weight may not (exp2_pair)
                 // the scores are in registers: the next product may overwrite them
                 tc_fence_before();
                 __syncwarp();
