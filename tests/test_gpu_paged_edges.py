@@ -35,3 +35,35 @@ def test_one_key_that_is_no_number(B, H, Hkv, hd, value):
         rows = torch.zeros(B, H, dtype=torch.bool)
         rows[:, :gqa] = ~up
         check_attention(o[rows], lse[rows], tuple(t[rows] for t in want), hd)
+
+
+@pytest.mark.usefixtures("prefix_room")
+@pytest.mark.parametrize("B,H,Hkv,hd", [(4, 6, 2, 64), (30, 6, 2, 64), (90, 6, 2, 64), (30, 8, 2, 128), (4, 4, 2, 32)])
+@pytest.mark.parametrize("scale", [1e7, 1e8, 1e10, 1e13])
+def test_scores_beyond_their_own_rounding(B, H, Hkv, hd, scale):
+    """Finite scores of 1e8 to 1e15 differ by more than the rounding of any of them, so each row is its best key's value - which
+    lies in several places, so that several tiles hold it."""
+    c = cache_case([40] * B, H, Hkv, hd, 16, prefix_lens=[700], seed=B)
+    for b in range(B):  # own keys that are the prefix's: the maximum again, in another part and another tile
+        c["ks"][b], c["vs"][b] = c["ks"][B][300:340], c["vs"][B][300:340]
+    c["ks"][B][600:640], c["vs"][B][600:640] = c["ks"][B][300:340], c["vs"][B][300:340]
+    for pool, lists in ((c["k_pages"], c["ks"]), (c["v_pages"], c["vs"])):
+        fill(pool, c["page_table"], [40] * B, lists[:B])
+        fill(pool, c["prefix_table"], [700], lists[B:])
+    o, lse = (t.double().cpu() for t in run_attention(c, scale=scale))
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+    gqa, sure = H // Hkv, 0
+    for b in range(B):
+        for h in range(H):
+            k, q = c["ks"][B][:, h // gqa].double(), c["q"][b, h].double()
+            s, v = k @ q * scale, c["vs"][B][:, h // gqa].double()
+            off = (hd + 8) * 2.0**-24 * float((k.abs() @ q.abs()).max()) * scale  # of a score, natural units
+            best = int(s.argmax())
+            top, second = float(s[best]), float(s[(k != k[best]).any(-1)].max())
+            # the score's error, two roundings of the result (2^-23 in all, half a step each), log(740) for keys alike, a cut at 8 log(2)
+            assert abs(float(lse[b, h]) - top) <= off + 2.0**-23 * abs(top) + 13
+            if top - second > 2 * off + 100:
+                # one rounding of the weight to bf16 next to its fp32 sum, one of the result: 2^-8 each
+                sure += 1
+                assert ((o[b, h] - v[best]).abs() <= 2.0**-7 * v[best].abs() + 2.0**-40).all()
+    assert sure > B * H // 2
