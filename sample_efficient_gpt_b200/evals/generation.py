@@ -23,6 +23,7 @@ evals/chat_web.py:89-110).
 
 from __future__ import annotations
 
+import warnings
 from contextlib import nullcontext
 from dataclasses import dataclass, field
 from pathlib import Path
@@ -704,6 +705,14 @@ class ChatEngine:
 
     MAX_PAGED_ROWS = 256
 
+    def _kernel_status(self) -> int:
+        """The package's status word of this engine's device, which is cleared by reading."""
+        if self.device.type != "cuda":
+            return 0
+        from sample_efficient_gpt_b200.ops import gemm
+
+        return gemm.take_status(self.device.index)
+
     @torch.inference_mode()
     def _decode_paged(self, prompts: list[list[int]], p: SamplingParams, gen=None) -> list[list[list[int]]]:
         """Prompts of any lengths, ``p.n`` rows each -> new token ids per prompt and row (stop token excluded)."""
@@ -719,6 +728,8 @@ class ChatEngine:
         out = torch.full((R, budget), -1, dtype=torch.long, device=self.device)
         done = torch.zeros(R, dtype=torch.bool, device=self.device)
         process = LogitsProcessor(p, rows, budget, self.model.vocab_size, self.device)
+        if (code := self._kernel_status()) != 0:  # not this generation's, which is judged by what it does itself
+            warnings.warn(f"a kernel had reported status {code} before this generation", RuntimeWarning, stacklevel=2)
         logits, steps = self.paged.start([prompts[i] for i in live], p.n, [room[i] for i in live]), 0
         for t in range(budget):
             if t > 0:
@@ -735,12 +746,8 @@ class ChatEngine:
             if (t + 1) % self.sync_every == 0 and bool(done.all()):
                 break
         tokens = out[:, :steps].cpu().tolist()
-        if self.device.type == "cuda":
-            from sample_efficient_gpt_b200.ops import gemm
-
-            code = gemm.status(self.device.index)
-            if code != 0:
-                raise RuntimeError(f"a kernel reported status {code} during generation")
+        if (code := self._kernel_status()) != 0:
+            raise RuntimeError(f"a kernel reported status {code} during generation")
         for j, i in enumerate(live):
             for k in range(p.n):
                 row = tokens[j * p.n + k]

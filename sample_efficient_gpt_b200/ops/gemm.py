@@ -77,3 +77,13 @@ def status(device_index: int | None = None) -> int:
     if device_index is None:
         device_index = torch.cuda.current_device()
     return int(ops.ext().gemm_status(device_index))
+
+
+def take_status(device_index: int | None = None) -> int:
+    """``status``, and the word is cleared: the next reader sees only what happened after this call."""
+    if device_index is None:
+        device_index = torch.cuda.current_device()
+    code = status(device_index)
+    if code != 0:
+        ops.ext().gemm_reset_status(device_index)
+    return code

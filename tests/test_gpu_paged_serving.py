@@ -1,0 +1,48 @@
+"""The paged decoder and the chat engine on the GPU around failures: status words, captures, what earlier calls leave behind."""
+
+import warnings
+
+import pytest
+import torch
+
+from sample_efficient_gpt_b200 import ops
+from sample_efficient_gpt_b200.evals.generation import ChatEngine, PagedDecoder, SamplingParams
+from sample_efficient_gpt_b200.ops import gemm
+
+from tests.test_gpu_paged_generation import gpu_model
+from tests.test_paged_generation import PROMPTS, Tok
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _clean_status():
+    assert ops.ext() is not None and gemm.status() == 0
+    yield
+    assert gemm.take_status() == 0
+
+
+def test_a_status_is_reported_once(monkeypatch):
+    eng = ChatEngine(gpu_model(), Tok(), "cuda", max_model_len=64, paged=True)
+    run = lambda: eng.generate_ids([list(x) for x in PROMPTS], SamplingParams(max_tokens=8, temperature=0.0))  # noqa: E731
+    want = run()
+    # a report that is not the generation's own
+    ops.process_logits(torch.zeros(1, 64, device="cuda"), mask=torch.zeros(1, 2, dtype=torch.int32, device="cuda"),
+                       mask_rows=torch.ones(1, dtype=torch.int32, device="cuda"))
+    with pytest.warns(RuntimeWarning, match="status 57 before"):
+        assert run() == want
+    # a generation that fails: page numbers beyond the pool, which the kernels leave out
+    tables = PagedDecoder._tables
+
+    def beyond(self, *args):
+        table = tables(self, *args)
+        table.fill_(10**7)
+        return table
+
+    monkeypatch.setattr(PagedDecoder, "_tables", beyond)
+    with pytest.raises(RuntimeError, match="status 5[24] during"):
+        run()
+    monkeypatch.undo()
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        assert run() == want and run() == want
