@@ -281,10 +281,13 @@ class PagedDecoder:
 
     ``start(prompts, n, budget)`` prefills the prompts (any lengths, each once) and gives the first logits of ``len(prompts) * n``
     rows; ``step(tokens)`` feeds one token per row.  With ``n`` > 1 a prompt's pages are a prefix that its rows share, and each row has
-    pages of its own for ``budget`` tokens; with one row per prompt both lie in the row's pages.  Buffers (and the graph) are kept
-    between calls and replaced when a call needs more rows or pages.  On a GPU bf16; on the CPU the statements of each op, fp32."""
+    pages of its own for ``budget`` tokens; with one row per prompt both lie in the row's pages.  The pools are kept between calls
+    and replaced when a call needs more pages; tables and graph are kept for the last few shapes of a call (rows, prompts and the
+    tables' widths), so that a call's kernels, and with them its results, do not depend on what was asked for before.  On a GPU bf16; on
+    the CPU the statements of each op, fp32."""
 
     PREFILL_TOKENS = 32768  # tokens that one prefill pass takes at most (a longer prompt goes by itself)
+    KEPT_SHAPES = 4  # each with a graph, whose activations and logits take up to about 0.2 GB at 256 rows
 
     def __init__(self, model, device, engine=None, page_size: int = 64):
         from sample_efficient_gpt_b200.training.engine import FusedEngine
@@ -301,8 +304,17 @@ class PagedDecoder:
         self.pages, self.shape = 0, None
         self.graph: torch.cuda.CUDAGraph | None = None
         self.logits: Tensor | None = None
+        self._kept: dict[tuple, dict] = {}  # buffers of the shapes before the present one, the latest last
 
     # ---- buffers
+    _BUFFERS = ("token", "lens", "pos_base", "table", "prefix_table", "prefix_lens", "group_rows", "graph", "logits")
+
+    @staticmethod
+    def _width(pages: int) -> int:
+        """A table's width for so many pages: the next 2^k or 3 * 2^k, so that neighbouring lengths share a graph."""
+        power = 1 << max(0, pages - 1).bit_length()
+        return 3 * power // 4 if power >= 4 and pages <= 3 * power // 4 else power
+
     def _reserve(self, pages: int, rows: int, width: int, groups: int, prefix_width: int):
         i32 = lambda *n: torch.zeros(*n, dtype=torch.int32, device=self.device)  # noqa: E731
         if pages > self.pages:
@@ -310,19 +322,26 @@ class PagedDecoder:
             # by head, so that a page's tokens of one head lie next to each other
             mk = lambda: torch.zeros(pages, self.Hkv, self.P, self.hd, dtype=self.lp, device=self.device).transpose(1, 2)  # noqa: E731
             self.graph = None
+            self._kept.clear()  # their graphs read the old pools
             self.kp = self.vp = None  # before the new pools take their place
             self.pages = 0  # should they not fit
             self.kp, self.vp = [mk() for _ in self.model.blocks], [mk() for _ in self.model.blocks]
             self.pages = pages
-        old = self.shape
-        if old is None or old[0] != rows or old[2] != groups or width > old[1] or prefix_width > old[3]:
-            if old is not None:
-                width, prefix_width = max(width, old[1]), max(prefix_width, old[3])
-            self.graph = None
-            self.shape = (rows, width, groups, prefix_width)
-            self.token, self.lens, self.pos_base, self.table = torch.zeros(rows, dtype=torch.long, device=self.device), i32(rows), i32(rows), i32(rows, width)
-            self.prefix_table = i32(groups, max(1, prefix_width)) if groups else None
-            self.prefix_lens, self.group_rows = (i32(groups), i32(groups + 1)) if groups else (None, None)
+        shape = (rows, self._width(width), groups, self._width(prefix_width))
+        if shape == self.shape:
+            return
+        if self.shape is not None:
+            self._kept[self.shape] = {name: getattr(self, name) for name in self._BUFFERS}
+        buffers = self._kept.pop(shape, None)
+        if buffers is None:
+            while len(self._kept) >= self.KEPT_SHAPES:
+                del self._kept[next(iter(self._kept))]
+            buffers = dict(token=torch.zeros(rows, dtype=torch.long, device=self.device), lens=i32(rows), pos_base=i32(rows), table=i32(rows, shape[1]),
+                           prefix_table=i32(groups, shape[3]) if groups else None, prefix_lens=i32(groups) if groups else None,
+                           group_rows=i32(groups + 1) if groups else None, graph=None, logits=None)
+        for name, value in buffers.items():
+            setattr(self, name, value)
+        self.shape = shape
 
     def _tables(self, prompts: list[list[int]], n: int, budget: list[int]):
         """Hands out pages and fills the tables; returns the table that the prompts are written through."""

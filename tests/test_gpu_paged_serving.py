@@ -46,3 +46,29 @@ def test_a_status_is_reported_once(monkeypatch):
     with warnings.catch_warnings():
         warnings.simplefilter("error")
         assert run() == want and run() == want
+
+
+def test_results_do_not_depend_on_what_was_served_before():
+    """100 rows on one prompt: behind a prompt of 16000 tokens the same short one keeps its kernels, its graph and its bits."""
+    dec = PagedDecoder(gpu_model(max_seq_len=20000), "cuda")
+    tokens = torch.arange(100, device="cuda")
+
+    def served(prompt):
+        out = [dec.start([prompt], 100, 40).clone()]
+        for _ in range(3):
+            out.append(dec.step(tokens).clone())
+        return out
+
+    short, long = [3, 4, 5, 6, 7] * 20, [i % 500 for i in range(16000)]
+    want = served(short)
+    graph, width = dec.graph, dec.prefix_table.size(1)
+    first = served(long)
+    again = served(short)
+    assert all(torch.equal(a, b) for a, b in zip(want, again))
+    assert dec.prefix_table.size(1) == width
+    assert all(torch.equal(a, b) for a, b in zip(first, served(long)))  # and the other way round
+    served(short)
+    kept = dec.graph
+    served(long)
+    served(short)
+    assert graph is not None and dec.graph is kept  # captured once for both shapes in turn

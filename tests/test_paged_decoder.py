@@ -1,0 +1,34 @@
+"""The paged decoder on the CPU (fp32 statements of each op): what earlier calls leave behind, rows at their limits."""
+
+import pytest
+import torch
+
+from sample_efficient_gpt_b200.evals.generation import PagedDecoder
+
+from tests.test_paged_generation import PROMPTS, model
+
+
+@pytest.mark.parametrize("n", [1, 3])
+def test_buffers_do_not_depend_on_earlier_calls(n):
+    """The kernels are chosen by the tables' widths: a short batch after a long one is laid out as it would be by itself."""
+    m = model()
+    dec, fresh = PagedDecoder(m, "cpu", page_size=4), PagedDecoder(m, "cpu", page_size=4)
+    short, long = [[3, 4, 5], [6, 7]], [[1 + i % 50 for i in range(300)], [2] * 200]
+    want = fresh.start(short, n, 5)
+    dec.start(long, n, 9)
+    assert torch.equal(dec.start(short, n, 5), want)
+    for name in ("table", "prefix_table", "lens", "token"):
+        a, b = getattr(dec, name), getattr(fresh, name)
+        assert (a is None) == (b is None) and (a is None or (a.shape == b.shape and torch.equal(a, b)))
+    # many shapes in turn: only the last few are kept, and each gives its own results again
+    firsts = [dec.start([p], n, 4) for p in PROMPTS]
+    for b in range(2, 9):
+        dec.start([[5] * (7 * b)] * b, n, 4)
+    assert len(dec._kept) <= dec.KEPT_SHAPES
+    for p, want in zip(PROMPTS, firsts):
+        assert torch.equal(dec.start([p], n, 4), want)
+
+
+def test_width_of_a_table():
+    got = [PagedDecoder._width(n) for n in range(1, 34)]
+    assert got == [1, 2, 3, 4, 6, 6, 8, 8] + [12] * 4 + [16] * 4 + [24] * 8 + [32] * 8 + [48]
