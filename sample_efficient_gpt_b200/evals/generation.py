@@ -484,9 +484,10 @@ class PagedDecoder:
                         for _ in range(2):
                             self._step()
                     torch.cuda.current_stream().wait_stream(side)
-                    self.graph = torch.cuda.CUDAGraph()
-                    with torch.cuda.graph(self.graph):
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph):
                         self.logits = self._step()
+                    self.graph = graph  # only a capture that came to its end is replayed
                 self.graph.replay()
         self.lens.add_(1 if active is None else active.to(torch.int32))
         return self.logits

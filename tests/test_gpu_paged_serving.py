@@ -72,3 +72,26 @@ def test_results_do_not_depend_on_what_was_served_before():
     served(long)
     served(short)
     assert graph is not None and dec.graph is kept  # captured once for both shapes in turn
+
+
+def test_a_capture_that_fails_is_made_again(monkeypatch):
+    dec = PagedDecoder(gpu_model(), "cuda", page_size=16)
+    tokens = torch.tensor([5, 6], device="cuda")
+    dec.start(PROMPTS[:2], 1, 8)
+    want = dec.step(tokens).clone()
+    dec = PagedDecoder(gpu_model(), "cuda", page_size=16)
+    dec.start(PROMPTS[:2], 1, 8)
+    block, calls = PagedDecoder._block, []
+
+    def fails(self, i, *args):
+        calls.append(i)
+        if len(calls) == 2 * self.model.n_layers + 2:  # both warm-up steps pass, the captured one ends in its second block
+            raise MemoryError("no room")
+        return block(self, i, *args)
+
+    monkeypatch.setattr(PagedDecoder, "_block", fails)
+    with pytest.raises(MemoryError):
+        dec.step(tokens)
+    monkeypatch.undo()
+    assert torch.equal(dec.step(tokens), want)
+    assert torch.equal(dec.step(tokens), dec.logits) and dec.graph is not None
