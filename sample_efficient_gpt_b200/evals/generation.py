@@ -307,7 +307,7 @@ class PagedDecoder:
         self._kept: dict[tuple, dict] = {}  # buffers of the shapes before the present one, the latest last
 
     # ---- buffers
-    _BUFFERS = ("token", "lens", "pos_base", "table", "prefix_table", "prefix_lens", "group_rows", "graph", "logits")
+    _BUFFERS = ("token", "lens", "place", "last", "pos_base", "table", "prefix_table", "prefix_lens", "group_rows", "graph", "logits")
 
     @staticmethod
     def _width(pages: int) -> int:
@@ -336,8 +336,8 @@ class PagedDecoder:
         if buffers is None:
             while len(self._kept) >= self.KEPT_SHAPES:
                 del self._kept[next(iter(self._kept))]
-            buffers = dict(token=torch.zeros(rows, dtype=torch.long, device=self.device), lens=i32(rows), pos_base=i32(rows), table=i32(rows, shape[1]),
-                           prefix_table=i32(groups, shape[3]) if groups else None, prefix_lens=i32(groups) if groups else None,
+            buffers = dict(token=torch.zeros(rows, dtype=torch.long, device=self.device), lens=i32(rows), place=i32(rows), last=i32(rows), pos_base=i32(rows),
+                           table=i32(rows, shape[1]), prefix_table=i32(groups, shape[3]) if groups else None, prefix_lens=i32(groups) if groups else None,
                            group_rows=i32(groups + 1) if groups else None, graph=None, logits=None)
         for name, value in buffers.items():
             setattr(self, name, value)
@@ -369,9 +369,11 @@ class PagedDecoder:
             self.group_rows.copy_(i32([g * n for g in range(groups + 1)]))
             self.lens.zero_()
             self.pos_base.copy_(i32([t for t in lens for _ in range(n)]))
+            self.last.copy_(i32([b - 1 for b in budget for _ in range(n)]))
             return self.prefix_table
         self.lens.copy_(i32(lens))
         self.pos_base.zero_()
+        self.last.copy_(i32([t + b - 1 for t, b in zip(lens, budget)]))
         return self.table
 
     # ---- model
@@ -437,10 +439,10 @@ class PagedDecoder:
     def _step(self) -> Tensor:
         from sample_efficient_gpt_b200 import ops
 
-        lens = self.lens + 1  # with the token of this step
+        lens = self.place + 1  # with the token of this step
 
         def attend(i, qkv, v1, qgain):
-            q, _, v = self._append(i, qkv, v1, qgain, self.table, self.lens, None, self.pos_base, False, v1 is None)
+            q, _, v = self._append(i, qkv, v1, qgain, self.table, self.place, None, self.pos_base, False, v1 is None)
             o, _ = ops.paged_attention(q, self.kp[i], self.vp[i], self.table, lens, self.prefix_table, self.prefix_lens, self.group_rows)
             return o, v if v1 is None else v1
 
@@ -471,8 +473,14 @@ class PagedDecoder:
 
     @torch.inference_mode()
     def step(self, tokens: Tensor, active: Tensor | None = None) -> Tensor:
-        """Feed one token per row; logits [R, V] (a static buffer).  Rows that are not ``active`` stay where they are."""
+        """Feed one token per row; logits [R, V] (a static buffer).  Rows that are not ``active`` stay where they are: their tokens go to
+        the place behind their last one, or, where they have taken their whole budget, to the last."""
         self.token.copy_(tokens.view(-1))
+        if active is None:
+            self.place.copy_(self.lens)
+        else:
+            torch.minimum(self.lens, self.last, out=self.place)
+            torch.where(active, self.lens, self.place, out=self.place)
         if self.device.type != "cuda":
             self.logits = self._step()
         else:

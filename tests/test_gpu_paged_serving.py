@@ -95,3 +95,24 @@ def test_a_capture_that_fails_is_made_again(monkeypatch):
     monkeypatch.undo()
     assert torch.equal(dec.step(tokens), want)
     assert torch.equal(dec.step(tokens), dec.logits) and dec.graph is not None
+
+
+@pytest.mark.parametrize("n", [1, 2])
+def test_a_row_that_has_taken_its_budget_is_left_alone(n):
+    """Nothing is reported for it, and the rows beside it get what they get by themselves."""
+    m = gpu_model(max_seq_len=48)
+    both, alone = PagedDecoder(m, "cuda", page_size=16), PagedDecoder(m, "cuda", page_size=16)
+    prompts, budget = [list(range(32)), [7, 8, 9]], [16, 45]  # up to the rotation table's end, one of them in full pages
+    both.start(prompts, n, budget)
+    alone.start(prompts, n, budget)
+    limit = torch.tensor([b for b in budget for _ in range(n)], device="cuda")
+    for t in range(45):
+        nxt = torch.arange(2 * n, device="cuda") + t
+        a = both.step(nxt, limit > t)
+        if t < 16:
+            alone.step(nxt)
+        else:  # the same rows with the first ones put back to where they were
+            with torch.inference_mode():
+                alone.lens[:n] -= 1
+            assert torch.equal(a[n:], alone.step(nxt)[n:])
+    assert gemm.status() == 0

@@ -32,3 +32,23 @@ def test_buffers_do_not_depend_on_earlier_calls(n):
 def test_width_of_a_table():
     got = [PagedDecoder._width(n) for n in range(1, 34)]
     assert got == [1, 2, 3, 4, 6, 6, 8, 8] + [12] * 4 + [16] * 4 + [24] * 8 + [32] * 8 + [48]
+
+
+@pytest.mark.parametrize("n", [1, 2])
+def test_a_row_that_has_taken_its_budget_beside_others(n):
+    """It must not be active any more; the others go on, up to the last position of the rotation table."""
+    m = model(max_seq_len=12)
+    dec = PagedDecoder(m, "cpu", page_size=4)
+    prompts, budget = [[3, 4, 5, 6], [7, 8]], [8, 6]  # 12 and 8 positions; full pages where a prompt has one row
+    rows = [list(x) for x in prompts for _ in range(n)]
+    limit = torch.tensor([b for b in budget for _ in range(n)])
+    dec.start(prompts, n, budget)
+    for t in range(10):
+        nxt = torch.arange(len(rows)) + t
+        active = limit > t
+        logits = dec.step(nxt, active)
+        for r, ids in enumerate(rows):
+            if bool(active[r]):
+                ids.append(int(nxt[r]))
+                assert torch.allclose(logits[r], m(torch.tensor([ids]))[0][0, -1], atol=2e-4, rtol=1e-4)
+    assert [len(x) for x in rows] == [12] * n + [8] * n
