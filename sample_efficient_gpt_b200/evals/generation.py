@@ -723,9 +723,12 @@ class ChatEngine:
                     done = done | complete
                 step_in, steps = nxt[:, None], t + 1
                 if on_token is not None:
-                    if bool(done[0]):
+                    token = int(out[0, t])
+                    if token == -1:
                         break
-                    on_token(int(nxt[0]))
+                    on_token(token)
+                    if complete is not None and bool(complete[0]):
+                        break
                 elif (t + 1) % self.sync_every == 0 and bool(done.all()):
                     break
         rows = out[:, :steps].cpu().tolist()

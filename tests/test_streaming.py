@@ -1,0 +1,40 @@
+"""Streaming from the chat engine on the CPU."""
+
+import pytest
+import torch
+
+from sample_efficient_gpt_b200.evals.generation import ChatEngine, SamplingParams
+
+from tests.test_paged_generation import Tok, model
+
+
+class ChatTok(Tok):
+    def encode(self, text, add_special_tokens=False):
+        return [ord(c) % 61 for c in text]
+
+
+TALK = [{"role": "user", "content": "hello"}]
+
+
+def engine(paged=False, **kw):
+    return ChatEngine(model(), ChatTok(), "cpu", max_model_len=64, paged=paged, **kw)
+
+
+def streamed(eng, **kw):
+    return "".join(eng.stream(TALK, SamplingParams(**{**dict(max_tokens=8, temperature=0.0), **kw})))
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(choices=[[10, 11, 12], [10, 13], [14]]), dict(choices=[[20]]), dict(allowed_token_ids=[7, 20], temperature=1.0),
+                                dict(frequency_penalty=1e6), dict(max_tokens=1)])
+def test_a_stream_is_the_whole_answer(kw):
+    eng = engine()
+    torch.manual_seed(3)
+    want = eng.chat([TALK], SamplingParams(**{**dict(max_tokens=8, temperature=0.0), **kw}))[0][0]
+    torch.manual_seed(3)
+    assert streamed(eng, **kw) == want
+
+
+def test_a_stream_ends_at_a_stop_token():
+    eng = engine()
+    answer = [int(t) for t in streamed(eng).split()]
+    assert [int(t) for t in streamed(eng, stop_token_ids=[answer[3]]).split()] == answer[: answer.index(answer[3])]
