@@ -826,13 +826,17 @@ class ChatEngine:
         def run():
             try:
                 self._decode_batch(prompt, p, None, on_token=q.put)
-            finally:
+            except BaseException as e:  # raised where the answer is read
+                q.put(e)
+            else:
                 q.put(None)
 
         threading.Thread(target=run, daemon=True).start()
         ids: list[int] = []
         shown = ""
         while (tok := q.get()) is not None:
+            if isinstance(tok, BaseException):
+                raise tok
             ids.append(tok)
             text = self.tokenizer.decode(ids, skip_special_tokens=True)
             if text.endswith("�"):

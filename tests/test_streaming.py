@@ -38,3 +38,26 @@ def test_a_stream_ends_at_a_stop_token():
     eng = engine()
     answer = [int(t) for t in streamed(eng).split()]
     assert [int(t) for t in streamed(eng, stop_token_ids=[answer[3]]).split()] == answer[: answer.index(answer[3])]
+
+
+def test_a_refusal_reaches_the_reader(monkeypatch):
+    eng = engine()
+    with pytest.raises(ValueError, match="at least one token"):
+        streamed(eng, allowed_token_ids=[])
+    with pytest.raises(ValueError, match="finite"):
+        streamed(eng, frequency_penalty=float("nan"))
+    forward, calls = eng.model.forward, []
+
+    def fails(*args, **kw):
+        calls.append(1)
+        if len(calls) == 3:
+            raise RuntimeError("no more")
+        return forward(*args, **kw)
+
+    monkeypatch.setattr(eng.model, "forward", fails)
+    pieces = []
+    with pytest.raises(RuntimeError, match="no more"):
+        for piece in eng.stream(TALK, SamplingParams(max_tokens=8, temperature=0.0)):
+            pieces.append(piece)
+    monkeypatch.undo()
+    assert len(pieces) == 2 and streamed(eng).startswith("".join(pieces))
