@@ -23,6 +23,7 @@ evals/chat_web.py:89-110).
 
 from __future__ import annotations
 
+import threading
 import warnings
 from contextlib import nullcontext
 from dataclasses import dataclass, field
@@ -658,6 +659,7 @@ class ChatEngine:
         if paged and self.device.type == "cuda" and (dtype or torch.bfloat16) != torch.bfloat16:
             raise ValueError("paged decode runs in bfloat16 on a GPU")
         self.paged = PagedDecoder(self.model, self.device) if paged else None
+        self._paged_turn = threading.Lock()
 
     # ---- prompt rendering -------------------------------------------------------------------------------------------
     def render(self, messages: list[dict]) -> list[int]:
@@ -744,9 +746,14 @@ class ChatEngine:
 
         return gemm.take_status(self.device.index)
 
-    @torch.inference_mode()
     def _decode_paged(self, prompts: list[list[int]], p: SamplingParams, gen=None) -> list[list[list[int]]]:
-        """Prompts of any lengths, ``p.n`` rows each -> new token ids per prompt and row (stop token excluded)."""
+        """Prompts of any lengths, ``p.n`` rows each -> new token ids per prompt and row (stop token excluded).  Calls from several threads
+        take turns: they share the decoder's tables."""
+        with self._paged_turn:
+            return self._decode_paged_now(prompts, p, gen)
+
+    @torch.inference_mode()
+    def _decode_paged_now(self, prompts: list[list[int]], p: SamplingParams, gen) -> list[list[list[int]]]:
         room = [min(p.max_tokens, self.max_model_len - len(x)) for x in prompts]
         live = [i for i, r in enumerate(room) if r > 0]
         results: list[list[list[int]]] = [[[] for _ in range(p.n)] for _ in prompts]
@@ -818,7 +825,6 @@ class ChatEngine:
         """Generator of text pieces for one conversation (decodes the growing id list so multi-byte characters that span
         tokens come out whole)."""
         import queue
-        import threading
 
         q: queue.Queue = queue.Queue()
         prompt = torch.tensor([self.render(messages)[-(self.max_model_len - 1):]], dtype=torch.long, device=self.device)

@@ -1,11 +1,13 @@
 """The paged decoder on the CPU (fp32 statements of each op): what earlier calls leave behind, rows at their limits."""
 
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
-from sample_efficient_gpt_b200.evals.generation import PagedDecoder
+from sample_efficient_gpt_b200.evals.generation import ChatEngine, PagedDecoder, SamplingParams
 
-from tests.test_paged_generation import PROMPTS, model
+from tests.test_paged_generation import PROMPTS, Tok, model
 
 
 @pytest.mark.parametrize("n", [1, 3])
@@ -52,3 +54,14 @@ def test_a_row_that_has_taken_its_budget_beside_others(n):
                 ids.append(int(nxt[r]))
                 assert torch.allclose(logits[r], m(torch.tensor([ids]))[0][0, -1], atol=2e-4, rtol=1e-4)
     assert [len(x) for x in rows] == [12] * n + [8] * n
+
+
+def test_two_calls_at_once():
+    """Two threads on one engine: each gets what it gets by itself."""
+    eng = ChatEngine(model(), Tok(), "cpu", max_model_len=40, paged=True)
+    p = SamplingParams(max_tokens=12, temperature=0.0)
+    asked = [[list(x)] for x in PROMPTS[:3]] + [[list(x) for x in PROMPTS[1:3]]]
+    want = [eng.generate_ids([list(x) for x in a], p) for a in asked]
+    with ThreadPoolExecutor(len(asked)) as pool:
+        for _ in range(3):
+            assert list(pool.map(lambda a: eng.generate_ids([list(x) for x in a], p), asked)) == want
