@@ -26,7 +26,7 @@ from __future__ import annotations
 import threading
 import warnings
 from contextlib import nullcontext
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from pathlib import Path
 
 import torch
@@ -728,8 +728,7 @@ class ChatEngine:
                     token = int(out[0, t])
                     if token == -1:
                         break
-                    on_token(token)
-                    if complete is not None and bool(complete[0]):
+                    if on_token(token) or (complete is not None and bool(complete[0])):
                         break
                 elif (t + 1) % self.sync_every == 0 and bool(done.all()):
                     break
@@ -746,14 +745,14 @@ class ChatEngine:
 
         return gemm.take_status(self.device.index)
 
-    def _decode_paged(self, prompts: list[list[int]], p: SamplingParams, gen=None) -> list[list[list[int]]]:
-        """Prompts of any lengths, ``p.n`` rows each -> new token ids per prompt and row (stop token excluded).  Calls from several threads
-        take turns: they share the decoder's tables."""
+    def _decode_paged(self, prompts: list[list[int]], p: SamplingParams, gen=None, on_token=None) -> list[list[list[int]]]:
+        """Prompts of any lengths, ``p.n`` rows each -> new token ids per prompt and row (stop token excluded).  Calls from several threads,
+        an unfinished stream's among them, take turns: they share the decoder's tables."""
         with self._paged_turn:
-            return self._decode_paged_now(prompts, p, gen)
+            return self._decode_paged_now(prompts, p, gen, on_token)
 
     @torch.inference_mode()
-    def _decode_paged_now(self, prompts: list[list[int]], p: SamplingParams, gen) -> list[list[list[int]]]:
+    def _decode_paged_now(self, prompts: list[list[int]], p: SamplingParams, gen, on_token) -> list[list[list[int]]]:
         room = [min(p.max_tokens, self.max_model_len - len(x)) for x in prompts]
         live = [i for i, r in enumerate(room) if r > 0]
         results: list[list[list[int]]] = [[[] for _ in range(p.n)] for _ in prompts]
@@ -781,7 +780,11 @@ class ChatEngine:
             if complete is not None:
                 done = done | complete
             steps = t + 1
-            if (t + 1) % self.sync_every == 0 and bool(done.all()):
+            if on_token is not None:  # one row
+                token = int(out[0, t])
+                if token == -1 or on_token(token) or (complete is not None and bool(complete[0])):
+                    break
+            elif (t + 1) % self.sync_every == 0 and bool(done.all()):
                 break
         tokens = out[:, :steps].cpu().tolist()
         if (code := self._kernel_status()) != 0:
@@ -823,15 +826,23 @@ class ChatEngine:
 
     def stream(self, messages: list[dict], p: SamplingParams):
         """Generator of text pieces for one conversation (decodes the growing id list so multi-byte characters that span
-        tokens come out whole)."""
+        tokens come out whole).  Decoding ends with the answer or when the generator is closed."""
         import queue
 
         q: queue.Queue = queue.Queue()
-        prompt = torch.tensor([self.render(messages)[-(self.max_model_len - 1):]], dtype=torch.long, device=self.device)
+        prompt = self.render(messages)[-(self.max_model_len - 1):]
+        closed = threading.Event()
+
+        def on_token(token: int) -> bool:
+            q.put(token)
+            return closed.is_set()
 
         def run():
             try:
-                self._decode_batch(prompt, p, None, on_token=q.put)
+                if self.paged is not None:
+                    self._decode_paged([prompt], replace(p, n=1), None, on_token)
+                else:
+                    self._decode_batch(torch.tensor([prompt], dtype=torch.long, device=self.device), p, None, on_token)
             except BaseException as e:  # raised where the answer is read
                 q.put(e)
             else:
@@ -840,16 +851,19 @@ class ChatEngine:
         threading.Thread(target=run, daemon=True).start()
         ids: list[int] = []
         shown = ""
-        while (tok := q.get()) is not None:
-            if isinstance(tok, BaseException):
-                raise tok
-            ids.append(tok)
-            text = self.tokenizer.decode(ids, skip_special_tokens=True)
-            if text.endswith("�"):
-                continue
-            if len(text) > len(shown):
-                yield text[len(shown):]
-                shown = text
+        try:
+            while (tok := q.get()) is not None:
+                if isinstance(tok, BaseException):
+                    raise tok
+                ids.append(tok)
+                text = self.tokenizer.decode(ids, skip_special_tokens=True)
+                if text.endswith("�"):
+                    continue
+                if len(text) > len(shown):
+                    yield text[len(shown):]
+                    shown = text
+        finally:
+            closed.set()
 
 
 def load_chat_template(tokenizer_dir) -> str | None:

@@ -11,6 +11,7 @@ from sample_efficient_gpt_b200.ops import gemm
 
 from tests.test_gpu_paged_generation import gpu_model
 from tests.test_paged_generation import PROMPTS, Tok
+from tests.test_streaming import TALK, ChatTok
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +117,18 @@ def test_a_row_that_has_taken_its_budget_is_left_alone(n):
                 alone.lens[:n] -= 1
             assert torch.equal(a[n:], alone.step(nxt)[n:])
     assert gemm.status() == 0
+
+
+def test_streams_of_a_paged_engine():
+    """Captured on the stream's own thread; the same tokens as the whole answer, again and beside other calls."""
+    eng = ChatEngine(gpu_model(), ChatTok(), "cuda", max_model_len=96, paged=True)
+    p = SamplingParams(max_tokens=24, temperature=0.0)
+    parts = "".join(eng.stream(TALK, p))
+    assert parts == eng.chat([TALK], p)[0][0] == "".join(eng.stream(TALK, p)) and len(parts.split()) == 24
+    stream = eng.stream(TALK, p)
+    head = next(stream)
+    other = eng.generate_ids([list(PROMPTS[2])], SamplingParams(n=3, max_tokens=12, temperature=0.0))  # waits for its turn
+    assert head + "".join(stream) == parts and other[0][0] == other[0][2]
+    choice = "".join(eng.stream(TALK, SamplingParams(max_tokens=24, temperature=0.0, choices=[[10, 11, 12], [20]])))
+    assert choice in ("10 11 12", "20")
+    assert not eng._decoders  # no static caches beside the pages

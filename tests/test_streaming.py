@@ -1,5 +1,7 @@
 """Streaming from the chat engine on the CPU."""
 
+import threading
+
 import pytest
 import torch
 
@@ -61,3 +63,35 @@ def test_a_refusal_reaches_the_reader(monkeypatch):
             pieces.append(piece)
     monkeypatch.undo()
     assert len(pieces) == 2 and streamed(eng).startswith("".join(pieces))
+
+
+def test_a_paged_engine_streams_over_its_pages(monkeypatch):
+    plain, eng = engine(), engine(paged=True)
+    monkeypatch.setattr(eng, "_decode_batch", None)  # the static caches are not used
+    for kw in (dict(), dict(n=3), dict(max_tokens=100), dict(choices=[[10, 11, 12], [10, 13], [14]]), dict(max_tokens=0)):
+        assert streamed(eng, **kw) == streamed(plain, **kw)
+    answer = [int(t) for t in streamed(eng).split()]
+    assert [int(t) for t in streamed(eng, stop_token_ids=[answer[3]]).split()] == answer[: answer.index(answer[3])]
+    with pytest.raises(ValueError, match="at least one token"):
+        streamed(eng, allowed_token_ids=[])
+
+
+def test_a_stream_that_is_closed_stops_decoding(monkeypatch):
+    eng = engine(paged=True)
+    seen, taken = eng.paged.step, threading.Event()
+    steps = []
+
+    def step(*args):
+        taken.wait(10)  # the reader has its first piece and closes before the second step
+        steps.append(1)
+        return seen(*args)
+
+    monkeypatch.setattr(eng.paged, "step", step)
+    stream = eng.stream(TALK, SamplingParams(max_tokens=40, temperature=0.0))
+    next(stream)
+    stream.close()
+    taken.set()
+    with eng._paged_turn:  # free again once the thread has stopped
+        assert len(steps) <= 1
+    monkeypatch.undo()
+    assert streamed(eng) == streamed(engine())
