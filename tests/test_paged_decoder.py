@@ -5,7 +5,7 @@ from concurrent.futures import ThreadPoolExecutor
 import pytest
 import torch
 
-from sample_efficient_gpt_b200.evals.generation import ChatEngine, PagedDecoder, SamplingParams
+from sample_efficient_gpt_b200.evals.generation import ChatEngine, LogitsProcessor, PagedDecoder, SamplingParams
 
 from tests.test_paged_generation import PROMPTS, Tok, model
 
@@ -65,3 +65,15 @@ def test_two_calls_at_once():
     with ThreadPoolExecutor(len(asked)) as pool:
         for _ in range(3):
             assert list(pool.map(lambda a: eng.generate_ids([list(x) for x in a], p), asked)) == want
+
+
+def test_parameters_that_32_bits_cannot_hold_are_refused():
+    mk = lambda **kw: LogitsProcessor(SamplingParams(**kw), [[1], [2]], 4, 61, "cpu")  # noqa: E731
+    for kw in (dict(repetition_penalty=1e39), dict(presence_penalty=-1e39), dict(frequency_penalty=1e39), dict(logit_bias={1: 1e39}), dict(logit_bias={1: -1e40})):
+        with pytest.raises(ValueError, match="finite"):
+            mk(**kw)
+    with pytest.raises(ValueError, match="positive"):
+        mk(repetition_penalty=1e-50)
+    x = torch.randn(2, 61)
+    y = mk(repetition_penalty=1e30, frequency_penalty=-3e38, logit_bias={1: 3e38, 2: -3e38})(x)
+    assert not torch.isnan(y).any()
