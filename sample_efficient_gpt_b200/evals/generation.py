@@ -459,6 +459,9 @@ class PagedDecoder:
         budget = [budget] * len(prompts) if isinstance(budget, int) else list(budget)
         if not prompts or not all(prompts) or n < 1 or len(budget) != len(prompts) or min(budget) < 1:
             raise ValueError("start() needs prompts of at least one token, n >= 1 and budget >= 1")
+        vocab = self.model.embedding.weight.size(0)
+        if any(min(x) < 0 or max(x) >= vocab for x in prompts):  # on the device a failing index would end the process
+            raise ValueError(f"a prompt's tokens lie in [0, {vocab})")
         longest = max(len(x) + b for x, b in zip(prompts, budget))
         if longest > self.model.blocks[0].attn.rope.cos.size(0):
             raise ValueError(f"{longest} positions do not fit the model's rotation table")

@@ -77,3 +77,12 @@ def test_parameters_that_32_bits_cannot_hold_are_refused():
     x = torch.randn(2, 61)
     y = mk(repetition_penalty=1e30, frequency_penalty=-3e38, logit_bias={1: 3e38, 2: -3e38})(x)
     assert not torch.isnan(y).any()
+
+
+@pytest.mark.parametrize("token", [-1, 61, 10**9])
+def test_prompts_of_tokens_that_do_not_exist_are_refused(token):
+    dec = PagedDecoder(model(), "cpu")
+    want = dec.start(PROMPTS, 2, 5)
+    with pytest.raises(ValueError, match="tokens lie in"):
+        dec.start([[3, 4], [5, token, 6]], 2, 5)
+    assert torch.equal(dec.start(PROMPTS, 2, 5), want)
