@@ -535,10 +535,12 @@ class LogitsProcessor:
         full = lambda v: torch.full((R,), float(v), device=device)  # noqa: E731
         self.args: dict = {}
         if p.penalised:
-            # as the kernel takes them, in fp32: 1e-50 is no positive factor there, 1e39 is not finite
-            if not self._in_fp32(p.repetition_penalty) > 0.0 or not all(
-                    abs(self._in_fp32(v)) < float("inf") for v in (p.repetition_penalty, p.presence_penalty, p.frequency_penalty)):
-                raise ValueError("repetition_penalty must be positive, and all penalties finite (in 32 bits)")
+            # 1e30 times a count of 2^29 and a logit of 1e8 stay finite in fp32.  A row whose allowed tokens all overflow to -inf could not be
+            # sampled: on the device that is a failing assertion.
+            if not 1e-30 <= p.repetition_penalty <= 1e30:
+                raise ValueError("repetition_penalty must be positive, finite and within 1e-30 .. 1e30")
+            if not all(abs(v) <= 1e29 for v in (p.presence_penalty, p.frequency_penalty)):
+                raise ValueError("presence and frequency penalties must be finite, 1e29 at most")
             lens = [len(x) for x in rows]
             history = torch.full((R, max(lens) + budget), -1, dtype=torch.int32)
             for r, x in enumerate(rows):
@@ -546,8 +548,8 @@ class LogitsProcessor:
             self.args.update(tokens=history.to(device), prompt_lens=i32(lens), token_lens=i32(lens), repetition=full(p.repetition_penalty),
                              presence=full(p.presence_penalty), frequency=full(p.frequency_penalty))
         if p.logit_bias:
-            if any(not 0 <= t < vocab or not abs(self._in_fp32(v)) < float("inf") for t, v in p.logit_bias.items()):
-                raise ValueError(f"logit_bias takes finite values (in 32 bits) for tokens in [0, {vocab})")
+            if any(not 0 <= t < vocab or not abs(v) <= 1e38 for t, v in p.logit_bias.items()):
+                raise ValueError(f"logit_bias takes finite values, 1e38 at most, for tokens in [0, {vocab})")
             self.args.update(bias_ids=i32(list(p.logit_bias)).expand(R, -1).contiguous(),
                              bias_values=torch.tensor(list(p.logit_bias.values()), dtype=torch.float32, device=device).expand(R, -1).contiguous())
         self.state: Tensor | None = None
@@ -568,10 +570,6 @@ class LogitsProcessor:
                 self.children = torch.tensor([list(node) + [-1] * (wide - len(node)) for node in nodes] + [[-1] * wide], device=device)
                 self.next = torch.tensor([list(node.values()) + [0] * (wide - len(node)) for node in nodes] + [[len(nodes)] * wide], device=device)
                 self.end, self.state = len(nodes), torch.zeros(R, dtype=torch.long, device=device)
-
-    @staticmethod
-    def _in_fp32(v: float) -> float:
-        return float(torch.tensor(v, dtype=torch.float32))
 
     @staticmethod
     def _trie(choices: list[list[int]]) -> list[dict[int, int]]:

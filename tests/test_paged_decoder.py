@@ -74,9 +74,23 @@ def test_parameters_that_32_bits_cannot_hold_are_refused():
             mk(**kw)
     with pytest.raises(ValueError, match="positive"):
         mk(repetition_penalty=1e-50)
-    x = torch.randn(2, 61)
-    y = mk(repetition_penalty=1e30, frequency_penalty=-3e38, logit_bias={1: 3e38, 2: -3e38})(x)
-    assert not torch.isnan(y).any()
+
+
+def test_allowed_tokens_stay_finite():
+    """Whatever the parameters, an allowed token can be sampled: 2^29 occurrences is the most that a history counts."""
+    for kw in (dict(frequency_penalty=1e38), dict(frequency_penalty=-3e38), dict(presence_penalty=2e38), dict(repetition_penalty=3e38), dict(repetition_penalty=1e-38),
+               dict(logit_bias={5: -3e38})):
+        with pytest.raises(ValueError):
+            LogitsProcessor(SamplingParams(allowed_token_ids=[5], **kw), [[5] * 40], 4, 61, "cpu")
+    largest = dict(frequency_penalty=1e29, presence_penalty=1e29, logit_bias={5: -1e38})
+    for kw in (dict(repetition_penalty=1e30, **largest), dict(repetition_penalty=1e-30, **largest)):
+        proc = LogitsProcessor(SamplingParams(allowed_token_ids=[5], **kw), [[5] * 40], 4, 61, "cpu")
+        for x in (torch.full((1, 61), -1e8), torch.full((1, 61), 1e8)):
+            for _ in range(4):
+                proc.push(torch.tensor([5]))
+            y = proc(x)
+            assert torch.isfinite(y[0, 5]) and int(torch.isfinite(y).sum()) == 1
+    assert 1e29 * 2.0**29 + 1e29 + 1e38 + 1e38 < torch.finfo(torch.float32).max
 
 
 @pytest.mark.parametrize("token", [-1, 61, 10**9])
