@@ -596,7 +596,9 @@ class LogitsProcessor:
     def __call__(self, logits: Tensor) -> Tensor:
         from sample_efficient_gpt_b200 import ops
 
-        return ops.process_logits(logits, **self.args) if self.args else logits
+        if not self.args:
+            return logits
+        return ops.process_logits(logits.float() if logits.dtype == torch.float16 else logits, **self.args)
 
     def push(self, tokens: Tensor) -> Tensor | None:
         """Take the sampled tokens [R] into account; rows whose choice is complete (or None)."""

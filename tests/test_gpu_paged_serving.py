@@ -132,3 +132,12 @@ def test_streams_of_a_paged_engine():
     choice = "".join(eng.stream(TALK, SamplingParams(max_tokens=24, temperature=0.0, choices=[[10, 11, 12], [20]])))
     assert choice in ("10 11 12", "20")
     assert not eng._decoders  # no static caches beside the pages
+
+
+def test_constraints_of_an_engine_in_half_precision():
+    """Its logits are fp16, which the kernel does not take."""
+    eng = ChatEngine(gpu_model(), Tok(), "cuda", max_model_len=64, dtype=torch.float16)
+    run = lambda **kw: eng.generate_ids([[3, 4, 5], [3, 4, 5, 6]], SamplingParams(**{**dict(max_tokens=8, temperature=0.0), **kw}))  # noqa: E731
+    assert {t for r in run(allowed_token_ids=[7, 200, 511], temperature=1.0, seed=0) for t in r[0]} <= {7, 200, 511}
+    assert all(set(r[0]) == {33} for r in run(logit_bias={33: 1e9}))  # beyond fp16
+    assert all(len(set(r[0])) == 8 for r in run(frequency_penalty=1e6))
