@@ -111,6 +111,11 @@ struct Lists {  // cumulative units per item of the sequences, and units per kv 
   int n_groups;
 };
 
+// Rows of the prefix items before the one that starts at row h0 of a group's `all` rows of head kvh (small form).
+__device__ __forceinline__ int64_t prefix_row(const PagedAttnParams& p, int r0, int all, int kvh, int h0) {
+  return (int64_t)r0 * p.H + (int64_t)kvh * all + h0;
+}
+
 template <int HD>
 __device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + Cfg<HD>::kKeys - 1) / Cfg<HD>::kKeys + kItemCost : 0; }
 
@@ -420,7 +425,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     while (t < share && ok) {
       const int units = min(share - t, c.units - c.unit);
       const int step0 = max(0, c.unit - kItemCost), steps = max(0, c.unit + units - kItemCost) - step0;
-      if (c.unit == 0 && lane == 0) ws.meta[c.item] = item_parts(c.own ? c.item : c.item - n.items_s, t0 + t, c.units, workers, total);
+      if (c.unit == 0 && lane == 0) ws.meta[c.item] = item_parts(c.own ? c.item : 0, t0 + t, c.units, workers, total);
       float o[HD / 8][4] = {};
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
       uint32_t qf[HD / 16][4];
@@ -457,7 +462,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       }
       // ---- the row's result, or the part of it
       const bool whole = c.own && p.G == 0 && units == c.units;
-      const int64_t part = ((c.own ? c.item : c.item - n.items_s) + worker) * (c.own ? n.rows_s : kRows);
+      const int64_t part = c.own ? (c.item + worker) * n.rows_s : prefix_row(p, c.row0, all, c.kvh, c.h0) + worker * kRows;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = (lane >> 2) + 8 * h, x = c.h0 + r, col = (lane & 3) * 2;
@@ -525,22 +530,24 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 8) paged_attn_join_kernel(con
     gr = load_group(p, g);
   }
   const int len = clamp_len(p.lens[b], p.table_width, p.pool.P, p.status);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (p.groups != nullptr && ws.meta[n.items_s + n.items_p].x != 0) gr.len = 0;  // borders out of order: no prefixes
-  const bool shared = gr.len > 0 && b >= gr.r0 && b < gr.r1;
+  bool shared = gr.len > 0 && b >= gr.r0 && b < gr.r1;
   const int x = shared ? (b - gr.r0) * n.gqa + hl : 0, row_p = x % n.rows_p;
+  const int item_p = shared ? first_item(n, p, g, gr.r0) + kvh * row_tiles(gr, n) + x / n.rows_p : 0;
+  const int64_t pre_row = row_p + (n.form == kPrefixSmall ? prefix_row(p, gr.r0, (gr.r1 - gr.r0) * n.gqa, kvh, x - row_p) : 0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.groups != nullptr && ws.meta[n.items_s + n.items_p].x != 0) shared = false;  // borders out of order: no prefixes
   int2 pre = make_int2(0, 0), own = make_int2(0, 0);
-  if (shared) pre = ws.meta[first_item(n, p, g, gr.r0) + kvh * row_tiles(gr, n) + x / n.rows_p];
+  if (shared) pre = ws.meta[item_p];
   if (len > 0) own = ws.meta[(b * p.Hkv + kvh) * n.RT + hl / kRows];
   if (p.G == 0 && own.y == 1) return;  // written by the worker that held the whole item (the same for all warps of the row)
   // a wait that gave up leaves items without their entries
-  if (pre.x < 0 || pre.y < 0 || (int64_t)pre.x + pre.y > (int64_t)n.items_p + n.ctas_p) pre = make_int2(0, 0);
+  if (pre.x < 0 || pre.y < 0 || (int64_t)pre.x + pre.y > (n.form == kPrefixSmall ? 0 : (int64_t)n.items_p) + n.ctas_p) pre = make_int2(0, 0);
   if (own.x < 0 || own.y < 0 || (int64_t)own.x + own.y > (int64_t)n.items_s + n.workers) own = make_int2(0, 0);
   pre.x *= n.parts_p;
   pre.y *= n.parts_p;
   const int total = pre.y + own.y;
   const auto place = [&](int i) {
-    return i < pre.y ? (int64_t)(pre.x + i) * n.part_rows_p + row_p : (int64_t)(own.x + i - pre.y) * n.rows_s + hl % kRows;
+    return i < pre.y ? (int64_t)(pre.x + i) * n.part_rows_p + pre_row : (int64_t)(own.x + i - pre.y) * n.rows_s + hl % kRows;
   };
   float m = -INFINITY, l = 0.f, acc[kPer] = {};
   const int first = kSplit == 1 ? 0 : total * warp / kSplit, last = kSplit == 1 ? total : total * (warp + 1) / kSplit;
@@ -654,6 +661,12 @@ Plan make_plan(const PagedAttnParams& p) {
 }
 
 int64_t round_up(int64_t n) { return (n + 255) / 256 * 256; }
+int64_t own_part_rows(const Plan& n) { return ((int64_t)n.items_s + n.workers) * n.rows_s; }
+int64_t prefix_part_rows(const PagedAttnParams& p, const Plan& n) {
+  if (p.G == 0) return 0;
+  if (n.form == kPrefixSmall) return (int64_t)p.B * p.H + (int64_t)n.workers * kRows;
+  return ((int64_t)n.items_p + n.ctas_p) * n.parts_p * n.part_rows_p;
+}
 
 template <int HD, bool kTma>
 int launch(const PagedAttnParams& p, const Plan& n, const Work& ws, cudaStream_t st) {
@@ -704,7 +717,7 @@ int64_t paged_attn_workspace(const PagedAttnParams& p) {
   if (p.hd != 32 && p.hd != 64 && p.hd != 128) return -1;
   if (p.B + p.G > kMaxLists) return -1;
   const Plan n = make_plan(p);
-  const int64_t ss = ((int64_t)n.items_s + n.workers) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas_p) * n.parts_p * n.part_rows_p : 0;
+  const int64_t ss = own_part_rows(n), sp = prefix_part_rows(p, n);
   return round_up(ss * p.hd * 4) + round_up(ss * 8) + round_up(sp * p.hd * 4) + round_up(sp * 8) + round_up(((int64_t)n.items_s + n.items_p + 1) * 8);
 }
 
@@ -712,7 +725,7 @@ int paged_attn(const PagedAttnParams& p, void* workspace, cudaStream_t st) {
   if (p.B == 0) return 0;
   if (p.H < 1 || p.Hkv < 1 || p.H % p.Hkv != 0 || p.H > 65535 || p.B + p.G > kMaxLists) return -10;
   const Plan n = make_plan(p);
-  const int64_t ss = ((int64_t)n.items_s + n.workers) * n.rows_s, sp = p.G > 0 ? ((int64_t)n.items_p + n.ctas_p) * n.parts_p * n.part_rows_p : 0;
+  const int64_t ss = own_part_rows(n), sp = prefix_part_rows(p, n);
   uint8_t* at = static_cast<uint8_t*>(workspace);
   Work ws;
   ws.acc_s = reinterpret_cast<float*>(at);

@@ -43,14 +43,15 @@ struct Plan {            // sizes that host and device derive alike
 };
 
 // Every (item, worker) pair with work gets the part number item + worker: both only grow along the row of tiles, so the numbers are
-// distinct, and consecutive for the parts of one item.
+// distinct, and consecutive for the parts of one item.  The small form's prefix items have 1 to 16 rows; there the part of worker w
+// starts at row `rows of the items before + 16 w`, distinct for the same reason, so that many small groups take no more than their rows.
 struct Work {
   float* acc_s;    // [items_s + workers, rows_s, HD]
   float2* ml_s;    // [items_s + workers, rows_s]
-  float* acc_p;    // [(items_p + ctas_p) * parts_p, part_rows_p, HD]
+  float* acc_p;    // [(items_p + ctas_p) * parts_p, part_rows_p, HD]; small form: [B H + 16 workers, HD]
   float2* ml_p;
-  int2* meta;      // [items_s + items_p + 1] first part and number of parts of every item that has tiles; x of the last: group_rows
-                   // are out of order (written where there are any)
+  int2* meta;      // [items_s + items_p + 1] first part (small form's prefix items: first worker) and number of parts of every item that
+                   // has tiles; x of the last: group_rows are out of order (written where there are any)
 };
 
 __device__ __forceinline__ float exp2_(float x) {

@@ -5,8 +5,10 @@ import math
 import pytest
 import torch
 
+from sample_efficient_gpt_b200 import ops
+
 from tests.paged_cases import attention_oracle, cache_case, check_attention, fill
-from tests.test_gpu_paged import _clean_status, prefix_room, run_attention  # noqa: F401  (fixtures)
+from tests.test_gpu_paged import DEV, _clean_status, i32, prefix_room, run_attention, to_dev  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +69,34 @@ def test_scores_beyond_their_own_rounding(B, H, Hkv, hd, scale):
                 sure += 1
                 assert ((o[b, h] - v[best]).abs() <= 2.0**-7 * v[best].abs() + 2.0**-40).all()
     assert sure > B * H // 2
+
+
+@pytest.mark.parametrize("H,Hkv,hd,groups", [(32, 32, 128, 3000), (64, 16, 64, 4000), (34, 2, 64, 700)])
+def test_scratch_of_many_small_groups(H, Hkv, hd, groups):
+    """Parts take the rows that there are, however the groups divide them: 17 query heads a kv head, one, or four."""
+    sizes = [1] * groups
+    sizes[groups // 2], sizes[groups // 3] = 0, 5
+    rows = [0]
+    for n in sizes:
+        rows.append(rows[-1] + n)
+    B = rows[-1]
+    plens = [(7 * g) % 40 for g in range(groups)]
+    c = cache_case([b % 3 for b in range(B)], H, Hkv, hd, 16, "token", plens, seed=groups)
+    d = to_dev(c)
+    args = d["q"], d["k_pages"], d["v_pages"], d["page_table"], d["seq_lens"], d["prefix_table"], d["prefix_lens"], i32(rows)
+    o, lse = ops.paged_attention(*args)
+    torch.cuda.synchronize()
+    del o, lse
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    o, lse = ops.paged_attention(*args)
+    used = torch.cuda.max_memory_allocated() - before
+    # (m, l, fp32 row) of every row for its prefix and for its own tokens (16 rows for every 17), and of 16 rows a warp for each; results
+    room = 2.0 * (B * H * (32 / 17 if H == 34 else 1) + 148 * 16 * 16) * (hd * 4 + 8) + B * H * (hd * 2 + 4) + 64 * Hkv * B + (4 << 20)
+    assert used <= room, (used, room)
+    group = [g for g, n in enumerate(sizes) for _ in range(n)]
+    some = torch.tensor(sorted({0, 1, B // 3 - 2, B // 3, groups // 3, groups // 3 + 3, B // 2, B - 1}))
+    picked = [int(b) for b in some]
+    lists = [c["ks"][b] for b in picked] + c["ks"][B:], [c["vs"][b] for b in picked] + c["vs"][B:]
+    want = attention_oracle(c["q"][some], *lists, [group[b] for b in picked], len(picked))
+    check_attention(o[some.to(DEV)], lse[some.to(DEV)], want, hd)
