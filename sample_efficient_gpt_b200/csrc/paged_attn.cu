@@ -285,11 +285,12 @@ __device__ __forceinline__ void attend(const PagedAttnParams& p, int left, const
         }
       }
     }
-    // scaled before the mask and the maximum, for the scale may be zero or negative
+    // relative to the reference; scaled before the mask and the maximum, for the scale may be zero or negative
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int e = 0; e < kE; ++e) sc[n][e] = __fmul_rn(sc[n][e], p.scale_log2);  // not to be fused with the difference below
+      for (int e = 0; e < kE; ++e) sc[n][e] = fmaf(sc[n][e], p.scale_log2, -ref[e >> 1]);
     if (left < C::kKeys) {
 #pragma unroll
       for (int n = 0; n < kN; ++n)
@@ -308,16 +309,15 @@ __device__ __forceinline__ void attend(const PagedAttnParams& p, int left, const
     for (int n = 0; n < kN; ++n)
 #pragma unroll
       for (int e = 0; e < kE; e += 2) mx[e >> 1] = max3(mx[e >> 1], sc[n][e], sc[n][e + 1]);
-    // Relative to a reference that is the product of some score and the scale, rounded as these are: that score lies at exactly zero.
-    const auto is_low = [](float top, float m) { return m == -INFINITY ? top > -INFINITY : top - m > 8.f; };
-    const bool low = is_low(mx[0], m[0]) || (!kHalf && is_low(mx[1], m[1]));
+    bool low = mx[0] > 8.f || (m[0] == -INFINITY && mx[0] > -INFINITY);
+    if (!kHalf) low = low || mx[1] > 8.f || (m[1] == -INFINITY && mx[1] > -INFINITY);
     if (__any_sync(0xffffffffu, low)) {  // move the references to the maxima (always in an item's first step, rarely after it)
 #pragma unroll
       for (int h = 0; h < (kHalf ? 1 : 2); ++h) {
         float t = mx[h];
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-        const float m_new = fmaxf(m[h], t);
+        const float m_new = fmaxf(m[h], ref[h] + t);
         if (m_new == -INFINITY) continue;
         const float a = m[h] == -INFINITY ? 1.f : exp2_(m[h] - m_new);
         l[h] *= a;
@@ -326,10 +326,16 @@ __device__ __forceinline__ void attend(const PagedAttnParams& p, int left, const
           o[d][2 * h] *= a;
           o[d][2 * h + 1] *= a;
         }
+        // In this order no score ends above zero.  (One above 1e8 may have come here by its own rounding, 2^-24 of it, with the reference
+        // left where it was.)
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          sc[n][2 * h] = __fadd_rn(__fadd_rn(sc[n][2 * h], ref[h]), -m_new);
+          sc[n][2 * h + 1] = __fadd_rn(__fadd_rn(sc[n][2 * h + 1], ref[h]), -m_new);
+        }
         m[h] = m_new;
       }
     }
-    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
     uint32_t pf[kN / 2][4];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
@@ -339,7 +345,7 @@ __device__ __forceinline__ void attend(const PagedAttnParams& p, int left, const
           pf[n / 2][(n & 1) * 2 + 1] = 0u;
           continue;
         }
-        const float e0 = exp2_(sc[n][2 * h] - ref[h]), e1 = exp2_(sc[n][2 * h + 1] - ref[h]);
+        const float e0 = exp2_(sc[n][2 * h]), e1 = exp2_(sc[n][2 * h + 1]);
         l[h] += e0 + e1;
         pf[n / 2][(n & 1) * 2 + h] = pack_bf16(e0, e1);  // weights rounded to bf16 (at most 2^-8 relative), as operands of the tensor core
       }
