@@ -255,7 +255,6 @@ __device__ __forceinline__ void load_step(const PagedAttnParams& p, const CUtens
       copy16(stage + swz<HD>(r, c), w.k + page * p.pool.k_page + slot * p.pool.k_slot + c * 8, live);
       copy16(stage + C::kMat + swz<HD>(r, c), w.v + page * p.pool.v_page + slot * p.pool.v_slot + c * 8, live);
     }
-    copy_commit();
   }
 }
 
@@ -422,7 +421,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         ++ahead.unit;
         ++t_ahead;
       }
-      if (!kTma) copy_commit();
+      if (!kTma) copy_commit();  // one group a call, with or without a step: the waits count them
     };
     bool ok = true;
     int it = 0, items = 0;

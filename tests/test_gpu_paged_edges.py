@@ -7,7 +7,7 @@ import torch
 
 from sample_efficient_gpt_b200 import ops
 
-from tests.paged_cases import attention_oracle, cache_case, check_attention, fill
+from tests.paged_cases import attention_oracle, cache_case, check_attention, fill, make_pool, make_tables
 from tests.test_gpu_paged import DEV, _clean_status, i32, prefix_room, run_attention, to_dev  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
@@ -100,3 +100,31 @@ def test_scratch_of_many_small_groups(H, Hkv, hd, groups):
     lists = [c["ks"][b] for b in picked] + c["ks"][B:], [c["vs"][b] for b in picked] + c["vs"][B:]
     want = attention_oracle(c["q"][some], *lists, [group[b] for b in picked], len(picked))
     check_attention(o[some.to(DEV)], lse[some.to(DEV)], want, hd)
+
+
+@pytest.mark.parametrize("H,Hkv,hd", [(8, 8, 32), (40, 2, 32), (18, 6, 64), (32, 8, 128)])
+def test_pages_read_with_and_without_boxes_give_the_same_bits(H, Hkv, hd):
+    """Pages of 8 are read as boxes, pages of 4 and 6 with a copy a lane, four stages deep at 32 dims: the same steps over the same keys,
+    in items of one step, of many, and cut between warps, with a prefix and without."""
+    lens = [0, 1, 33, 700, 31, 64, 2, 0, 260, 5] * 12
+    c = cache_case(lens, H, Hkv, hd, 8, prefix_lens=[70, 0, 500], seed=hd)
+    rows, B = [0, 50, 60, 110], len(lens)
+    want = {pre: None for pre in (False, True)}
+    for P in (8, 4, 6):
+        a = {**cache_case([0] * B, H, Hkv, hd, P, prefix_lens=[0, 0, 0]), "q": c["q"], "seq_lens": c["seq_lens"], "prefix_lens": c["prefix_lens"]}
+        total = sum(-(-n // P) for n in lens + [70, 0, 500])
+        order = torch.randperm(total, generator=torch.Generator().manual_seed(P)).tolist()
+        # tables for as many tokens in every case: the plan goes by them
+        a["page_table"], used = make_tables(lens, P, order, 744 // P)
+        a["prefix_table"], _ = make_tables([70, 0, 500], P, order[used:], 504 // P)
+        a["k_pages"], a["v_pages"] = make_pool(total, P, Hkv, hd), make_pool(total, P, Hkv, hd)
+        for pool, lists in ((a["k_pages"], c["ks"]), (a["v_pages"], c["vs"])):
+            fill(pool, a["page_table"], lens, lists[:B])
+            fill(pool, a["prefix_table"], [70, 0, 500], lists[B:])
+        for pre in want:
+            got = run_attention(a, rows) if pre else run_attention({**a, "prefix_table": None, "prefix_lens": None})
+            if want[pre] is None:
+                want[pre] = got
+                group = [0] * 50 + [1] * 10 + [2] * 50 + [-1] * 10 if pre else None
+                check_attention(*got, attention_oracle(c["q"], c["ks"], c["vs"], group, B), hd)
+            assert torch.equal(got[0], want[pre][0]) and torch.equal(got[1], want[pre][1]), (P, pre)
