@@ -141,3 +141,41 @@ def test_constraints_of_an_engine_in_half_precision():
     assert {t for r in run(allowed_token_ids=[7, 200, 511], temperature=1.0, seed=0) for t in r[0]} <= {7, 200, 511}
     assert all(set(r[0]) == {33} for r in run(logit_bias={33: 1e9}))  # beyond fp16
     assert all(len(set(r[0])) == 8 for r in run(frequency_penalty=1e6))
+
+
+@pytest.mark.parametrize("kw", [dict(attn_qknorm=False), dict(attn_val_residual=False), dict(attn_qknorm=False, attn_gating=False, attn_val_residual=False),
+                                dict(n_heads=8, n_kv_heads=8), dict(n_heads=2, n_kv_heads=1), dict(weight_tying=False)])
+@pytest.mark.parametrize("n", [1, 3])
+def test_logits_of_other_models_track_the_module_path(kw, n):
+    """Without QK-norm, value residual or gate; heads of 32 and of 128: bf16 kernels against the fp32 module path, as the default model is
+    held to it."""
+    m = gpu_model(**kw)
+    dec = PagedDecoder(m, "cuda", page_size=16)
+    rows = [list(x) for x in PROMPTS for _ in range(n)]
+    logits = dec.start(PROMPTS, n, 24)
+    g = torch.Generator().manual_seed(0)
+    for _ in range(12):
+        with torch.no_grad():
+            want = torch.stack([m(torch.tensor([r], device="cuda"))[0][0, -1] for r in rows])
+        assert torch.allclose(logits.float(), want, atol=0.15, rtol=0.05), float((logits - want).abs().max())
+        nxt = torch.randint(0, 512, (len(rows),), generator=g)
+        for r, t in zip(rows, nxt.tolist()):
+            r.append(t)
+        logits = dec.step(nxt.cuda())
+
+
+def test_a_prefill_of_many_tokens_is_the_module_paths():
+    """Prompts long enough for the append kernel's ring in every layer, over page borders; then a few steps."""
+    m = gpu_model(max_seq_len=4096)
+    dec = PagedDecoder(m, "cuda", page_size=64)
+    prompts = [[(7 * i + b) % 512 for i in range(n)] for b, n in enumerate((3000, 1, 1501, 64))]
+    rows = [list(x) for x in prompts]
+    logits = dec.start(prompts, 1, 8)
+    for t in range(4):
+        with torch.no_grad():
+            want = torch.stack([m(torch.tensor([r], device="cuda"))[0][0, -1] for r in rows])
+        assert torch.allclose(logits.float(), want, atol=0.15, rtol=0.05), float((logits - want).abs().max())
+        nxt = torch.arange(4) + t
+        for r, x in zip(rows, nxt.tolist()):
+            r.append(x)
+        logits = dec.step(nxt.cuda())
