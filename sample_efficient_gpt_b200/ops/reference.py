@@ -185,6 +185,11 @@ def attention_bwd(do: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: T
 
 
 # ----------------------------------------------------------------------------- paged cache (serving)
+def _together(**args) -> None:
+    if len({x is None for x in args.values()}) > 1:
+        raise ValueError(" and ".join(args) + " come together")
+
+
 def _paged_rows(pages: Tensor, table_row: Tensor, n: int) -> Tensor:
     """The first n tokens that a row of a page table lists, [n, Hkv, hd]."""
     P = pages.size(1)
@@ -228,6 +233,11 @@ def qkv_post_paged(qkv, v1, cos, sin, qgain, a1, a2, vscale, H, Hkv, hd, qknorm,
 
 def paged_attention(q, k_pages, v_pages, page_table, seq_lens, prefix_table=None, prefix_lens=None, group_rows=None, scale=None):
     """One query token per sequence over its group's prefix and its own pages (see ``ops.paged_attention``)."""
+    _together(prefix_table=prefix_table, prefix_lens=prefix_lens)
+    if prefix_table is None and group_rows is not None:
+        raise ValueError("group_rows needs prefix_table and prefix_lens")
+    if prefix_table is not None and len(prefix_lens) != (1 if group_rows is None else len(group_rows) - 1):
+        raise ValueError(f"group_rows has an entry more than there are prefixes ({len(prefix_lens)}); without it there is one prefix for all rows")
     B, H, hd = q.shape
     Hkv = k_pages.size(2)
     scale = 1.0 / math.sqrt(hd) if scale is None else scale
@@ -261,6 +271,11 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, prefix_table=None
 def process_logits(logits, tokens=None, prompt_lens=None, token_lens=None, repetition=None, presence=None, frequency=None, bias_ids=None,
                    bias_values=None, mask=None, mask_rows=None, out=None):
     """Penalties, biases and the mask of allowed tokens (see ``ops.process_logits``)."""
+    _together(tokens=tokens, token_lens=token_lens)
+    _together(bias_ids=bias_ids, bias_values=bias_values)
+    _together(mask=mask, mask_rows=mask_rows)
+    if tokens is None and not all(x is None for x in (prompt_lens, repetition, presence, frequency)):
+        raise ValueError("penalties need tokens and token_lens")
     B, V = logits.shape
     x = logits.float().clone()
     if tokens is not None:
