@@ -479,6 +479,10 @@ class PagedDecoder:
     def step(self, tokens: Tensor, active: Tensor | None = None) -> Tensor:
         """Feed one token per row; logits [R, V] (a static buffer).  Rows that are not ``active`` stay where they are: their tokens go to
         the place behind their last one, or, where they have taken their whole budget, to the last."""
+        if self.shape is None:
+            raise ValueError("start() comes before step()")
+        if tokens.numel() != self.token.numel() or (active is not None and active.shape != self.token.shape):
+            raise ValueError(f"step() takes one token for each of {self.token.numel()} rows, and as many flags")
         self.token.copy_(tokens.view(-1))
         if active is None:
             self.place.copy_(self.lens)

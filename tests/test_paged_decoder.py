@@ -100,3 +100,15 @@ def test_prompts_of_tokens_that_do_not_exist_are_refused(token):
     with pytest.raises(ValueError, match="tokens lie in"):
         dec.start([[3, 4], [5, token, 6]], 2, 5)
     assert torch.equal(dec.start(PROMPTS, 2, 5), want)
+
+
+def test_steps_that_do_not_fit_the_rows_are_refused():
+    """One token for several rows would have been taken by all of them."""
+    dec = PagedDecoder(model(), "cpu")
+    with pytest.raises(ValueError, match="start"):
+        dec.step(torch.tensor([1]))
+    dec.start(PROMPTS, 1, 5)
+    for tokens, active in ((torch.tensor([1]), None), (torch.arange(5), None), (torch.arange(4), torch.tensor([True])), (torch.arange(4), torch.ones(4, 1, dtype=torch.bool))):
+        with pytest.raises(ValueError, match="4 rows"):
+            dec.step(tokens, active)
+    assert dec.step(torch.arange(4)[:, None], torch.ones(4, dtype=torch.bool)).shape == (4, 61)
