@@ -319,15 +319,22 @@ class PagedDecoder:
     def _reserve(self, pages: int, rows: int, width: int, groups: int, prefix_width: int):
         i32 = lambda *n: torch.zeros(*n, dtype=torch.int32, device=self.device)  # noqa: E731
         if pages > self.pages:
-            pages = max(pages, self.pages * 3 // 2)
             # by head, so that a page's tokens of one head lie next to each other
-            mk = lambda: torch.zeros(pages, self.Hkv, self.P, self.hd, dtype=self.lp, device=self.device).transpose(1, 2)  # noqa: E731
+            mk = lambda n: [torch.zeros(n, self.Hkv, self.P, self.hd, dtype=self.lp, device=self.device).transpose(1, 2) for _ in self.model.blocks]  # noqa: E731
             self.graph = None
             self._kept.clear()  # their graphs read the old pools
-            self.kp = self.vp = None  # before the new pools take their place
+            ample = max(pages, self.pages * 3 // 2)
             self.pages = 0  # should they not fit
-            self.kp, self.vp = [mk() for _ in self.model.blocks], [mk() for _ in self.model.blocks]
-            self.pages = pages
+            for n in (ample, pages):  # room for larger calls to come, where there is any
+                self.kp = self.vp = None  # before the new pools take their place
+                try:
+                    self.kp, self.vp = mk(n), mk(n)
+                except torch.OutOfMemoryError:
+                    if n == pages:
+                        raise
+                    continue
+                self.pages = n
+                break
         shape = (rows, self._width(width), groups, self._width(prefix_width))
         if shape == self.shape:
             return

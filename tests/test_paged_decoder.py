@@ -112,3 +112,25 @@ def test_steps_that_do_not_fit_the_rows_are_refused():
         with pytest.raises(ValueError, match="4 rows"):
             dec.step(tokens, active)
     assert dec.step(torch.arange(4)[:, None], torch.ones(4, dtype=torch.bool)).shape == (4, 61)
+
+
+def test_pools_that_grow_take_what_there_is(monkeypatch):
+    """Half as much again is room for later calls, not a need: a call that fits without it is served."""
+    dec = PagedDecoder(model(), "cpu", page_size=4)
+    dec.start([[3] * 40], 1, 40)  # 20 pages
+    make, asked = torch.zeros, []
+
+    def limited(*size, **kw):
+        if len(size) == 4:
+            asked.append(size[0])
+            if size[0] > 25:
+                raise torch.OutOfMemoryError("no room")
+        return make(*size, **kw)
+
+    monkeypatch.setattr(torch, "zeros", limited)
+    got = dec.start([[3] * 48], 1, 40)  # 22 pages
+    assert dec.pages == 22 and asked[0] == 30 and len(dec.kp) == len(dec.vp) == 3
+    with pytest.raises(torch.OutOfMemoryError):
+        dec.start([[3] * 80], 1, 40)
+    assert dec.pages == 0
+    assert torch.equal(dec.start([[3] * 48], 1, 40), got)
