@@ -189,7 +189,8 @@ std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor& k_page
     TORCH_CHECK(!groups.has_value(), "group_rows needs prefix_table and prefix_lens");
   }
   const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt((double)hd);
-  TORCH_CHECK(std::isfinite(sc), "scale must be finite");
+  const float scale_log2 = (float)(sc * 1.4426950408889634);
+  TORCH_CHECK(std::isfinite(scale_log2), "scale must be finite (in 32 bits), got ", sc);
   c10::cuda::CUDAGuard guard(dev);
   p.q = q.data_ptr();
   p.q_row = q.stride(0);
@@ -204,7 +205,7 @@ std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor& k_page
   p.plens = G > 0 ? plens->data_ptr<int>() : nullptr;
   p.groups = groups.has_value() ? groups->data_ptr<int>() : nullptr;
   p.B = (int)B; p.H = (int)H; p.Hkv = (int)Hkv; p.hd = (int)hd; p.G = (int)G;
-  p.scale_log2 = (float)(sc * 1.4426950408889634);
+  p.scale_log2 = scale_log2;
   p.status = status_word(dev);
   // positions and tile numbers are 32-bit inside the kernels
   const int64_t longest = std::max<int64_t>(p.table_width, p.ptable_width) * p.pool.P;

@@ -128,3 +128,12 @@ def test_pages_read_with_and_without_boxes_give_the_same_bits(H, Hkv, hd):
                 group = [0] * 50 + [1] * 10 + [2] * 50 + [-1] * 10 if pre else None
                 check_attention(*got, attention_oracle(c["q"], c["ks"], c["vs"], group, B), hd)
             assert torch.equal(got[0], want[pre][0]) and torch.equal(got[1], want[pre][1]), (P, pre)
+
+
+def test_a_scale_that_32_bits_cannot_hold_is_refused():
+    d = to_dev(cache_case([4, 7], 4, 2, 64, 16, seed=1))
+    for scale in (1e39, -3e38, math.inf, math.nan):
+        with pytest.raises(RuntimeError, match="finite"):
+            ops.paged_attention(d["q"], d["k_pages"], d["v_pages"], d["page_table"], d["seq_lens"], scale=scale)
+    o, _ = ops.paged_attention(d["q"], d["k_pages"], d["v_pages"], d["page_table"], d["seq_lens"], scale=1e30)
+    assert torch.isfinite(o).all()
