@@ -461,8 +461,9 @@ class PagedDecoder:
 
     @torch.inference_mode()
     def start(self, prompts: list[list[int]], n: int, budget: int | list[int]) -> Tensor:
-        """Logits [len(prompts) * n, V] after the prompts; the rows of a prompt lie next to each other.  ``budget``: tokens that
-        rows may take, one number or one for each prompt; a row that has taken them must not be active any more."""
+        """Logits [len(prompts) * n, V] after the prompts, with the model's weights as they are now; the rows of a prompt lie next to each
+        other.  ``budget``: tokens that rows may take, one number or one for each prompt; a row that has taken them must not be active
+        any more."""
         budget = [budget] * len(prompts) if isinstance(budget, int) else list(budget)
         if not prompts or not all(prompts) or n < 1 or len(budget) != len(prompts) or min(budget) < 1:
             raise ValueError("start() needs prompts of at least one token, n >= 1 and budget >= 1")
@@ -472,6 +473,7 @@ class PagedDecoder:
         longest = max(len(x) + b for x, b in zip(prompts, budget))
         if longest > self.model.blocks[0].attn.rope.cos.size(0):
             raise ValueError(f"{longest} positions do not fit the model's rotation table")
+        self.eng.refresh_shadows()  # gains and embeddings are read where they are, the matrices through copies
         table, out, a = self._tables(prompts, n, budget), [], 0
         while a < len(prompts):
             b, tokens = a + 1, len(prompts[a])

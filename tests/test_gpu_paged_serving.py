@@ -179,3 +179,19 @@ def test_a_prefill_of_many_tokens_is_the_module_paths():
         for r, x in zip(rows, nxt.tolist()):
             r.append(x)
         logits = dec.step(nxt.cuda())
+
+
+@pytest.mark.parametrize("cast", [False, True])
+def test_weights_that_change_between_calls(cast):
+    m = gpu_model()
+    eng = ChatEngine(m, Tok(), "cuda", max_model_len=64, paged=True, cast_weights=cast)
+    dec = eng.paged
+    dec.start(PROMPTS, 2, 5)
+    dec.step(torch.arange(8, device="cuda"))
+    with torch.no_grad():
+        for p in m.parameters():
+            p.mul_(0.75)
+    fresh = PagedDecoder(m, "cuda")
+    assert torch.equal(dec.start(PROMPTS, 2, 5), fresh.start(PROMPTS, 2, 5))
+    for _ in range(3):  # the step captured before
+        assert torch.equal(dec.step(torch.arange(8, device="cuda")), fresh.step(torch.arange(8, device="cuda")))

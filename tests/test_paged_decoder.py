@@ -134,3 +134,19 @@ def test_pools_that_grow_take_what_there_is(monkeypatch):
         dec.start([[3] * 80], 1, 40)
     assert dec.pages == 0
     assert torch.equal(dec.start([[3] * 48], 1, 40), got)
+
+
+def test_weights_that_change_between_calls():
+    """Each call runs with all of the model's weights as they are, not with some of an earlier time."""
+    m = model()
+    dec = PagedDecoder(m, "cpu", page_size=4)
+    dec.start(PROMPTS, 2, 5)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.mul_(1.25).add_(0.01)
+    fresh = PagedDecoder(m, "cpu", page_size=4)
+    assert torch.equal(dec.start(PROMPTS, 2, 5), fresh.start(PROMPTS, 2, 5))
+    for _ in range(3):
+        assert torch.equal(dec.step(torch.arange(8)), fresh.step(torch.arange(8)))
+    want = torch.stack([m(torch.tensor([x]))[0][0, -1] for x in PROMPTS]).repeat_interleave(2, 0)
+    assert torch.allclose(dec.start(PROMPTS, 2, 5), want, atol=2e-4, rtol=1e-4)
