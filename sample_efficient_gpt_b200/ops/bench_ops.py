@@ -317,6 +317,7 @@ def bench_decode(a):
     """Tokens per second of the one-token decode step of IMU-1 430M (random init, bf16), eager KV-cache decode against the
     CUDA-graph replay of the same step; the prompt is 128 tokens, 128 tokens are generated.  Then 32 samples of a prompt of 1500 tokens,
     over one static cache per row and over a paged cache whose prompt pages the samples share."""
+    import statistics
     import time
 
     from sample_efficient_gpt_b200.evals.generation import ChatEngine, SamplingParams
@@ -351,16 +352,16 @@ def bench_decode(a):
     row = {"op": "decode_samples", "samples": 32, "prompt": 1500, "new_tokens": 128}
     for name, paged in (("static", False), ("paged", True)):
         eng = ChatEngine(model, Tok(), "cuda", max_model_len=2048, cast_weights=True, paged=paged)
-        for new in (128, 1, 128):  # warm-up (and graph capture); prefill; prefill and 127 steps
+        took = {1: [], 128: []}  # prefill; prefill and 127 steps.  Medians: a single generation may meet anything on the host
+        for new in (128, 1, *[1, 128] * 7):
             p = SamplingParams(n=32, max_tokens=new, temperature=0.0)
             torch.cuda.synchronize()
             t0 = time.perf_counter()
             eng.generate_ids([[(j * 7) % 1000 + 10 for j in range(1500)]], p)
             torch.cuda.synchronize()
-            dt = time.perf_counter() - t0
-            if new == 1:
-                first = dt
-        row[f"{name}_first_token_ms"], row[f"{name}_ms_per_token"] = first * 1e3, (dt - first) / 127 * 1e3
+            took[new].append(time.perf_counter() - t0)
+        first, whole = (statistics.median(took[new][1:]) for new in (1, 128))  # without the warm-up (and the graph's capture)
+        row[f"{name}_first_token_ms"], row[f"{name}_ms_per_token"] = first * 1e3, (whole - first) / 127 * 1e3
         del eng
         torch.cuda.empty_cache()
     print(json.dumps(row))
