@@ -17,7 +17,7 @@
 // finds without reducing the maximum over lanes; weights are then at most 256, harmless for bf16 operands and fp32 sums.
 // Keys behind the length are masked by index and their values set to zero: what lies in those slots does not count.
 // Measured: 64 sequences of up to 8192 tokens, 6 kv heads of 64: 403 MB in 73 us, join included (5.5 TB/s); one sequence of 700
-// tokens 7.6 us, the latency of two launches and of length -> page -> keys -> parts.
+// tokens 7.8 us, the latency of two launches and of length -> page -> keys -> parts.
 #include <algorithm>
 
 #include "paged_common.cuh"
@@ -191,7 +191,7 @@ __device__ __forceinline__ void next_item(const PagedAttnParams& p, const Plan& 
   set_item(p, n, c, i, all);
 }
 
-// What a warp keeps of its ring: steps taken so far.
+// Where a warp's ring lies, and the queries beside it.
 struct Ring {
   uint32_t base;  // shared memory of the stages
   uint32_t full;  // mbarriers of the stages (TMA)
@@ -742,7 +742,7 @@ int paged_attn(const PagedAttnParams& p, void* workspace, cudaStream_t st) {
   ws.ml_p = reinterpret_cast<float2*>(at);
   at += round_up(sp * 8);
   ws.meta = reinterpret_cast<int2*>(at);
-  // Whole 8-row groups of the swizzle pattern.  64 ragged sequences of up to 8192 tokens: 73 us, with cp.async 112.
+  // Whole 8-row groups of the swizzle pattern.  64 ragged sequences of up to 8192 tokens: 73 us, with cp.async 109.
   const bool tma = pool_box(p.pool.P, 8) == 8;
   switch (p.hd) {
     case 32: return tma ? launch<32, true>(p, n, ws, st) : launch<32, false>(p, n, ws, st);

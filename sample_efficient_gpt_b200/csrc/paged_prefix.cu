@@ -21,7 +21,7 @@
 // memory.  Scores pass through the registers 32 columns at a time, the next load in flight; P goes back to tensor memory, from
 // where the second product reads it (through shared memory, each warp's fence between its stores and the tensor core's reads
 // cost 290 cycles a tile).  Registers and, at head_dim 64, shared memory leave room on the SM for CTAs of the kernel over own pages.
-// Measured: 256 sequences x 18 heads on 32768 tokens (6 kv heads of 64) 74 us with the join, of them about 20 before the first and
+// Measured: 256 sequences x 18 heads on 32768 tokens (6 kv heads of 64) 75 us with the join, of them about 20 before the first and
 // after the last tile; a 256 x 128 tile takes 2200 cycles, in which both halves do their softmax at the same time and then wait
 // for the products together (1075 cycles of the tensor core).  Four softmax warps a scheduler, 64-key tiles in two buffers and halves that take
 // turns were slower.

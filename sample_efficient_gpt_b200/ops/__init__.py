@@ -163,12 +163,14 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, prefix_table=None
     the prefix of its group: rows [group_rows[g], group_rows[g + 1]) share the first ``prefix_lens[g]`` tokens of
     ``prefix_table[g]`` ([G, Wp] int32), whose keys and values are read once for the group and not once per row.  ``group_rows``
     [G + 1] int32 ascends within [0, B] (groups may be empty, rows outside every group have no prefix); None: one group of
-    all rows.  ``scale`` defaults to 1 / sqrt(hd).  A row that sees no token gives o = 0, lse = -inf.  Slots behind a length and
-    table entries behind the last page needed are never read.
+    all rows.  ``scale`` defaults to 1 / sqrt(hd).  A row that sees no token, or only keys of score -inf, gives o = 0, lse = -inf; one
+    that sees a score of NaN or +inf is NaN.  What lies in slots behind a length does not count, table entries behind the last page
+    needed are not read.
 
     Lengths, pages and borders are read on the device only: a length beyond its table is cut to the table, a page outside the
     pool reads as zeros, and with borders out of order no row has a prefix; each sets the status word (``ops.gemm.status()``: 53, 54, 55).
-    CUDA: bf16, head_dim 32, 64 or 128, at most 8192 sequences and groups; capturable into a graph."""
+    CUDA: bf16, head_dim 32, 64 or 128, at most 8192 sequences and groups, (sequences + groups) x heads x (tokens that the wider table
+    holds / 32) below 2^31; capturable into a graph."""
     if _use_cuda(q, "paged_attention"):
         _count(2)
         return ext().paged_attention(q, k_pages, v_pages, page_table, seq_lens, prefix_table, prefix_lens, group_rows, scale)
