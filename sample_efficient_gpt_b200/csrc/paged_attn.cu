@@ -574,15 +574,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 8) paged_attn_join_kernel(con
         const float m_new = fmaxf(m, warp_max(ml.x)), old = part_weight(m, l, m_new);
         w = part_weight(ml.x, ml.y, m_new);
         l = l * old + warp_sum(w * ml.y);
+        if (ml.x == -INFINITY && ml.y == 0.f) w = -0.f;  // may not have been written
 #pragma unroll
         for (int c = 0; c < kPer; ++c) acc[c] *= old;
         m = m_new;
       }
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) {
-        const float wj = j0 + k < count ? __shfl_sync(0xffffffffu, w, j0 + k) : 0.f;
+        // left out by the sign, not by being zero: a weight that underflowed still meets what is no number among its part's values
+        const float wj = j0 + k < count ? __shfl_sync(0xffffffffu, w, j0 + k) : -0.f;
 #pragma unroll
-        for (int c = 0; c < kPer; ++c) acc[c] += wj != 0.f ? wj * part[k][c] : 0.f;  // a part without weight may not have been written
+        for (int c = 0; c < kPer; ++c) acc[c] += __float_as_uint(wj) != 0x80000000u ? wj * part[k][c] : 0.f;
       }
     }
   }

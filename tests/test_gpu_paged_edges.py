@@ -137,3 +137,23 @@ def test_a_scale_that_32_bits_cannot_hold_is_refused():
             ops.paged_attention(d["q"], d["k_pages"], d["v_pages"], d["page_table"], d["seq_lens"], scale=scale)
     o, _ = ops.paged_attention(d["q"], d["k_pages"], d["v_pages"], d["page_table"], d["seq_lens"], scale=1e30)
     assert torch.isfinite(o).all()
+
+
+@pytest.mark.usefixtures("prefix_room")
+@pytest.mark.parametrize("B,H,Hkv,hd", [(4, 6, 2, 64), (30, 6, 2, 64), (90, 6, 2, 64), (30, 8, 2, 128)])
+@pytest.mark.parametrize("scale", [None, 200.0])
+def test_one_value_that_is_no_number(B, H, Hkv, hd, scale):
+    """A NaN among the values makes its component NaN in all rows of its kv head, also where the key's weight has underflowed beside
+    another part's (scores of thousands), and leaves the others as they are."""
+    c = cache_case([5] * B, H, Hkv, hd, 16, prefix_lens=[300], seed=B)
+    gqa = H // Hkv
+    clean, lse0 = (t.cpu() for t in run_attention(c, scale=scale))
+    for at in (0, 6, 7, 100, 255, 299):
+        v = c["vs"][B].clone()
+        v[at, 0, 3] = math.nan
+        fill(c["v_pages"], c["prefix_table"], [300], [v])
+        o, lse = (t.cpu() for t in run_attention(c, scale=scale))
+        bad = torch.zeros(B, H, hd, dtype=torch.bool)
+        bad[:, :gqa, 3] = True
+        assert torch.equal(torch.isnan(o), bad), at
+        assert torch.equal(o[~bad], clean[~bad]) and torch.equal(lse, lse0)
