@@ -497,7 +497,7 @@ class PagedDecoder:
             self.place.copy_(self.lens)
         else:
             torch.minimum(self.lens, self.last, out=self.place)
-            torch.where(active, self.lens, self.place, out=self.place)
+            torch.where(active.to(torch.bool), self.lens, self.place, out=self.place)
         if self.device.type != "cuda":
             self.logits = self._step()
         else:
@@ -514,7 +514,7 @@ class PagedDecoder:
                         self.logits = self._step()
                     self.graph = graph  # only a capture that came to its end is replayed
                 self.graph.replay()
-        self.lens.add_(1 if active is None else active.to(torch.int32))
+        self.lens.add_(1 if active is None else active.to(torch.bool))
         return self.logits
 
 

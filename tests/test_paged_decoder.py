@@ -150,3 +150,14 @@ def test_weights_that_change_between_calls():
         assert torch.equal(dec.step(torch.arange(8)), fresh.step(torch.arange(8)))
     want = torch.stack([m(torch.tensor([x]))[0][0, -1] for x in PROMPTS]).repeat_interleave(2, 0)
     assert torch.allclose(dec.start(PROMPTS, 2, 5), want, atol=2e-4, rtol=1e-4)
+
+
+@pytest.mark.parametrize("dtype", [torch.bool, torch.int32, torch.int64, torch.float32])
+def test_flags_of_any_type(dtype):
+    """Whatever is not zero is active, by one token."""
+    dec = PagedDecoder(model(), "cpu", page_size=4)
+    dec.start(PROMPTS, 1, 5)
+    flags = torch.tensor([1, 0, 3, 0]).to(dtype)
+    before = dec.lens.clone()
+    dec.step(torch.arange(4), flags)
+    assert torch.equal(dec.lens - before, torch.tensor([1, 0, 1, 0], dtype=torch.int32))
