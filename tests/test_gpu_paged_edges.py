@@ -157,3 +157,51 @@ def test_one_value_that_is_no_number(B, H, Hkv, hd, scale):
         bad[:, :gqa, 3] = True
         assert torch.equal(torch.isnan(o), bad), at
         assert torch.equal(o[~bad], clean[~bad]) and torch.equal(lse, lse0)
+
+
+@pytest.mark.usefixtures("prefix_room")
+@pytest.mark.parametrize("B,H,Hkv,hd", [(4, 6, 2, 64), (30, 6, 2, 64), (90, 6, 2, 64), (30, 8, 2, 128)])
+@pytest.mark.parametrize("low", [0.0, 1e-8, -math.inf])
+@pytest.mark.parametrize("scale", [1.0, 1e7, 1e10, -1e10])
+def test_scores_that_become_large_on_the_way(B, H, Hkv, hd, low, scale):
+    """Tiles of small scores (or of none: keys that no query can prefer), then tiles whose maximum climbs over every border, then small
+    ones again: each row is its best key's value, or, with a scale of one, what the formula says."""
+    n = 900
+    c = cache_case([3] * B, H, Hkv, hd, 16, prefix_lens=[n], seed=B)
+    c["q"][:, :, 0] = c["q"][:, :, 0].abs() + 0.1
+    keys = c["ks"][B].float()
+    size = torch.ones(n)
+    size[:300], size[300:600], size[700:] = 1e-8, torch.logspace(-8, 0, 300), 1e-3
+    keys = keys * size[:, None, None]
+    if low == 0.0:
+        keys[:300] = 0.0
+    elif low == -math.inf:
+        keys[:300, :, 0] = low if scale > 0 else math.inf
+    c["ks"][B] = keys.bfloat16()
+    for b in range(B):
+        c["ks"][b] = (c["ks"][b].float() * 1e-6).bfloat16()
+    fill(c["k_pages"], c["page_table"], [3] * B, c["ks"][:B])
+    fill(c["k_pages"], c["prefix_table"], [n], [c["ks"][B]])
+    o, lse = run_attention(c, scale=scale)
+    live = c["ks"][B][300:], c["vs"][B][300:]
+    if scale == 1.0:
+        lists = (c["ks"][:B] + [live[0]], c["vs"][:B] + [live[1]]) if low == -math.inf else (c["ks"], c["vs"])
+        check_attention(o, lse, attention_oracle(c["q"], *lists, [0] * B, B, scale=scale), hd)
+        return
+    o, lse = o.double().cpu(), lse.double().cpu()
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+    gqa, sure = H // Hkv, 0
+    for b in range(B):
+        for h in range(H):
+            k = torch.cat((live[0], c["ks"][b]))[:, h // gqa].double()
+            v = torch.cat((live[1], c["vs"][b]))[:, h // gqa].double()
+            q = c["q"][b, h].double()
+            s = k @ q * scale
+            off = (hd + 8) * 2.0**-24 * float((k.abs() @ q.abs()).max()) * abs(scale)
+            best = int(s.argmax())
+            top, second = float(s[best]), float(s.topk(2).values[1])
+            if top - second > 2 * off + 100 and top > 2 * off + 100:  # above the keys of zero as well
+                sure += 1
+                assert abs(float(lse[b, h]) - top) <= off + 2.0**-23 * abs(top) + 13
+                assert ((o[b, h] - v[best]).abs() <= 2.0**-7 * v[best].abs() + 2.0**-40).all()
+    assert sure > B * H // 2
